@@ -415,6 +415,59 @@ int mmsum_decode_self_attn(int dtype, const void* q, long ldq, void* k_cache, vo
                            void* out, long ldo, int rows, int H, int len, int Tmax, float scale, const void* k_new, const void* v_new,
                            long ld_new, void* stream);
 
+/* ---- Tuning from preferences and rewards ---------------------------------------------------------------------------------------
+ * Losses on the log-probability of given tokens.  Rows are positions (r = n T + t of N sequences of T), ld / ldd row pitches in elements;
+ * rows may start at any element (packed [N, T, V] logits with an odd V).  A label outside 0 .. V-1 marks a position that does not count:
+ * its logits are not read, its log-probability is 0 and its gradient a row of zeros.  dlogits [R, W >= V] (pitch ldd) is written whole,
+ * columns V .. W-1 as zeros; it may be the logits themselves (same pitch).  Sums are f32 in a fixed order: results are reproducible.
+ *
+ * logp[r] = log_softmax(logits[r, :V])[labels[r]]; stats (may be NULL): {max, sum of exponentials} of every row, for the backward pass. */
+int mmsum_token_logprob(int dtype, const void* logits, long ld, const int64_t* labels, float* logp, float* stats, int R, int V, void* stream);
+/* dlogits[r] = c ([v == label] - softmax(logits[r])_v), c = coef[r / rows_per_coef] (* *alpha, device f32, may be NULL). */
+int mmsum_token_logprob_bwd(int dtype, const void* logits, long ld, const int64_t* labels, const float* stats, const float* coef, int rows_per_coef,
+                            const float* alpha, void* dlogits, long ldd, int W, int R, int V, void* stream);
+/* out[n] = sum (average: mean, 0 if there is none) of sequence n's counted log-probabilities. */
+int mmsum_sequence_logprob(const float* logp, const int64_t* labels, int N, int T, int V, int average, float* out, void* stream);
+/* Paired preference loss: sequences 0 .. P-1 are the chosen, P .. 2P-1 the rejected ones.  S = sum (average: mean) of a sequence's counted
+ * log-probabilities, ref [2P] the frozen model's (NULL: zeros), h_p = beta ((S_p - ref_p) - (S_{P+p} - ref_{P+p})),
+ * loss = mean_p (1 - smoothing) softplus(-h_p) + smoothing softplus(h_p).
+ * _pairs: from log-probabilities; also seq [2P] = S, margins [P] = h, pair_loss [P], coef [2P] = dloss / d(log-probability of a token of the
+ * sequence) for mmsum_token_logprob_bwd with rows_per_coef = T.  _loss: logits to gradient; workspace: mmsum_preference_workspace bytes. */
+int mmsum_preference_pairs(const float* logp, const int64_t* labels, const float* ref, int P, int T, int V, float beta, float smoothing, int average,
+                           float* seq, float* margins, float* pair_loss, float* coef, float* loss, void* stream);
+long mmsum_preference_workspace(int P, int T);
+int mmsum_preference_loss(int dtype, const void* logits, long ld, const int64_t* labels, const float* ref, int P, int T, int V, float beta, float smoothing,
+                          int average, float* loss, float* margins, float* seq, void* dlogits, long ldd, int W, void* workspace, void* stream);
+/* Clipped policy loss with a KL term: ratio = exp(logp - old_logp), A = adv[row] (adv_per_token) or adv[sequence],
+ * token loss = max(-A ratio, -A min(max(ratio, 1 - clip_low), 1 + clip_high)) + kl_coef kl, kl = e^d - d - 1 with d = ref_logp - logp (ref_logp NULL:
+ * none); mean over the counted tokens, or (seq_mean) over the sequences of the mean over a sequence's counted tokens (an empty one counts 0).
+ * out [3] = {loss, the same mean of kl, the same mean of [the bounded branch is the larger]}.  old_logp, ref_logp [N T].
+ * _terms: from log-probabilities, coef [N T] for mmsum_token_logprob_bwd with rows_per_coef = 1.  _loss: logits to gradient with the logits read
+ * once; logp [N T].  workspace: mmsum_policy_workspace bytes. */
+long mmsum_policy_workspace(int N, int T);
+int mmsum_policy_terms(const float* logp, const int64_t* labels, const float* old_logp, const float* ref_logp, const float* adv, int adv_per_token, int N,
+                       int T, int V, float clip_low, float clip_high, float kl_coef, int seq_mean, float* out, float* coef, void* workspace, void* stream);
+int mmsum_policy_loss(int dtype, const void* logits, long ld, const int64_t* labels, const float* old_logp, const float* ref_logp, const float* adv,
+                      int adv_per_token, int N, int T, int V, float clip_low, float clip_high, float kl_coef, int seq_mean, float* out, float* logp,
+                      void* dlogits, long ldd, int W, void* workspace, void* stream);
+
+/* Embedding lookup with scaling: y[i] = scale E[ids[i]] (one rounding); ids outside 0 .. V-1 give zero rows. */
+int mmsum_embed_fwd(int dtype, const int64_t* ids, const void* E, long lde, void* y, long ldy, long n, int V, int D, float scale, void* stream);
+/* dE[v] (+)= scale sum of dy[i] over ids[i] == v, f32 [V, D] packed, written whole unless `accumulate` (then only rows that ids name change).  By
+ * sorted tokens, without floating-point atomics: reproducible.  ids outside 0 .. V-1 and pad_id (-1: none) leave no gradient.
+ * workspace: mmsum_embed_bwd_workspace bytes; n < 2^30. */
+long mmsum_embed_bwd_workspace(long n, int D);
+int mmsum_embed_bwd(int dtype, const void* dy, long lddy, const int64_t* ids, long n, int V, int D, float scale, int64_t pad_id, int accumulate, float* dE,
+                    void* workspace, void* stream);
+
+/* 8-bit integer products (inference): q [M, ldq] = 127 x / max |x| of the row, rounded to the nearest (ties to even), columns K .. ldq-1 zero;
+ * scale [M] = max |x| / 127.  A row with a value that is not finite gets a scale that is not finite.  ldq a multiple of 64, q 16-byte aligned. */
+int mmsum_quantize_i8(int dtype, const void* x, long ldx, int M, int K, void* q, long ldq, float* scale, void* stream);
+/* y[m][n] = sx[m] sw[n] sum_k qx[m][k] qw[n][k] (+ bias[n], f32, may be NULL) (gelu: erf form).  The sum is exact.  K (padded with zeros) a multiple of
+ * 64, at most 131,072; pitches in bytes, multiples of 16; qx, qw 16-byte aligned. */
+int mmsum_gemm_i8(const void* qx, long ldx, const float* sx, const void* qw, long ldw, const float* sw, const float* bias, int dtype_out, void* y, long ldy,
+                  int M, int N, int K, int gelu, void* stream);
+
 #pragma GCC visibility pop
 #ifdef __cplusplus
 }

@@ -122,6 +122,21 @@ SIGNATURES = {
                                 c_void_p, c_void_p, c_int, c_float, c_int, c_int, c_void_p]),
     "mmsum_decode_self_attn": (c_int, [c_int, c_void_p, c_long, c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_long, c_int, c_int, c_int,
                                        c_int, c_float, c_void_p, c_void_p, c_long, c_void_p]),
+    "mmsum_token_logprob": (c_int, [c_int, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "mmsum_token_logprob_bwd": (c_int, [c_int, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_void_p]),
+    "mmsum_sequence_logprob": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "mmsum_preference_pairs": (c_int, [c_void_p] * 3 + [c_int] * 3 + [c_float, c_float, c_int] + [c_void_p] * 6),
+    "mmsum_preference_workspace": (c_long, [c_int, c_int]),
+    "mmsum_preference_loss": (c_int, [c_int, c_void_p, c_long, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_float, c_int, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_long, c_int, c_void_p, c_void_p]),
+    "mmsum_policy_workspace": (c_long, [c_int, c_int]),
+    "mmsum_policy_terms": (c_int, [c_void_p] * 5 + [c_int] * 4 + [c_float] * 3 + [c_int] + [c_void_p] * 4),
+    "mmsum_policy_loss": (c_int, [c_int, c_void_p, c_long] + [c_void_p] * 4 + [c_int] * 4 + [c_float] * 3 + [c_int] + [c_void_p] * 3 + [c_long, c_int, c_void_p, c_void_p]),
+    "mmsum_embed_fwd": (c_int, [c_int, c_void_p, c_void_p, c_long, c_void_p, c_long, c_long, c_int, c_int, c_float, c_void_p]),
+    "mmsum_embed_bwd_workspace": (c_long, [c_long, c_int]),
+    "mmsum_embed_bwd": (c_int, [c_int, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_float, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
+    "mmsum_quantize_i8": (c_int, [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_long, c_void_p, c_void_p]),
+    "mmsum_gemm_i8": (c_int, [c_void_p, c_long, c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_int, c_void_p, c_long, c_int, c_int, c_int, c_int, c_void_p]),
 }
 
 

@@ -1,0 +1,441 @@
+// Embedding lookup with scaling, y[i] = scale E[ids[i]], and the table's gradient dE[v] = scale sum of dy[i] over ids[i] == v.
+//
+// The gradient goes by SORTED tokens: a stable radix sort brings equal ids together in batch order, fixed stretches of the sorted list
+// are summed each by one wave, and a token's stretches are added in order -- no floating-point atomics, so a gradient is the same bit
+// for bit on every run, and a frequent token (padding excluded, still a few percent of a text) is summed by many waves at once.
+// Ids outside 0 .. V-1 read as zero rows and leave no gradient, and so does pad_id in the gradient.
+// Bound: HBM (dy once, dE once).
+#include "mmsum_device.h"
+#include "mmsum_kernels.h"
+
+namespace {
+
+inline int ok() { return hipGetLastError() == hipSuccess ? MMSUM_OK : MMSUM_ERR_HIP; }
+
+// ---- lookup ------------------------------------------------------------------------------------------------------------------------
+// VEC elements a thread and step; tpr threads a row (a power of two <= 256), 256 / tpr rows at a time, ROWS of them in flight
+template <typename T, int VEC> struct Vec;
+template <> struct Vec<bf16_t, 8> { typedef u32x4_t type; };
+template <> struct Vec<float, 4> { typedef u32x4_t type; };
+template <> struct Vec<bf16_t, 1> { typedef bf16_t type; };
+template <> struct Vec<float, 1> { typedef float type; };
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void embed_fwd_kernel(const int64_t* __restrict__ ids, const T* __restrict__ E, long lde, T* __restrict__ y, long ldy, long n,
+                                                        int V, int D, float scale, int tpr_log2) {
+    constexpr int ROWS = 4;
+    const int tpr = 1 << tpr_log2, rpb = 256 >> tpr_log2;
+    const int c0 = ((int)threadIdx.x & (tpr - 1)) * VEC;
+    const long r0 = (long)blockIdx.x * (rpb * ROWS) + (threadIdx.x >> tpr_log2);
+    int64_t id[ROWS];
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) id[j] = r0 + j * rpb < n ? ids[r0 + j * rpb] : -1;
+    for (int c = c0; c < D; c += tpr * VEC) {
+        typename Vec<T, VEC>::type v[ROWS];
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j)
+            if (id[j] >= 0 && id[j] < V) v[j] = *reinterpret_cast<const typename Vec<T, VEC>::type*>(E + (long)id[j] * lde + c);
+            else v[j] = typename Vec<T, VEC>::type{};
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j)
+            if (r0 + j * rpb < n) {
+                T t[VEC];
+                __builtin_memcpy(t, &v[j], sizeof(t));
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) t[k] = from_f32<T>(to_f32(t[k]) * scale);
+                __builtin_memcpy(&v[j], t, sizeof(t));
+                *reinterpret_cast<typename Vec<T, VEC>::type*>(y + (r0 + j * rpb) * ldy + c) = v[j];
+            }
+    }
+}
+
+// ---- sort --------------------------------------------------------------------------------------------------------------------------
+// Least-significant-digit radix sort of (key, position), 8 bits a pass.  A key is the id, or V for a position without a gradient (sorted
+// behind every id).  A pass is stable: within a tile a wave's rounds keep their order, tiles keep theirs.
+__device__ __forceinline__ uint32_t key_of(int64_t id, int V, int64_t pad_id) { return id >= 0 && id < V && id != pad_id ? (uint32_t)id : (uint32_t)V; }
+
+// lanes of the wave whose digit equals this lane's (among the `act` lanes)
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, uint64_t act) {
+    uint64_t m = act;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const uint64_t v = __ballot((d >> b) & 1);
+        m &= (d >> b) & 1 ? v : ~v;
+    }
+    return m;
+}
+
+// One round: every active lane of the wave gets its rank among the equal digits this wave has met (cnt: the wave's 256 counters)
+__device__ __forceinline__ int wave_rank(volatile int* cnt, uint32_t d, bool active, int lane) {
+    const uint64_t act = __ballot(active);
+    const uint64_t same = same_digit(d, act);
+    int base = 0;
+    if (active) base = cnt[d];
+    __builtin_amdgcn_wave_barrier();
+    const int before = __popcll(same & ((1ull << lane) - 1));
+    if (active && before == 0) cnt[d] = base + __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+    return base + before;
+}
+
+constexpr int kSub = 1024;               // elements a workgroup ranks at a time (four rounds of its four waves)
+constexpr int kMaxTiles = 256;
+
+// hist[tile][256]: digits of every tile
+template <bool FIRST>
+__global__ __launch_bounds__(256) void sort_hist_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys, int n, int tile, int V, int64_t pad_id, int shift,
+                                                        int* __restrict__ hist) {
+    __shared__ int h[256];
+    h[threadIdx.x] = 0;
+    __syncthreads();
+    const long lo = (long)blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n;
+    for (long i = lo + threadIdx.x; i < hi; i += 256) atomicAdd(&h[((FIRST ? key_of(ids[i], V, pad_id) : keys[i]) >> shift) & 255], 1);
+    __syncthreads();
+    hist[blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
+}
+
+// moves a tile's elements to their places: in front of a digit's elements of this tile come all smaller digits and the earlier tiles' equal ones
+template <bool FIRST>
+__global__ __launch_bounds__(256) void sort_scatter_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys, const int* __restrict__ pos, int n, int tile,
+                                                           int tiles, int V, int64_t pad_id, int shift, const int* __restrict__ hist, uint32_t* __restrict__ okeys,
+                                                           int* __restrict__ opos) {
+    __shared__ int cnt[4][256], wbase[4][256], scan[256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int total = 0, before = 0;
+    for (int t = 0; t < tiles; ++t) {
+        const int v = hist[t * 256 + tid];
+        before += t < (int)blockIdx.x ? v : 0;
+        total += v;
+    }
+    scan[tid] = total;
+    __syncthreads();
+    for (int o = 1; o < 256; o <<= 1) {                           // inclusive scan over the digits
+        const int v = tid >= o ? scan[tid - o] : 0;
+        __syncthreads();
+        scan[tid] += v;
+        __syncthreads();
+    }
+    int off = scan[tid] - total + before;                          // this digit's next place
+    const long lo = (long)blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n;
+    for (long base = lo; base < hi; base += kSub) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) cnt[w][tid] = 0;
+        __syncthreads();
+        uint32_t key[4];
+        int rank[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const long i = base + wave * 256 + r * 64 + lane;
+            const bool act = i < hi;
+            key[r] = act ? (FIRST ? key_of(ids[i], V, pad_id) : keys[i]) : 0u;
+            rank[r] = wave_rank(cnt[wave], (key[r] >> shift) & 255, act, lane);
+        }
+        __syncthreads();
+        {
+            int o = off;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) { wbase[w][tid] = o; o += cnt[w][tid]; }
+            off = o;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const long i = base + wave * 256 + r * 64 + lane;
+            if (i < hi) {
+                const int p = wbase[wave][(key[r] >> shift) & 255] + rank[r];
+                okeys[p] = key[r];
+                opos[p] = FIRST ? (int)i : pos[i];
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// the whole sort of up to 4096 ids in one workgroup's LDS
+constexpr int kSmall = 4096;
+__global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restrict__ ids, int n, int V, int64_t pad_id, int bits, uint32_t* __restrict__ okeys, int* __restrict__ opos) {
+    __shared__ uint32_t lk[2][kSmall];
+    __shared__ uint16_t lp[2][kSmall];
+    __shared__ int cnt[16][256];
+    __shared__ int scan[256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int i = tid; i < n; i += 1024) { lk[0][i] = key_of(ids[i], V, pad_id); lp[0][i] = (uint16_t)i; }
+    int cur = 0;
+    for (int shift = 0; shift < bits; shift += 8) {
+        for (int i = tid; i < 16 * 256; i += 1024) (&cnt[0][0])[i] = 0;
+        __syncthreads();
+        uint32_t key[4];
+        int rank[4], p[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = wave * 256 + r * 64 + lane;
+            const bool act = i < n;
+            key[r] = act ? lk[cur][i] : 0u;
+            p[r] = act ? lp[cur][i] : 0;
+            rank[r] = wave_rank(cnt[wave], (key[r] >> shift) & 255, act, lane);
+        }
+        __syncthreads();
+        int total = 0;
+        if (tid < 256) {
+            for (int w = 0; w < 16; ++w) { const int v = cnt[w][tid]; cnt[w][tid] = total; total += v; }
+            scan[tid] = total;
+        }
+        __syncthreads();
+        for (int o = 1; o < 256; o <<= 1) {
+            const int v = tid < 256 && tid >= o ? scan[tid - o] : 0;
+            __syncthreads();
+            if (tid < 256) scan[tid] += v;
+            __syncthreads();
+        }
+        if (tid < 256) scan[tid] -= total;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (wave * 256 + r * 64 + lane < n) {
+                const int d = (key[r] >> shift) & 255, o = scan[d] + cnt[wave][d] + rank[r];
+                lk[cur ^ 1][o] = key[r];
+                lp[cur ^ 1][o] = (uint16_t)p[r];
+            }
+        cur ^= 1;
+        __syncthreads();
+    }
+    for (int i = tid; i < n; i += 1024) { okeys[i] = lk[cur][i]; opos[i] = lp[cur][i]; }
+}
+
+// ---- sums --------------------------------------------------------------------------------------------------------------------------
+// A wave sums a stretch of kStretch sorted positions over 512 columns (eight a lane).  A token whose positions all lie in the stretch is
+// finished; a token that crosses its ends leaves partial sums: part[stretch][0] of the one that began before it, part[stretch][1] of the
+// one that begins in it and goes on (stretch_join_kernel adds those up).
+constexpr int kStretch = 32, kCols = 512;
+
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* __restrict__ row, int c, int D, int lane, float (&f)[8]) {
+    if constexpr (VEC) {
+        if (c < D) {
+            if constexpr (sizeof(T) == 2) {
+                T t[8];
+                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(row + c);
+                __builtin_memcpy(t, &v, 16);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) f[k] = to_f32(t[k]);
+            } else {
+                const f32x4_t a = *reinterpret_cast<const f32x4_t*>(row + c), b = *reinterpret_cast<const f32x4_t*>(row + c + 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { f[k] = a[k]; f[4 + k] = b[k]; }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (c + k * 64 < D) f[k] = to_f32(row[c + k * 64]);
+    }
+}
+// column of element k of a lane: VEC: eight neighbours; else: strided by 64 lanes
+template <bool VEC> __device__ __forceinline__ int col_of(int c, int k) { return VEC ? c + k : c + k * 64; }
+template <bool VEC> __device__ __forceinline__ void store8(float* __restrict__ row, int c, int D, const float (&f)[8], float scale, bool accumulate) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int cc = col_of<VEC>(c, k);
+        if (cc < D) row[cc] = accumulate ? row[cc] + scale * f[k] : scale * f[k];
+    }
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void stretch_sum_kernel(const T* __restrict__ dy, long lddy, const uint32_t* __restrict__ keys, const int* __restrict__ pos, int n, int V, int D,
+                                                          float scale, int accumulate, float* __restrict__ part, float* __restrict__ dE) {
+    const int lane = threadIdx.x & 63;
+    const long st = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long lo = st * kStretch;
+    if (lo >= n) return;
+    const int len = (int)(n - lo < kStretch ? n - lo : kStretch);
+    const int col0 = blockIdx.y * kCols, c = VEC ? col0 + lane * 8 : col0 + lane;
+    const int Dc = VEC ? D : (D < col0 + kCols ? D : col0 + kCols);
+    // the stretch's keys and positions ride on the lanes; lanes 62 / 63 hold the neighbours in front and behind
+    uint32_t k = (uint32_t)V;
+    int p = 0;
+    if (lane < len) { k = keys[lo + lane]; p = pos[lo + lane]; }
+    if (lane == 62 && lo > 0) k = keys[lo - 1];
+    if (lane == 63 && lo + len < n) k = keys[lo + len];
+    const uint32_t kbefore = lo > 0 ? (uint32_t)__builtin_amdgcn_readlane(k, 62) : 0xffffffffu;
+    const uint32_t kbehind = lo + len < n ? (uint32_t)__builtin_amdgcn_readlane(k, 63) : 0xffffffffu;
+    float acc[8] = {};
+    constexpr int AHEAD = 8;
+    float f[AHEAD][8];
+    bool open = false;                                             // the current token began before the stretch
+    for (int i0 = 0; i0 < len; i0 += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (i0 + u < len && (uint32_t)__builtin_amdgcn_readlane(k, i0 + u) < (uint32_t)V) load8<T, VEC>(dy + (long)__builtin_amdgcn_readlane(p, i0 + u) * lddy, c, Dc, lane, f[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = i0 + u;
+            if (i >= len) break;
+            const uint32_t key = __builtin_amdgcn_readlane(k, i);
+            if (key >= (uint32_t)V) return;                        // sorted behind every id: nothing more to sum
+            const uint32_t prev = i > 0 ? (uint32_t)__builtin_amdgcn_readlane(k, i - 1) : kbefore;
+            const uint32_t next = i + 1 < len ? (uint32_t)__builtin_amdgcn_readlane(k, i + 1) : kbehind;
+            if (i == 0) open = key == prev;
+            else if (key != prev) open = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = key != prev || i == 0 ? f[u][e] : acc[e] + f[u][e];
+            if (key != next || i + 1 == len) {
+                const bool goes_on = key == next;
+                if (!open && !goes_on) store8<VEC>(dE + (long)key * D, c, Dc, acc, scale, accumulate != 0);
+                else store8<VEC>(part + (st * 2 + (open ? 0 : 1)) * D, c, Dc, acc, 1.f, false);
+            }
+        }
+    }
+}
+
+// A token that begins in stretch st and goes on: part[st][1] + part[st + 1][0] + ... in order.  Four waves take every fourth stretch, so
+// that a token of many stretches is read four at a time; their sums are added in wave order.
+__global__ __launch_bounds__(256) void stretch_join_kernel(const uint32_t* __restrict__ keys, int n, int V, int D, float scale, int accumulate, const float* __restrict__ part,
+                                                           float* __restrict__ dE) {
+    __shared__ float sh[4][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long st = blockIdx.x, end = (st + 1) * kStretch;          // end < n: the grid leaves the last stretch out
+    const uint32_t key = keys[end - 1];
+    if (key >= (uint32_t)V || keys[end] != key) return;
+    if (keys[st * kStretch] == key && st > 0 && keys[st * kStretch - 1] == key) return;      // began earlier
+    // last stretch of the token: the first position behind it, by bisection
+    long a = end, b = n;
+    while (a < b) {
+        const long mid = (a + b) / 2;
+        if (keys[mid] == key) a = mid + 1;
+        else b = mid;
+    }
+    const long last = (a - 1) / kStretch;
+    const int c = blockIdx.y * 256 + lane * 4;
+    float acc[4] = {};
+    for (long q = st + wave; q <= last; q += 4) {
+        const float* row = part + (q * 2 + (q == st ? 1 : 0)) * D;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < D) acc[e] += row[c + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sh[wave][lane * 4 + e] = acc[e];
+    __syncthreads();
+    const int col = blockIdx.y * 256 + threadIdx.x;
+    if (col < D) {
+        const float s = scale * ((sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]));
+        float* const o = dE + (long)key * D + col;
+        *o = accumulate ? *o + s : s;
+    }
+}
+
+// rows of the table that no token of the batch names: zeros.  A wave takes 16 neighbouring rows, its lanes bisect the sorted keys for them.
+__global__ __launch_bounds__(256) void absent_rows_kernel(const uint32_t* __restrict__ keys, int n, int V, int D, float* __restrict__ dE) {
+    const int lane = threadIdx.x & 63;
+    const long v0 = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16;
+    if (v0 >= V) return;
+    const uint32_t v = (uint32_t)(v0 + (lane & 15));
+    int a = 0, b = n;
+    while (a < b) {
+        const int mid = (int)(((long)a + b) / 2);
+        if (keys[mid] < v) a = mid + 1;
+        else b = mid;
+    }
+    const uint64_t absent = __ballot(!(a < n && keys[a] == v));
+    for (int r = 0; r < 16 && v0 + r < V; ++r) {
+        if (!((absent >> r) & 1)) continue;
+        float* const row = dE + (v0 + r) * D;
+        if (D % 4 == 0 && ((uintptr_t)dE & 15) == 0) {
+            for (int c = lane * 4; c < D; c += 256) *reinterpret_cast<f32x4_t*>(row + c) = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        } else {
+            for (int c = lane; c < D; c += 64) row[c] = 0.f;
+        }
+    }
+}
+
+template <typename T>
+int embed_fwd_t(const int64_t* ids, const void* E, long lde, void* y, long ldy, long n, int V, int D, float scale, hipStream_t s) {
+    constexpr int VEC = 16 / sizeof(T);
+    const bool vec = D % VEC == 0 && lde % VEC == 0 && ldy % VEC == 0 && (((uintptr_t)E | (uintptr_t)y) & 15) == 0;
+    const int steps = vec ? D / VEC : D;
+    int lg = 0;
+    while ((1 << lg) < steps && lg < 8) ++lg;
+    const long blocks = (n + 4 * (256 >> lg) - 1) / (4 * (256 >> lg));
+    if (blocks > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    if (vec) hipLaunchKernelGGL((embed_fwd_kernel<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, ids, (const T*)E, lde, (T*)y, ldy, n, V, D, scale, lg);
+    else hipLaunchKernelGGL((embed_fwd_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, s, ids, (const T*)E, lde, (T*)y, ldy, n, V, D, scale, lg);
+    return ok();
+}
+
+struct SortPlan { int tile, tiles; };
+SortPlan sort_plan(int n) {
+    const int subs = (int)(((long)n + kSub - 1) / kSub), per = (subs + kMaxTiles - 1) / kMaxTiles;
+    return SortPlan{per * kSub, (subs + per - 1) / per};
+}
+long align16(long b) { return (b + 15) & ~15L; }
+
+template <typename T>
+int embed_bwd_t(const void* dy, long lddy, const int64_t* ids, int n, int V, int D, float scale, int64_t pad_id, int accumulate, float* dE, char* ws, hipStream_t s) {
+    const long nb = align16((long)n * 4);
+    uint32_t* k0 = reinterpret_cast<uint32_t*>(ws);
+    int* p0 = reinterpret_cast<int*>(ws + nb);
+    uint32_t* k1 = reinterpret_cast<uint32_t*>(ws + 2 * nb);
+    int* p1 = reinterpret_cast<int*>(ws + 3 * nb);
+    int* hist = reinterpret_cast<int*>(ws + 4 * nb);
+    float* part = reinterpret_cast<float*>(ws + 4 * nb + kMaxTiles * 256 * 4);
+    int bits = 0;
+    while (bits < 32 && ((uint32_t)V >> bits) != 0) ++bits;
+    if (n <= kSmall) {
+        hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(1024), 0, s, ids, n, V, pad_id, bits, k0, p0);
+    } else {
+        const SortPlan sp = sort_plan(n);
+        for (int shift = 0; shift < bits; shift += 8) {
+            if (shift == 0) {
+                hipLaunchKernelGGL((sort_hist_kernel<true>), dim3(sp.tiles), dim3(256), 0, s, ids, nullptr, n, sp.tile, V, pad_id, shift, hist);
+                hipLaunchKernelGGL((sort_scatter_kernel<true>), dim3(sp.tiles), dim3(256), 0, s, ids, nullptr, nullptr, n, sp.tile, sp.tiles, V, pad_id, shift, hist, k0, p0);
+            } else {
+                hipLaunchKernelGGL((sort_hist_kernel<false>), dim3(sp.tiles), dim3(256), 0, s, ids, k0, n, sp.tile, V, pad_id, shift, hist);
+                hipLaunchKernelGGL((sort_scatter_kernel<false>), dim3(sp.tiles), dim3(256), 0, s, ids, k0, p0, n, sp.tile, sp.tiles, V, pad_id, shift, hist, k1, p1);
+                uint32_t* tk = k0; k0 = k1; k1 = tk;
+                int* tp = p0; p0 = p1; p1 = tp;
+            }
+        }
+    }
+    const long stretches = ((long)n + kStretch - 1) / kStretch;
+    const unsigned cols = (unsigned)((D + kCols - 1) / kCols);
+    const bool vec = D % 8 == 0 && lddy % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)dy & 15) == 0;
+    const dim3 grid((unsigned)((stretches + 3) / 4), cols);
+    if (vec) hipLaunchKernelGGL((stretch_sum_kernel<T, true>), grid, dim3(256), 0, s, (const T*)dy, lddy, k0, p0, n, V, D, scale, accumulate, part, dE);
+    else hipLaunchKernelGGL((stretch_sum_kernel<T, false>), grid, dim3(256), 0, s, (const T*)dy, lddy, k0, p0, n, V, D, scale, accumulate, part, dE);
+    const long joins = ((long)n - 1) / kStretch;                    // stretches with another one behind them
+    if (joins > 0) hipLaunchKernelGGL(stretch_join_kernel, dim3((unsigned)joins, (unsigned)((D + 255) / 256)), dim3(256), 0, s, k0, n, V, D, scale, accumulate, part, dE);
+    if (!accumulate) hipLaunchKernelGGL(absent_rows_kernel, dim3((unsigned)((V + 63L) / 64)), dim3(256), 0, s, k0, n, V, D, dE);
+    return ok();
+}
+
+__global__ __launch_bounds__(256) void zero_kernel(float* __restrict__ p, long n) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) p[i] = 0.f;
+}
+
+}  // namespace
+
+extern "C" int mmsum_embed_fwd(int dtype, const int64_t* ids, const void* E, long lde, void* y, long ldy, long n, int V, int D, float scale, void* stream) {
+    if (n <= 0 || V <= 0 || D <= 0 || lde < D || ldy < D) return MMSUM_ERR_BAD_SHAPE;
+    if (dtype == MMSUM_BF16) return ((uintptr_t)E | (uintptr_t)y) & 1 ? MMSUM_ERR_BAD_ALIGN : embed_fwd_t<bf16_t>(ids, E, lde, y, ldy, n, V, D, scale, (hipStream_t)stream);
+    if (dtype == MMSUM_F32) return ((uintptr_t)E | (uintptr_t)y) & 3 ? MMSUM_ERR_BAD_ALIGN : embed_fwd_t<float>(ids, E, lde, y, ldy, n, V, D, scale, (hipStream_t)stream);
+    return MMSUM_ERR_BAD_DTYPE;
+}
+
+extern "C" long mmsum_embed_bwd_workspace(long n, int D) {
+    if (n < 0 || n > 0x3fffffffL || D <= 0) return 0;
+    return 4 * align16(n * 4) + kMaxTiles * 256 * 4 + (n + kStretch - 1) / kStretch * 2 * D * (long)sizeof(float);
+}
+extern "C" int mmsum_embed_bwd(int dtype, const void* dy, long lddy, const int64_t* ids, long n, int V, int D, float scale, int64_t pad_id, int accumulate, float* dE,
+                               void* workspace, void* stream) {
+    if (n < 0 || n > 0x3fffffffL || V <= 0 || V > 0x7ffffff0 || D <= 0 || lddy < D) return MMSUM_ERR_BAD_SHAPE;
+    if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
+    if (n > 0 && workspace == nullptr) return MMSUM_ERR_WORKSPACE;
+    if (((uintptr_t)workspace & 15) || ((uintptr_t)dE & 3) || ((uintptr_t)dy & (dtype == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
+    hipStream_t s = (hipStream_t)stream;
+    if (n == 0) {
+        if (!accumulate) hipLaunchKernelGGL(zero_kernel, dim3(2048), dim3(256), 0, s, dE, (long)V * D);
+        return ok();
+    }
+    if (dtype == MMSUM_BF16) return embed_bwd_t<bf16_t>(dy, lddy, ids, (int)n, V, D, scale, pad_id, accumulate, dE, static_cast<char*>(workspace), s);
+    return embed_bwd_t<float>(dy, lddy, ids, (int)n, V, D, scale, pad_id, accumulate, dE, static_cast<char*>(workspace), s);
+}

@@ -1,0 +1,558 @@
+// Losses on the log-probabilities of given tokens: scoring, the paired preference loss, the clipped policy loss with a KL term.
+//
+// A row is one position's V logits x, y its label; m = max x, s = sum exp(x - m):
+//   log p(y) = (x_y - m) - log s          d log p(y) / d x_v = [v == y] - exp(x_v - m) / s
+// so every loss here is a number c = dL / d log p(y) per row, and its gradient is c ([v == y] - exp(x_v - m) / s).  A label outside
+// 0 .. V-1 marks a position that does not count: log p = 0, c = 0, a row of zeros, and its logits are not read.
+//
+// Bound: HBM.  The policy loss knows c as soon as the row's own log p is known, so its kernel reads the logits once and writes the
+// gradient once, the row waiting in registers in between.  The preference loss needs the sums over both summaries of a pair first:
+// statistics (read), pairs, gradient (read, write).
+// Everything is summed in f32, in an order that depends on the sizes alone.
+#include "mmsum_device.h"
+#include "mmsum_kernels.h"
+
+namespace {
+
+inline int ok() { return hipGetLastError() == hipSuccess ? MMSUM_OK : MMSUM_ERR_HIP; }
+
+// 16 bytes of a row that starts at any element: packed [N, T, V] logits with an odd V have rows at odd multiples of the element size
+template <typename T> struct Chunk;
+template <> struct Chunk<bf16_t> { typedef u32x4_t type __attribute__((aligned(2))); };
+template <> struct Chunk<float> { typedef u32x4_t type __attribute__((aligned(4))); };
+template <typename T> constexpr int kPer = 16 / (int)sizeof(T);
+
+// columns [c, c + kPer) of a row, -inf behind V (adds nothing to a maximum or a sum of exponentials)
+template <typename T> __device__ __forceinline__ u32x4_t load_chunk(const T* x, int c, int V) {
+    if (c + kPer<T> <= V) return *reinterpret_cast<const typename Chunk<T>::type*>(x + c);
+    T t[kPer<T>];
+#pragma unroll
+    for (int k = 0; k < kPer<T>; ++k) t[k] = c + k < V ? x[c + k] : from_f32<T>(-INFINITY);
+    u32x4_t r;
+    __builtin_memcpy(&r, t, 16);
+    return r;
+}
+template <typename T> __device__ __forceinline__ void unpack(const u32x4_t& r, float (&f)[kPer<T>]) {
+    T t[kPer<T>];
+    __builtin_memcpy(t, &r, 16);
+#pragma unroll
+    for (int k = 0; k < kPer<T>; ++k) f[k] = to_f32(t[k]);
+}
+template <typename T> __device__ __forceinline__ void store_chunk(T* d, int c, int V, const float (&g)[kPer<T>]) {
+    T t[kPer<T>];
+#pragma unroll
+    for (int k = 0; k < kPer<T>; ++k) t[k] = from_f32<T>(g[k]);
+    if (c + kPer<T> <= V) {
+        u32x4_t r;
+        __builtin_memcpy(&r, t, 16);
+        *reinterpret_cast<typename Chunk<T>::type*>(d + c) = r;
+    } else {
+#pragma unroll
+        for (int k = 0; k < kPer<T>; ++k)
+            if (c + k < V) d[c + k] = t[k];
+    }
+}
+// bf16 results keep 8 bits: the hardware exponential (2^-22) is exact enough; f32 rows take the library's expf
+template <typename T> __device__ __forceinline__ float row_exp(float d) { return sizeof(T) == 2 ? __expf(d) : expf(d); }
+
+template <int NT> __device__ __forceinline__ float block_max(float v, float* sh) {
+    v = warp_max(v);
+    if constexpr (NT == 64) return v;
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, sh[w]);
+    return v;
+}
+template <int NT> __device__ __forceinline__ float block_sum(float v, float* sh) {
+    v = warp_sum(v);
+    if constexpr (NT == 64) return v;
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v += sh[w];
+    return v;
+}
+
+// What the policy loss takes per token besides the logits
+struct PolicyArgs {
+    const float* old_logp; const float* ref_logp; const float* adv;
+    const int* counts;              // counted tokens: of kCountParts stretches of the batch (token mean) or of every sequence (sequence mean)
+    int adv_per_token, seq_mean, N, T;
+    float lo, hi, kl_coef;
+    float* terms;                   // [3][R]: weighted loss, KL estimate, clipped indicator of every row
+};
+constexpr int kCountParts = 64;
+
+__device__ __forceinline__ float policy_weight(const PolicyArgs& p, int row, int lane) {
+    if (p.seq_mean) return 1.f / (fmaxf((float)p.counts[row / p.T], 1.f) * (float)p.N);
+    int n = p.counts[lane];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    return 1.f / fmaxf((float)n, 1.f);
+}
+// loss = max(-A r, -A clip(r, lo, hi)) + kl (e^d - d - 1) with r = exp(log p - old), d = ref - log p; returns dL / d log p.
+// The bounded branch carries no gradient; the KL estimate (non-negative, unbiased under the sampling policy) gives 1 - e^d.
+__device__ __forceinline__ float policy_token(const PolicyArgs& p, int row, float lp, float w, float (&t)[3]) {
+    const float ratio = expf(lp - p.old_logp[row]);
+    const float a = p.adv[p.adv_per_token ? row : row / p.T];
+    const float l1 = -a * ratio, l2 = -a * fminf(fmaxf(ratio, p.lo), p.hi);
+    float loss = l1 >= l2 ? l1 : l2, d = l1 >= l2 ? l1 : 0.f, kl = 0.f;
+    if (l1 != l1 || l2 != l2) loss = d = l1 + l2;                        // NaN in, NaN out: a comparison would lose it
+    if (p.ref_logp != nullptr) {
+        const float g = p.ref_logp[row] - lp, e = expf(g);
+        kl = expm1f(g) - g;
+        loss += p.kl_coef * kl;
+        d += p.kl_coef * (1.f - e);
+    }
+    t[0] = w * loss;
+    t[1] = w * kl;
+    t[2] = l1 < l2 ? w : 0.f;
+    return w * d;
+}
+
+template <typename T> struct RowArgs {
+    const T* logits; long ld; const int64_t* labels; int V;
+    float* logp; float* stats;      // stats [R][2] = {m, s}; may be NULL
+    T* dlogits; long ldd; int W;
+    int row0, n0, row1;             // block b works on row row0 + b, from the n0-th on row1 + (b - n0)
+    PolicyArgs pol;
+};
+
+template <typename T, int NT> __device__ __forceinline__ void zero_cols(T* d, int lo, int hi) {
+    for (int c = lo + (int)threadIdx.x; c < hi; c += NT) d[c] = from_f32<T>(0.f);
+}
+
+// One workgroup a row, the row in MAXC 16-byte chunks per thread: requested together, kept as loaded (packed), swept for the maximum,
+// for the sum and, for the policy loss, for the gradient.
+template <typename T, int NT, int MAXC, bool POLICY>
+__global__ __launch_bounds__(NT) void row_kernel(RowArgs<T> a) {
+    __shared__ float sh[2][NT / 64];
+    const int tid = threadIdx.x, b = blockIdx.x;
+    const int row = b < a.n0 ? a.row0 + b : a.row1 + (b - a.n0);
+    const int64_t y = a.labels[row];
+    T* const d = POLICY ? a.dlogits + (long)row * a.ldd : nullptr;
+    if (y < 0 || y >= a.V) {
+        if (tid == 0) {
+            a.logp[row] = 0.f;
+            if (a.stats) { a.stats[2 * (long)row] = 0.f; a.stats[2 * (long)row + 1] = 1.f; }
+            if constexpr (POLICY) {
+                const long R = (long)a.pol.N * a.pol.T;
+                a.pol.terms[row] = a.pol.terms[R + row] = a.pol.terms[2 * R + row] = 0.f;
+            }
+        }
+        if constexpr (POLICY) {
+            const float z[kPer<T>] = {};
+            for (int c = tid * kPer<T>; c < a.W; c += NT * kPer<T>) store_chunk(d, c, a.W, z);
+        }
+        return;
+    }
+    const T* x = a.logits + (long)row * a.ld;                       // no __restrict__: d may be x
+    u32x4_t reg[MAXC];
+#pragma unroll
+    for (int i = 0; i < MAXC; ++i) reg[i] = load_chunk(x, (i * NT + tid) * kPer<T>, a.V);
+    const float xy = to_f32(x[y]);                                   // read before any thread writes: d may be x
+    float w = 0.f;
+    if constexpr (POLICY) w = policy_weight(a.pol, row, tid & 63);
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < MAXC; ++i) {
+        float f[kPer<T>];
+        unpack<T>(reg[i], f);
+#pragma unroll
+        for (int k = 0; k < kPer<T>; ++k) m = fmaxf(m, f[k]);
+    }
+    m = block_max<NT>(m, sh[0]);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < MAXC; ++i) {
+        float f[kPer<T>], part = 0.f;
+        unpack<T>(reg[i], f);
+#pragma unroll
+        for (int k = 0; k < kPer<T>; ++k) part += row_exp<T>(f[k] - m);
+        s += part;
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    s = block_sum<NT>(s, sh[1]);
+    const float lp = (xy - m) - logf(s);
+    if (tid == 0) {
+        a.logp[row] = lp;
+        if (a.stats) { a.stats[2 * (long)row] = m; a.stats[2 * (long)row + 1] = s; }
+    }
+    if constexpr (POLICY) {
+        float t[3];
+        const float c0 = policy_token(a.pol, row, lp, w, t);
+        if (tid == 0) {
+            const long R = (long)a.pol.N * a.pol.T;
+            a.pol.terms[row] = t[0];
+            a.pol.terms[R + row] = t[1];
+            a.pol.terms[2 * R + row] = t[2];
+        }
+        const float cs = -c0 / s;
+#pragma unroll
+        for (int i = 0; i < MAXC; ++i) {
+            const int c = (i * NT + tid) * kPer<T>;
+            if (c < a.V) {
+                float f[kPer<T>];
+                unpack<T>(reg[i], f);
+#pragma unroll
+                for (int k = 0; k < kPer<T>; ++k) f[k] = c0 == 0.f ? 0.f : cs * row_exp<T>(f[k] - m);
+                if (y >= c && y < c + kPer<T>) {
+#pragma unroll
+                    for (int k = 0; k < kPer<T>; ++k)
+                        if (c + k == y) f[k] += c0;
+                }
+                store_chunk(d, c, a.V, f);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        zero_cols<T, NT>(d, a.V, a.W);
+    }
+}
+
+// The same for rows that do not fit the registers of a workgroup: a running maximum and sum, then the row again for the gradient.
+template <typename T, bool POLICY>
+__global__ __launch_bounds__(1024) void long_row_kernel(RowArgs<T> a) {
+    constexpr int NT = 1024;
+    __shared__ float sh[2][NT / 64];
+    const int tid = threadIdx.x, b = blockIdx.x;
+    const int row = b < a.n0 ? a.row0 + b : a.row1 + (b - a.n0);
+    const int64_t y = a.labels[row];
+    T* const d = POLICY ? a.dlogits + (long)row * a.ldd : nullptr;
+    const long R = (long)a.pol.N * a.pol.T;
+    if (y < 0 || y >= a.V) {
+        if (tid == 0) {
+            a.logp[row] = 0.f;
+            if (a.stats) { a.stats[2 * (long)row] = 0.f; a.stats[2 * (long)row + 1] = 1.f; }
+            if constexpr (POLICY) a.pol.terms[row] = a.pol.terms[R + row] = a.pol.terms[2 * R + row] = 0.f;
+        }
+        if constexpr (POLICY) zero_cols<T, NT>(d, 0, a.W);
+        return;
+    }
+    const T* x = a.logits + (long)row * a.ld;
+    const float xy = to_f32(x[y]);
+    float w = 0.f;
+    if constexpr (POLICY) w = policy_weight(a.pol, row, tid & 63);
+    float m = -INFINITY, s = 0.f;
+    for (long c = (long)tid * kPer<T>; c < a.V; c += NT * kPer<T>) {
+        float f[kPer<T>], mc = -INFINITY;
+        unpack<T>(load_chunk(x, (int)c, a.V), f);
+#pragma unroll
+        for (int k = 0; k < kPer<T>; ++k) mc = fmaxf(mc, f[k]);
+        if (mc > m) { s *= row_exp<T>(m - mc); m = mc; }
+        float part = 0.f;
+#pragma unroll
+        for (int k = 0; k < kPer<T>; ++k) part += f[k] == -INFINITY ? 0.f : row_exp<T>(f[k] - m);      // a thread may see nothing but -inf
+        s += part;
+    }
+    const float mine = m;
+    m = block_max<NT>(m, sh[0]);
+    s = block_sum<NT>((mine == -INFINITY && s == 0.f) ? 0.f : s * row_exp<T>(mine - m), sh[1]);
+    const float lp = (xy - m) - logf(s);
+    if (tid == 0) {
+        a.logp[row] = lp;
+        if (a.stats) { a.stats[2 * (long)row] = m; a.stats[2 * (long)row + 1] = s; }
+    }
+    if constexpr (POLICY) {
+        float t[3];
+        const float c0 = policy_token(a.pol, row, lp, w, t);
+        if (tid == 0) { a.pol.terms[row] = t[0]; a.pol.terms[R + row] = t[1]; a.pol.terms[2 * R + row] = t[2]; }
+        const float cs = -c0 / s;
+        for (long c = (long)tid * kPer<T>; c < a.V; c += NT * kPer<T>) {
+            float f[kPer<T>];
+            unpack<T>(load_chunk(x, (int)c, a.V), f);
+#pragma unroll
+            for (int k = 0; k < kPer<T>; ++k) f[k] = (c0 == 0.f ? 0.f : cs * row_exp<T>(f[k] - m)) + (c + k == y ? c0 : 0.f);
+            store_chunk(d, (int)c, a.V, f);
+        }
+        zero_cols<T, NT>(d, a.V, a.W);
+    }
+}
+
+// Gradient of the logits from the row statistics: coef[row / rows_per_coef] (* *alpha) ([v == y] - exp(x - m) / s).
+// A row whose factor is zero is not read.
+template <typename T>
+__global__ __launch_bounds__(256) void logprob_bwd_kernel(const T* logits, long ld, const int64_t* __restrict__ labels, const float* __restrict__ stats,
+                                                          const float* __restrict__ coef, int rows_per_coef, const float* __restrict__ alpha, T* dlogits,
+                                                          long ldd, int W, int V, int row0, int n0, int row1) {
+    constexpr int NT = 256, U = 4;
+    const int tid = threadIdx.x, b = blockIdx.x;
+    const int row = b < n0 ? row0 + b : row1 + (b - n0);
+    const int64_t y = labels[row];
+    T* const d = dlogits + (long)row * ldd;
+    float c0 = 0.f;
+    if (y >= 0 && y < V) c0 = coef[row / rows_per_coef];
+    if (alpha != nullptr) c0 *= *alpha;
+    if (c0 == 0.f || y < 0 || y >= V) {
+        const float z[kPer<T>] = {};
+        for (long c = (long)tid * kPer<T>; c < W; c += NT * kPer<T>) store_chunk(d, (int)c, W, z);
+        return;
+    }
+    const T* x = logits + (long)row * ld;
+    const float m = stats[2 * (long)row], cs = -c0 / stats[2 * (long)row + 1];
+    for (long c0i = (long)tid * kPer<T>; c0i < V; c0i += (long)U * NT * kPer<T>) {
+        u32x4_t reg[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long c = c0i + (long)u * NT * kPer<T>;
+            if (c < V) reg[u] = load_chunk(x, (int)c, V);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long c = c0i + (long)u * NT * kPer<T>;
+            if (c < V) {
+                float f[kPer<T>];
+                unpack<T>(reg[u], f);
+#pragma unroll
+                for (int k = 0; k < kPer<T>; ++k) f[k] = cs * row_exp<T>(f[k] - m);
+                if (y >= c && y < c + kPer<T>) {
+#pragma unroll
+                    for (int k = 0; k < kPer<T>; ++k)
+                        if (c + k == y) f[k] += c0;
+                }
+                store_chunk(d, (int)c, V, f);
+            }
+        }
+    }
+    zero_cols<T, NT>(d, V, W);
+}
+
+// out[n] = sum (or mean) of a sequence's counted log-probabilities; one wave a sequence, lanes stride over its tokens
+__device__ __forceinline__ void sequence_sum(const float* __restrict__ logp, const int64_t* __restrict__ labels, int n, int T, int V, int lane, float& sum, int& cnt) {
+    sum = 0.f;
+    cnt = 0;
+    for (int t = lane; t < T; t += 64) {
+        const int64_t y = labels[(long)n * T + t];
+        if (y >= 0 && y < V) { sum += logp[(long)n * T + t]; ++cnt; }
+    }
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) cnt += __shfl_xor(cnt, o);
+}
+__global__ __launch_bounds__(256) void sequence_sum_kernel(const float* logp, const int64_t* labels, int N, int T, int V, int average, float* out) {
+    const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (n >= N) return;
+    float s;
+    int cnt;
+    sequence_sum(logp, labels, n, T, V, lane, s, cnt);
+    if (lane == 0) out[n] = average ? s / fmaxf((float)cnt, 1.f) : s;
+}
+
+// log(1 + e^x) without overflow
+__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
+
+// Pair i = sequences (i, P + i): h = beta ((S_i - ref_i) - (S_{P+i} - ref_{P+i})), loss_i = (1 - e) softplus(-h) + e softplus(h),
+// d loss_i / d h = e - sigmoid(-h).  coef[n] = d (mean loss) / d log p of every counted token of sequence n.
+__global__ __launch_bounds__(256) void pair_kernel(const float* logp, const int64_t* labels, const float* ref, int P, int T, int V, float beta, float smoothing,
+                                                   int average, int pair0, int pairs, float* seq, float* margins, float* pair_loss, float* coef) {
+    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (i >= pairs) return;
+    const int p = pair0 + i;
+    float sc, sr;
+    int nc, nr;
+    sequence_sum(logp, labels, p, T, V, lane, sc, nc);
+    sequence_sum(logp, labels, P + p, T, V, lane, sr, nr);
+    if (lane != 0) return;
+    const float ic = average ? 1.f / fmaxf((float)nc, 1.f) : 1.f, ir = average ? 1.f / fmaxf((float)nr, 1.f) : 1.f;
+    sc *= ic;
+    sr *= ir;
+    const float h = beta * ((sc - (ref ? ref[p] : 0.f)) - (sr - (ref ? ref[P + p] : 0.f)));
+    const float dh = (smoothing - 1.f / (1.f + expf(h))) * beta / (float)P;
+    seq[p] = sc;
+    seq[P + p] = sr;
+    margins[p] = h;
+    pair_loss[p] = (smoothing == 0.f) ? softplus(-h) : (1.f - smoothing) * softplus(-h) + smoothing * softplus(h);
+    coef[p] = dh * ic;
+    coef[P + p] = -dh * ir;
+}
+
+// out[j] = scale * sum of x[j * n .. (j + 1) * n)
+__global__ __launch_bounds__(1024) void rows_mean_kernel(const float* __restrict__ x, long n, float scale, float* __restrict__ out) {
+    __shared__ float sh[16];
+    float s = 0.f;
+    for (long i = threadIdx.x; i < n; i += 1024) s += x[(long)blockIdx.x * n + i];
+    s = block_sum<1024>(s, sh);
+    if (threadIdx.x == 0) out[blockIdx.x] = s * scale;
+}
+
+// counts[i]: counted tokens of sequence i (seq) or of the i-th of kCountParts equal stretches of the batch
+__global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ labels, long R, long per, int V, int* __restrict__ counts) {
+    __shared__ int sh[4];
+    const long lo = (long)blockIdx.x * per, hi = lo + per < R ? lo + per : R;
+    int n = 0;
+    for (long i = lo + threadIdx.x; i < hi; i += 256) { const int64_t y = labels[i]; n += y >= 0 && y < V; }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) counts[blockIdx.x] = sh[0] + sh[1] + sh[2] + sh[3];
+}
+
+// The policy loss from log-probabilities that are there already (the two-step form): coef per row and the terms
+__global__ __launch_bounds__(256) void policy_terms_kernel(const float* __restrict__ logp, const int64_t* __restrict__ labels, int V, PolicyArgs p, float* __restrict__ coef) {
+    const long R = (long)p.N * p.T, row = (long)blockIdx.x * 256 + threadIdx.x;
+    float w = 0.f;
+    if (!p.seq_mean) w = policy_weight(p, 0, threadIdx.x & 63);       // the wave sums the stretches together
+    if (row >= R) return;
+    const int64_t y = labels[row];
+    float t[3] = {0.f, 0.f, 0.f}, c = 0.f;
+    if (y >= 0 && y < V) {
+        if (p.seq_mean) w = policy_weight(p, (int)row, 0);
+        c = policy_token(p, (int)row, logp[row], w, t);
+    }
+    coef[row] = c;
+    p.terms[row] = t[0];
+    p.terms[R + row] = t[1];
+    p.terms[2 * R + row] = t[2];
+}
+
+// Threads and chunks of a row: the smallest workgroup whose registers hold it, so that short rows keep many rows in flight on a CU
+// and a BART row (50,265 bf16 logits: 512 threads x 13 chunks, 52 registers; f32: 1024 x 13) is resident as a whole.
+template <typename T, bool POLICY>
+int launch_rows(const RowArgs<T>& a, int blocks, hipStream_t s) {
+    const long chunks = ((long)a.V + kPer<T> - 1) / kPer<T>;
+    if (chunks <= 64 * 4) hipLaunchKernelGGL((row_kernel<T, 64, 4, POLICY>), dim3(blocks), dim3(64), 0, s, a);
+    else if (chunks <= 256 * 8) hipLaunchKernelGGL((row_kernel<T, 256, 8, POLICY>), dim3(blocks), dim3(256), 0, s, a);
+    else if (chunks <= 512 * 13) hipLaunchKernelGGL((row_kernel<T, 512, 13, POLICY>), dim3(blocks), dim3(512), 0, s, a);
+    else if (chunks <= 1024 * 13) hipLaunchKernelGGL((row_kernel<T, 1024, 13, POLICY>), dim3(blocks), dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((long_row_kernel<T, POLICY>), dim3(blocks), dim3(1024), 0, s, a);
+    return ok();
+}
+
+bool bad_rows(long R, int V, long ld) { return R <= 0 || R > 0x7fffffffL || V <= 0 || V > 0x7fffffff - 16384 || ld < V; }
+bool bad_align(int dtype, const void* p) { return ((uintptr_t)p & (dtype == MMSUM_BF16 ? 1 : 3)) != 0; }
+
+template <typename T>
+RowArgs<T> row_args(const void* logits, long ld, const int64_t* labels, int V, float* logp, float* stats, int R) {
+    RowArgs<T> a = {};
+    a.logits = static_cast<const T*>(logits); a.ld = ld; a.labels = labels; a.V = V; a.logp = logp; a.stats = stats;
+    a.n0 = R;
+    return a;
+}
+
+template <typename T>
+int launch_bwd(const void* logits, long ld, const int64_t* labels, const float* stats, const float* coef, int rows_per_coef, const float* alpha, void* dlogits,
+               long ldd, int W, int V, int row0, int n0, int row1, int blocks, hipStream_t s) {
+    hipLaunchKernelGGL((logprob_bwd_kernel<T>), dim3(blocks), dim3(256), 0, s, static_cast<const T*>(logits), ld, labels, stats, coef, rows_per_coef, alpha,
+                       static_cast<T*>(dlogits), ldd, W, V, row0, n0, row1);
+    return ok();
+}
+
+long count_slots(int N, int seq_mean) { return seq_mean ? N : kCountParts; }
+int launch_counts(const int64_t* labels, int N, int T, int V, int seq_mean, int* counts, hipStream_t s) {
+    const long R = (long)N * T, per = seq_mean ? T : (R + kCountParts - 1) / kCountParts;
+    hipLaunchKernelGGL(count_kernel, dim3((unsigned)count_slots(N, seq_mean)), dim3(256), 0, s, labels, R, per, V, counts);
+    return ok();
+}
+
+}  // namespace
+
+extern "C" int mmsum_token_logprob(int dtype, const void* logits, long ld, const int64_t* labels, float* logp, float* stats, int R, int V, void* stream) {
+    if (bad_rows(R, V, ld)) return MMSUM_ERR_BAD_SHAPE;
+    if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
+    if (bad_align(dtype, logits)) return MMSUM_ERR_BAD_ALIGN;
+    if (dtype == MMSUM_BF16) return launch_rows<bf16_t, false>(row_args<bf16_t>(logits, ld, labels, V, logp, stats, R), R, (hipStream_t)stream);
+    return launch_rows<float, false>(row_args<float>(logits, ld, labels, V, logp, stats, R), R, (hipStream_t)stream);
+}
+
+extern "C" int mmsum_token_logprob_bwd(int dtype, const void* logits, long ld, const int64_t* labels, const float* stats, const float* coef, int rows_per_coef,
+                                       const float* alpha, void* dlogits, long ldd, int W, int R, int V, void* stream) {
+    if (bad_rows(R, V, ld) || rows_per_coef <= 0 || W < V || W > 0x7fffffff - 16384 || ldd < W) return MMSUM_ERR_BAD_SHAPE;
+    if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
+    if (bad_align(dtype, logits) || bad_align(dtype, dlogits)) return MMSUM_ERR_BAD_ALIGN;
+    if (dtype == MMSUM_BF16) return launch_bwd<bf16_t>(logits, ld, labels, stats, coef, rows_per_coef, alpha, dlogits, ldd, W, V, 0, R, 0, R, (hipStream_t)stream);
+    return launch_bwd<float>(logits, ld, labels, stats, coef, rows_per_coef, alpha, dlogits, ldd, W, V, 0, R, 0, R, (hipStream_t)stream);
+}
+
+extern "C" int mmsum_sequence_logprob(const float* logp, const int64_t* labels, int N, int T, int V, int average, float* out, void* stream) {
+    if (N <= 0 || T <= 0 || V <= 0 || (long)N * T > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    hipLaunchKernelGGL(sequence_sum_kernel, dim3((N + 3) / 4), dim3(256), 0, (hipStream_t)stream, logp, labels, N, T, V, average, out);
+    return ok();
+}
+
+extern "C" int mmsum_preference_pairs(const float* logp, const int64_t* labels, const float* ref, int P, int T, int V, float beta, float smoothing, int average,
+                                      float* seq, float* margins, float* pair_loss, float* coef, float* loss, void* stream) {
+    if (P <= 0 || T <= 0 || V <= 0 || 2L * P * T > 0x7fffffffL || !(smoothing >= 0.f && smoothing <= 1.f)) return MMSUM_ERR_BAD_SHAPE;
+    hipStream_t s = (hipStream_t)stream;
+    hipLaunchKernelGGL(pair_kernel, dim3((P + 3) / 4), dim3(256), 0, s, logp, labels, ref, P, T, V, beta, smoothing, average, 0, P, seq, margins, pair_loss, coef);
+    hipLaunchKernelGGL(rows_mean_kernel, dim3(1), dim3(1024), 0, s, pair_loss, (long)P, 1.f / (float)P, loss);
+    return ok();
+}
+
+// workspace: logp [2PT], stats [2PT][2], pair_loss [P], coef [2P]
+extern "C" long mmsum_preference_workspace(int P, int T) { return P <= 0 || T <= 0 ? 0 : (6L * P * T + 3L * P) * (long)sizeof(float); }
+extern "C" int mmsum_preference_loss(int dtype, const void* logits, long ld, const int64_t* labels, const float* ref, int P, int T, int V, float beta, float smoothing,
+                                     int average, float* loss, float* margins, float* seq, void* dlogits, long ldd, int W, void* workspace, void* stream) {
+    if (P <= 0 || T <= 0 || bad_rows(2L * P * T, V, ld) || W < V || W > 0x7fffffff - 16384 || ldd < W || !(smoothing >= 0.f && smoothing <= 1.f)) return MMSUM_ERR_BAD_SHAPE;
+    if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
+    if (workspace == nullptr) return MMSUM_ERR_WORKSPACE;
+    if (bad_align(dtype, logits) || bad_align(dtype, dlogits) || ((uintptr_t)workspace & 15)) return MMSUM_ERR_BAD_ALIGN;
+    const int R = 2 * P * T;
+    float* const logp = static_cast<float*>(workspace);
+    float* const stats = logp + R;
+    float* const pair_loss = stats + 2L * R;
+    float* const coef = pair_loss + P;
+    int rc = mmsum_token_logprob(dtype, logits, ld, labels, logp, stats, R, V, stream);
+    if (rc == MMSUM_OK) rc = mmsum_preference_pairs(logp, labels, ref, P, T, V, beta, smoothing, average, seq, margins, pair_loss, coef, loss, stream);
+    if (rc == MMSUM_OK) rc = mmsum_token_logprob_bwd(dtype, logits, ld, labels, stats, coef, T, nullptr, dlogits, ldd, W, R, V, stream);
+    return rc;
+}
+
+// workspace: terms [3][NT], counts
+extern "C" long mmsum_policy_workspace(int N, int T) {
+    return N <= 0 || T <= 0 ? 0 : 3L * N * T * (long)sizeof(float) + (long)(N > kCountParts ? N : kCountParts) * (long)sizeof(int);
+}
+static int policy_setup(PolicyArgs& p, const float* old_logp, const float* ref_logp, const float* adv, int adv_per_token, int N, int T, float clip_low,
+                        float clip_high, float kl_coef, int seq_mean, void* workspace) {
+    if (!(clip_low >= 0.f) || !(clip_high >= 0.f) || kl_coef != kl_coef) return MMSUM_ERR_BAD_SHAPE;
+    if (workspace == nullptr) return MMSUM_ERR_WORKSPACE;
+    if ((uintptr_t)workspace & 15) return MMSUM_ERR_BAD_ALIGN;
+    p.old_logp = old_logp; p.ref_logp = ref_logp; p.adv = adv;
+    p.terms = static_cast<float*>(workspace);
+    p.counts = reinterpret_cast<int*>(p.terms + 3L * N * T);
+    p.adv_per_token = adv_per_token; p.seq_mean = seq_mean; p.N = N; p.T = T;
+    p.lo = 1.f - clip_low; p.hi = 1.f + clip_high; p.kl_coef = kl_coef;
+    return MMSUM_OK;
+}
+
+extern "C" int mmsum_policy_terms(const float* logp, const int64_t* labels, const float* old_logp, const float* ref_logp, const float* adv, int adv_per_token, int N,
+                                  int T, int V, float clip_low, float clip_high, float kl_coef, int seq_mean, float* out, float* coef, void* workspace, void* stream) {
+    if (N <= 0 || T <= 0 || V <= 0 || (long)N * T > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    PolicyArgs p = {};
+    int rc = policy_setup(p, old_logp, ref_logp, adv, adv_per_token, N, T, clip_low, clip_high, kl_coef, seq_mean, workspace);
+    hipStream_t s = (hipStream_t)stream;
+    const long R = (long)N * T;
+    if (rc == MMSUM_OK) rc = launch_counts(labels, N, T, V, seq_mean, const_cast<int*>(p.counts), s);
+    if (rc != MMSUM_OK) return rc;
+    hipLaunchKernelGGL(policy_terms_kernel, dim3((unsigned)((R + 255) / 256)), dim3(256), 0, s, logp, labels, V, p, coef);
+    hipLaunchKernelGGL(rows_mean_kernel, dim3(3), dim3(1024), 0, s, p.terms, R, 1.f, out);
+    return ok();
+}
+
+extern "C" int mmsum_policy_loss(int dtype, const void* logits, long ld, const int64_t* labels, const float* old_logp, const float* ref_logp, const float* adv,
+                                 int adv_per_token, int N, int T, int V, float clip_low, float clip_high, float kl_coef, int seq_mean, float* out, float* logp,
+                                 void* dlogits, long ldd, int W, void* workspace, void* stream) {
+    if (N <= 0 || T <= 0 || bad_rows((long)N * T, V, ld) || W < V || W > 0x7fffffff - 16384 || ldd < W) return MMSUM_ERR_BAD_SHAPE;
+    if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
+    if (bad_align(dtype, logits) || bad_align(dtype, dlogits)) return MMSUM_ERR_BAD_ALIGN;
+    PolicyArgs p = {};
+    int rc = policy_setup(p, old_logp, ref_logp, adv, adv_per_token, N, T, clip_low, clip_high, kl_coef, seq_mean, workspace);
+    hipStream_t s = (hipStream_t)stream;
+    const int R = N * T;
+    if (rc == MMSUM_OK) rc = launch_counts(labels, N, T, V, seq_mean, const_cast<int*>(p.counts), s);
+    if (rc != MMSUM_OK) return rc;
+    if (dtype == MMSUM_BF16) {
+        RowArgs<bf16_t> a = row_args<bf16_t>(logits, ld, labels, V, logp, nullptr, R);
+        a.dlogits = static_cast<bf16_t*>(dlogits); a.ldd = ldd; a.W = W; a.pol = p;
+        rc = launch_rows<bf16_t, true>(a, R, s);
+    } else {
+        RowArgs<float> a = row_args<float>(logits, ld, labels, V, logp, nullptr, R);
+        a.dlogits = static_cast<float*>(dlogits); a.ldd = ldd; a.W = W; a.pol = p;
+        rc = launch_rows<float, true>(a, R, s);
+    }
+    if (rc != MMSUM_OK) return rc;
+    hipLaunchKernelGGL(rows_mean_kernel, dim3(3), dim3(1024), 0, s, p.terms, (long)R, 1.f, out);
+    return ok();
+}

@@ -1,0 +1,45 @@
+"""Linear layers in 8-bit integers for inference: a frozen model that scores or writes summaries.
+
+Weights are quantised once, one scale per output channel; activations in every call, one scale per token; the integer sum is exact.
+"""
+import torch
+import torch.nn as nn
+
+from . import kernels as kn
+
+
+class Int8Linear(nn.Module):
+    """y = x W^T (+ bias) (then GELU, erf form) with W [N, K] (f32 or bf16) held as int8 [N, Kp] + one f32 scale per row.  x [..., K] f32 or bf16,
+    y [..., N] in out_dtype (default: x's).  A token whose values are not all finite gives NaN.  No gradient: inputs that require one are refused."""
+
+    def __init__(self, weight, bias=None, gelu=False, out_dtype=None):
+        super().__init__()
+        if weight.dim() != 2 or 0 in weight.shape:
+            raise ValueError("weight: [N, K] expected, got %s" % (tuple(weight.shape),))
+        if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+            raise ValueError("bias: [%d] expected, got %s" % (weight.shape[0], tuple(bias.shape)))
+        if out_dtype not in (None, torch.float32, torch.bfloat16):
+            raise TypeError("unsupported dtype %s" % out_dtype)
+        self.out_features, self.in_features = weight.shape
+        self.gelu, self.out_dtype = bool(gelu), out_dtype
+        q, scale = kn.quantize_rows(weight.detach())
+        self.register_buffer("qweight", q)
+        self.register_buffer("scale", scale)
+        self.register_buffer("bias", None if bias is None else bias.detach().to(torch.float32).clone())
+
+    @classmethod
+    def from_linear(cls, linear, **kw):
+        return cls(linear.weight, linear.bias, **kw)
+
+    def forward(self, x):
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("Int8Linear is for inference: no gradient (use torch.no_grad() or detach the input)")
+        if x.dim() < 1 or x.shape[-1] != self.in_features:
+            raise ValueError("x: [..., %d] expected, got %s" % (self.in_features, tuple(x.shape)))
+        rows = x.reshape(-1, self.in_features)
+        if self.in_features > 1 and rows.stride(1) != 1:
+            rows = rows.contiguous()
+        q, scale = kn.quantize_rows(rows)
+        y = torch.empty(rows.shape[0], self.out_features, dtype=self.out_dtype or x.dtype, device=x.device)
+        kn.gemm_i8(q, scale, self.qweight, self.scale, y, self.bias, self.gelu)
+        return y.reshape(*x.shape[:-1], self.out_features)

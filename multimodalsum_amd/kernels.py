@@ -580,3 +580,269 @@ def gemm_pair(xs, x2s, ws, outs, biases):
         o.A, o.A2, o.B, o.C, o.bias = _p(xs[i]), _p(x2s[i]), _p(ws[i]), _p(outs[i]), _p(biases[i])
         o.lda, o.lda2, o.ldb, o.ldc = _ld(xs[i]), (_ld(x2s[i]) if x2s[i] is not None else 0), _ld(ws[i]), _ld(outs[i])
     check(lib.mmsum_gemm_pair(arr, M, N, K, k1 if k2 else 0, _stream()), "mmsum_gemm_pair")
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------
+# Tuning from preferences and rewards, the scaled embedding, 8-bit products.  These refuse bad arguments with ValueError / TypeError, take
+# their workspaces from the allocator call by call (nothing is shared between streams or captured graphs) and launch on the device that the
+# tensors live on, whichever is current.
+# ---------------------------------------------------------------------------------------------------------------------------------
+def _need(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _device(*tensors):
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("libmmsum_hip kernels need device tensors (no CPU fallback exists)")
+        if dev is None:
+            dev = t.device
+        _need(t.device == dev, "tensors on different devices: %s and %s" % (dev, t.device))
+    return dev
+
+
+def _launch(name, device, *args):
+    if device.index == torch.cuda.current_device():
+        rc = getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream)
+    check(rc, name)
+
+
+def _rows_of(t, what):
+    """[N, T, V] with unit inner stride and one row pitch -> (N, T, V, pitch)."""
+    _need(t.dim() == 3, "%s: [N, T, V] expected, got %s" % (what, tuple(t.shape)))
+    _dt(t)
+    N, T, V = t.shape
+    _need(N > 0 and T > 0 and V > 0, "%s: empty (%s)" % (what, tuple(t.shape)))
+    _need(V == 1 or t.stride(2) == 1, "%s: unit inner stride expected" % what)
+    ld = t.stride(1) if T > 1 else (t.stride(0) if N > 1 else V)
+    _need(ld >= V and (N == 1 or t.stride(0) == T * ld), "%s: rows of one pitch expected (strides %s)" % (what, tuple(t.stride())))
+    _need(N * T < 2 ** 31, "%s: too many rows" % what)
+    return N, T, V, ld
+
+
+def _labels_of(labels, N, T):
+    if labels.dtype != torch.int64:
+        raise TypeError("labels: int64 expected, got %s" % labels.dtype)
+    _need(labels.shape == (N, T), "labels: shape %s expected, got %s" % ((N, T), tuple(labels.shape)))
+    return labels.contiguous()
+
+
+def _f32_of(t, shape, what):
+    if t is None:
+        return None
+    if t.dtype != torch.float32:
+        raise TypeError("%s: float32 expected, got %s" % (what, t.dtype))
+    _need(tuple(t.shape) == tuple(shape), "%s: shape %s expected, got %s" % (what, tuple(shape), tuple(t.shape)))
+    return t.contiguous()
+
+
+def _span(t):
+    n = 1 + sum((s - 1) * abs(st) for s, st in zip(t.shape, t.stride())) if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _dlogits_of(dlogits, logits, N, T, V, ld):
+    """The gradient's buffer: the caller's [N, T, W >= V] (the logits themselves, or memory apart from them) or a new one of the logits' pitch
+    (unless they are a narrow view of something much wider)."""
+    if dlogits is None:
+        ld = ld if ld - V < 256 else V
+        return torch.empty(N, T, ld, dtype=logits.dtype, device=logits.device)[:, :, :V], ld, V
+    if dlogits.dtype != logits.dtype:
+        raise TypeError("dlogits: %s expected, got %s" % (logits.dtype, dlogits.dtype))
+    n, t, W, ldd = _rows_of(dlogits, "dlogits")
+    _need((n, t) == (N, T) and W >= V, "dlogits: [%d, %d, >= %d] expected, got %s" % (N, T, V, tuple(dlogits.shape)))
+    a, b = _span(logits), _span(dlogits)
+    _need(a[0] >= b[1] or b[0] >= a[1] or (a[0] == b[0] and ld == ldd), "dlogits overlaps the logits without being them")
+    return dlogits, ldd, W
+
+
+def token_logprob(logits, labels, stats=None):
+    """logp f32 [N, T] = log_softmax(logits)[labels] (0 where a label is outside 0 .. V-1).  stats f32 [N, T, 2] (optional): what
+    token_logprob_bwd needs."""
+    N, T, V, ld = _rows_of(logits, "logits")
+    labels = _labels_of(labels, N, T)
+    if stats is not None:
+        _need(stats.dtype == torch.float32 and stats.shape == (N, T, 2) and stats.is_contiguous(), "stats: packed float32 [N, T, 2] expected")
+    dev = _device(logits, labels, stats)
+    logp = torch.empty(N, T, dtype=torch.float32, device=dev)
+    _launch("mmsum_token_logprob", dev, _dt(logits), _p(logits), ld, _p(labels), _p(logp), _p(stats), N * T, V)
+    return logp
+
+
+def token_logprob_bwd(logits, labels, stats, coef, alpha=None, dlogits=None):
+    """dlogits = c ([v == label] - softmax): c = coef f32 [N, T] or [N] (one for a sequence), times alpha (device f32 scalar)."""
+    N, T, V, ld = _rows_of(logits, "logits")
+    labels = _labels_of(labels, N, T)
+    _need(stats.dtype == torch.float32 and stats.shape == (N, T, 2) and stats.is_contiguous(), "stats: packed float32 [N, T, 2] expected")
+    coef = _f32_of(coef, (N,) if coef.dim() == 1 else (N, T), "coef")
+    if alpha is not None:
+        _need(alpha.dtype == torch.float32 and alpha.numel() == 1, "alpha: one float32 expected")
+    dev = _device(logits, labels, stats, coef, alpha, dlogits)
+    dlogits, ldd, W = _dlogits_of(dlogits, logits, N, T, V, ld)
+    _launch("mmsum_token_logprob_bwd", dev, _dt(logits), _p(logits), ld, _p(labels), _p(stats), _p(coef), T if coef.dim() == 1 else 1, _p(alpha),
+            _p(dlogits), ldd, W, N * T, V)
+    return dlogits
+
+
+def sequence_logprob(logp, labels, V, average=False):
+    """out f32 [N]: the sum (mean) of every sequence's counted log-probabilities."""
+    N, T = logp.shape
+    labels, logp = _labels_of(labels, N, T), _f32_of(logp, (N, T), "logp")
+    dev = _device(logp, labels)
+    out = torch.empty(N, dtype=torch.float32, device=dev)
+    _launch("mmsum_sequence_logprob", dev, _p(logp), _p(labels), N, T, int(V), int(bool(average)), _p(out))
+    return out
+
+
+def _pairs_of(N, ref, smoothing):
+    _need(N % 2 == 0, "preference loss: [chosen; rejected] sequences expected, got an odd number (%d)" % N)
+    _need(0.0 <= smoothing <= 1.0, "label_smoothing: 0 .. 1 expected, got %r" % (smoothing,))
+    return N // 2, _f32_of(ref, (N,), "ref_logps")
+
+
+def preference_pairs(logp, labels, ref, V, beta, smoothing, average):
+    """From log-probabilities -> (loss [], margins [P], sequence log-probabilities [2P], coef [2P])."""
+    N, T = logp.shape
+    labels, logp = _labels_of(labels, N, T), _f32_of(logp, (N, T), "logp")
+    P, ref = _pairs_of(N, ref, smoothing)
+    dev = _device(logp, labels, ref)
+    seq, margins, pair_loss, coef, loss = torch.empty(6 * P + 1, dtype=torch.float32, device=dev).split([2 * P, P, P, 2 * P, 1])
+    _launch("mmsum_preference_pairs", dev, _p(logp), _p(labels), _p(ref), P, T, int(V), float(beta), float(smoothing), int(bool(average)), _p(seq), _p(margins),
+            _p(pair_loss), _p(coef), _p(loss))
+    return loss.reshape(()), margins, seq, coef
+
+
+def preference_loss(logits, labels, ref, beta, smoothing, average, dlogits=None):
+    """Logits to gradient -> (loss [], margins [P], sequence log-probabilities [2P], dlogits)."""
+    N, T, V, ld = _rows_of(logits, "logits")
+    labels = _labels_of(labels, N, T)
+    P, ref = _pairs_of(N, ref, smoothing)
+    dlogits, ldd, W = _dlogits_of(dlogits, logits, N, T, V, ld)
+    dev = _device(logits, labels, ref, dlogits)
+    seq, margins, loss = torch.empty(3 * P + 1, dtype=torch.float32, device=dev).split([2 * P, P, 1])
+    ws = torch.empty(lib.mmsum_preference_workspace(P, T), dtype=torch.uint8, device=dev)
+    _launch("mmsum_preference_loss", dev, _dt(logits), _p(logits), ld, _p(labels), _p(ref), P, T, V, float(beta), float(smoothing), int(bool(average)), _p(loss),
+            _p(margins), _p(seq), _p(dlogits), ldd, W, _p(ws))
+    return loss.reshape(()), margins, seq, dlogits
+
+
+def _policy_of(N, T, old, adv, ref, clip_low, clip_high, kl_coef, reduction):
+    _need(reduction in ("token", "sequence"), "reduction: 'token' or 'sequence' expected, got %r" % (reduction,))
+    _need(clip_low >= 0.0 and clip_high >= 0.0, "clip_low, clip_high: not negative")
+    _need(kl_coef == kl_coef and (kl_coef == 0.0 or ref is not None), "kl_coef without ref_logps")
+    return _f32_of(old, (N, T), "old_logps"), _f32_of(adv, (N,) if adv.dim() == 1 else (N, T), "advantages"), _f32_of(ref, (N, T), "ref_logps")
+
+
+def policy_terms(logp, labels, old, adv, ref, V, clip_low, clip_high, kl_coef, reduction):
+    """From log-probabilities -> (out f32 [3] = loss, KL, clipped share; coef [N, T])."""
+    N, T = logp.shape
+    labels, logp = _labels_of(labels, N, T), _f32_of(logp, (N, T), "logp")
+    old, adv, ref = _policy_of(N, T, old, adv, ref, clip_low, clip_high, kl_coef, reduction)
+    dev = _device(logp, labels, old, adv, ref)
+    out, coef = torch.empty(3, dtype=torch.float32, device=dev), torch.empty(N, T, dtype=torch.float32, device=dev)
+    ws = torch.empty(lib.mmsum_policy_workspace(N, T), dtype=torch.uint8, device=dev)
+    _launch("mmsum_policy_terms", dev, _p(logp), _p(labels), _p(old), _p(ref), _p(adv), int(adv.dim() == 2), N, T, int(V), float(clip_low), float(clip_high),
+            float(kl_coef), int(reduction == "sequence"), _p(out), _p(coef), _p(ws))
+    return out, coef
+
+
+def policy_loss(logits, labels, old, adv, ref, clip_low, clip_high, kl_coef, reduction, dlogits=None):
+    """Logits to gradient, the logits read once -> (out f32 [3] = loss, KL, clipped share; logp [N, T]; dlogits)."""
+    N, T, V, ld = _rows_of(logits, "logits")
+    labels = _labels_of(labels, N, T)
+    old, adv, ref = _policy_of(N, T, old, adv, ref, clip_low, clip_high, kl_coef, reduction)
+    dlogits, ldd, W = _dlogits_of(dlogits, logits, N, T, V, ld)
+    dev = _device(logits, labels, old, adv, ref, dlogits)
+    out, logp = torch.empty(3, dtype=torch.float32, device=dev), torch.empty(N, T, dtype=torch.float32, device=dev)
+    ws = torch.empty(lib.mmsum_policy_workspace(N, T), dtype=torch.uint8, device=dev)
+    _launch("mmsum_policy_loss", dev, _dt(logits), _p(logits), ld, _p(labels), _p(old), _p(ref), _p(adv), int(adv.dim() == 2), N, T, V, float(clip_low),
+            float(clip_high), float(kl_coef), int(reduction == "sequence"), _p(out), _p(logp), _p(dlogits), ldd, W, _p(ws))
+    return out, logp, dlogits
+
+
+def _ids_of(ids):
+    if ids.dtype != torch.int64:
+        raise TypeError("ids: int64 expected, got %s" % ids.dtype)
+    return ids.reshape(-1)
+
+
+def _pitch2(t, what):
+    _need(t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1), "%s: [rows, columns] with unit inner stride expected" % what)
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    _need(ld >= t.shape[1], "%s: overlapping rows" % what)
+    return ld
+
+
+def embed_fwd(ids, table, scale=1.0):
+    """y [*ids.shape, D] = scale * table[ids] in the table's type; ids outside 0 .. V-1 give zero rows."""
+    flat, lde = _ids_of(ids).contiguous(), _pitch2(table, "table")
+    (V, D), n = table.shape, flat.numel()
+    _need(V > 0 and D > 0, "table: empty")
+    _dt(table)
+    dev = _device(ids, table)
+    y = torch.empty(*ids.shape, D, dtype=table.dtype, device=dev)
+    if n:
+        _launch("mmsum_embed_fwd", dev, _dt(table), _p(flat), _p(table), lde, _p(y), D, n, V, D, float(scale))
+    return y
+
+
+def embed_bwd(dy, ids, V, scale=1.0, pad_id=None, out=None, accumulate=False):
+    """out f32 [V, D] (+)= scale * sum of dy rows by id (pad_id and ids outside 0 .. V-1: none)."""
+    flat = _ids_of(ids).contiguous()
+    D, n = dy.shape[-1], flat.numel()
+    _need(dy.shape[:-1] == ids.shape, "dy: shape %s expected, got %s" % ((*ids.shape, D), tuple(dy.shape)))
+    _need(V > 0 and D > 0 and n < 2 ** 30, "embed_bwd: %d ids into [%d, %d]" % (n, V, D))
+    dy = dy.reshape(-1, D)
+    if n and D > 1 and dy.stride(1) != 1:
+        dy = dy.contiguous()
+    lddy = _pitch2(dy, "dy") if n else D
+    _need(not accumulate or out is not None, "accumulate without out")
+    _need(out is None or (out.dtype == torch.float32 and out.shape == (V, D) and out.is_contiguous()), "out: packed float32 [%d, %d] expected" % (V, D))
+    _dt(dy)
+    dev = _device(dy, ids, out)
+    if out is None:
+        out = torch.empty(V, D, dtype=torch.float32, device=dev)
+    ws = torch.empty(max(1, lib.mmsum_embed_bwd_workspace(n, D)), dtype=torch.uint8, device=dev)
+    _launch("mmsum_embed_bwd", dev, _dt(dy), _p(dy), lddy, _p(flat), n, V, D, float(scale), -1 if pad_id is None else int(pad_id), int(bool(accumulate)), _p(out), _p(ws))
+    return out
+
+
+I8_K_STEP = 128                  # the 8-bit operands' reduction length is padded with zeros to a multiple of this
+
+
+def quantize_rows(x):
+    """x [M, K] -> (q int8 [M, Kp] = 127 x / max |x| of the row, ties to even, Kp = K padded with zeros; scale f32 [M] = max |x| / 127)."""
+    ldx = _pitch2(x, "x")
+    M, K = x.shape
+    _need(0 < K <= 131072, "quantize_rows: K = %d, 1 .. 131072 expected" % K)
+    _dt(x)
+    dev = _device(x)
+    Kp = -(-K // I8_K_STEP) * I8_K_STEP
+    q, scale = torch.empty(M, Kp, dtype=torch.int8, device=dev), torch.empty(M, dtype=torch.float32, device=dev)
+    if M:
+        _launch("mmsum_quantize_i8", dev, _dt(x), _p(x), ldx, M, K, _p(q), Kp, _p(scale))
+    return q, scale
+
+
+def gemm_i8(qx, sx, qw, sw, out, bias=None, gelu=False):
+    """out [M, N] = sx[m] sw[n] (qx . qw^T) (+ bias) (GELU), operands as quantize_rows leaves them; the integer sum is exact."""
+    (M, K), N = qx.shape, qw.shape[0]
+    for t, what in ((qx, "qx"), (qw, "qw")):
+        if t.dtype != torch.int8:
+            raise TypeError("%s: int8 expected, got %s" % (what, t.dtype))
+    _need(qw.shape[1] == K and K % I8_K_STEP == 0 and 0 < K <= 131072, "gemm_i8: operands as quantize_rows leaves them expected")
+    _need(out.shape == (M, N), "out: shape %s expected, got %s" % ((M, N), tuple(out.shape)))
+    sx, sw, bias = _f32_of(sx, (M,), "sx"), _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias")
+    ldx, ldw, ldy = _pitch2(qx, "qx"), _pitch2(qw, "qw"), _pitch2(out, "out")
+    _dt(out)
+    dev = _device(qx, sx, qw, sw, out, bias)
+    if M and N:
+        _launch("mmsum_gemm_i8", dev, _p(qx), ldx, _p(sx), _p(qw), ldw, _p(sw), _p(bias), _dt(out), _p(out), ldy, M, N, K, int(bool(gelu)))
+    return out
