@@ -461,10 +461,10 @@ int mmsum_embed_bwd(int dtype, const void* dy, long lddy, const int64_t* ids, lo
                     void* workspace, void* stream);
 
 /* 8-bit integer products (inference): q [M, ldq] = 127 x / max |x| of the row, rounded to the nearest (ties to even), columns K .. ldq-1 zero;
- * scale [M] = max |x| / 127.  A row with a value that is not finite gets a scale that is not finite.  ldq a multiple of 64, q 16-byte aligned. */
+ * scale [M] = max |x| / 127.  A row with a value that is not finite gets a scale that is not finite.  ldq a multiple of 128, q 16-byte aligned. */
 int mmsum_quantize_i8(int dtype, const void* x, long ldx, int M, int K, void* q, long ldq, float* scale, void* stream);
 /* y[m][n] = sx[m] sw[n] sum_k qx[m][k] qw[n][k] (+ bias[n], f32, may be NULL) (gelu: erf form).  The sum is exact.  K (padded with zeros) a multiple of
- * 64, at most 131,072; pitches in bytes, multiples of 16; qx, qw 16-byte aligned. */
+ * 128, at most 131,072; pitches in bytes, multiples of 16 below 4 MiB; qx, qw 16-byte aligned. */
 int mmsum_gemm_i8(const void* qx, long ldx, const float* sx, const void* qw, long ldw, const float* sw, const float* bias, int dtype_out, void* y, long ldy,
                   int M, int N, int K, int gelu, void* stream);
 

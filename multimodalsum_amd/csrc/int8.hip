@@ -5,52 +5,395 @@
 // are not all finite has a scale that is not finite and gives NaN; a row of zeros gives the bias.
 // Bound: the integer matrix cores (twice the bf16 rate) for many rows, HBM (the weights once, half the bf16 bytes) for few.
 #include "gemm_common.h"
+#include <type_traits>
 
 namespace {
 
 inline int ok() { return hipGetLastError() == hipSuccess ? MMSUM_OK : MMSUM_ERR_HIP; }
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef u32x4_t u32x4_a4_t __attribute__((aligned(4)));
 
-// ---- quantisation: one workgroup a row ---------------------------------------------------------------------------------------------
-// 127 x first, so that x = max / 2 lands on the tie it is; rows near the end of the f32 range are taken down by 2^8 before that
-__device__ __forceinline__ float row_pre(float top) { return top > 0x1p119f ? 0x1p-8f : 1.f; }
-__device__ __forceinline__ int quantize(float x, float pre, float top_pre) {
-    const float q = rintf((x * pre) * 127.f / top_pre);
-    return q == q ? (int)fminf(fmaxf(q, -127.f), 127.f) : 0;
+// ---- quantisation ------------------------------------------------------------------------------------------------------------------
+// 127 x first, so that x = max / 2 lands on the tie it is; the quotient by max correctly rounded: with rc = 1 / max rounded to the nearest,
+// q = y rc is within an ulp, y - q max is exact in an fma, and q + (y - q max) rc rounds to the quotient (Markstein).  Rows near either end
+// of the f32 range are moved by 2^64 first.  The maximum is taken over the bits of |x|, where NaN is larger than infinity: it survives.
+struct RowQuant { float mul, top, rc, scale; bool zero; };
+__device__ __forceinline__ RowQuant row_quant(uint32_t top_bits) {
+    const float top = __builtin_bit_cast(float, top_bits);
+    const float pre = top > 0x1p100f ? 0x1p-64f : top < 0x1p-60f ? 0x1p64f : 1.f;
+    RowQuant r;
+    r.zero = !(top > 0.f && top < INFINITY);                        // nothing to quantise: zeros (a scale that is not finite makes them NaN)
+    r.mul = 127.f * pre;
+    r.top = top * pre;
+    r.rc = 1.f / r.top;
+    r.scale = top / 127.f;
+    return r;
+}
+__device__ __forceinline__ int quantize(float x, const RowQuant& r) {
+    const float y = x * r.mul, q = y * r.rc;
+    return (int)rintf(fmaf(fmaf(-q, r.top, y), r.rc, q));
+}
+template <typename T> __device__ __forceinline__ void load_row8(const T* __restrict__ x, int k, int K, float (&f)[8]) {
+    if (k + 8 <= K) {
+        if constexpr (sizeof(T) == 2) {
+            typedef u32x4_t v_t __attribute__((aligned(2)));
+            const u32x4_t v = *reinterpret_cast<const v_t*>(x + k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = __builtin_bit_cast(float, e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16);
+        } else {
+            const u32x4_t a = *reinterpret_cast<const u32x4_a4_t*>(x + k), b = *reinterpret_cast<const u32x4_a4_t*>(x + k + 4);
+            __builtin_memcpy(f, &a, 16);
+            __builtin_memcpy(f + 4, &b, 16);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = k + e < K ? to_f32(x[k + e]) : 0.f;
+    }
+}
+__device__ __forceinline__ uint32_t top8(uint32_t top, const float (&f)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float v = f[e];
+        const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+        top = u > top ? u : top;
+    }
+    return top;
+}
+__device__ __forceinline__ u32x2_t pack8(const float (&f)[8], const RowQuant& r) {
+    uint32_t w[2] = {0, 0};
+    if (!r.zero)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e >> 2] |= ((uint32_t)quantize(f[e], r) & 255u) << (8 * (e & 3));
+    return u32x2_t{w[0], w[1]};
+}
+__device__ __forceinline__ uint32_t wave_top(uint32_t t) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t v = __shfl_xor((int)t, o);
+        t = v > t ? v : t;
+    }
+    return t;
 }
 
+// A wave a row, eight neighbouring values a lane and step, the row held in registers between the maximum and the rounding (K <= 512 CH).
+// Bound: HBM (the row once, a byte out for each value).
+template <typename T, int CH>
+__global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, long ldx, int M, int K, int8_t* __restrict__ q, long ldq, float* __restrict__ scale) {
+    const int lane = threadIdx.x & 63;
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= M) return;
+    float f[CH][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) load_row8(x + row * ldx, (i * 64 + lane) * 8, K, f[i]);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) top = top8(top, f[i]);
+    const RowQuant r = row_quant(wave_top(top));
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int k = (i * 64 + lane) * 8;
+        if (k < ldq) *reinterpret_cast<u32x2_t*>(q + row * ldq + k) = pack8(f[i], r);
+    }
+    if (lane == 0) scale[row] = r.scale;
+}
+// longer rows: a workgroup a row, read twice
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, long ldx, int K, int8_t* __restrict__ q, long ldq, float* __restrict__ scale) {
-    __shared__ float sh[4];
-    __shared__ int bad[4];
+__global__ __launch_bounds__(256) void quantize_long_kernel(const T* __restrict__ x, long ldx, int K, int8_t* __restrict__ q, long ldq, float* __restrict__ scale) {
+    __shared__ uint32_t sh[4];
     const long row = blockIdx.x;
     const int tid = threadIdx.x;
-    float top = 0.f;
-    int nan = 0;
-    for (int k = tid; k < K; k += 256) {
-        const float v = to_f32(x[row * ldx + k]);
-        top = fmaxf(top, fabsf(v));
-        nan |= v != v;
+    uint32_t top = 0;
+    for (int k = tid * 8; k < K; k += 2048) {
+        float f[8];
+        load_row8(x + row * ldx, k, K, f);
+        top = top8(top, f);
     }
-    top = warp_max(top);
-    const bool wave_nan = __any(nan);
-    if ((tid & 63) == 0) { sh[tid >> 6] = top; bad[tid >> 6] = wave_nan; }
+    top = wave_top(top);
+    if ((tid & 63) == 0) sh[tid >> 6] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-    if (bad[0] | bad[1] | bad[2] | bad[3]) top = NAN;
-    const float pre = row_pre(top), tp = top * pre;
-    for (int k = tid; k < (int)ldq; k += 256) q[row * ldq + k] = k < K ? (int8_t)quantize(to_f32(x[row * ldx + k]), pre, tp) : (int8_t)0;
-    if (tid == 0) scale[row] = top / 127.f;
+    const uint32_t a = sh[0] > sh[1] ? sh[0] : sh[1], b = sh[2] > sh[3] ? sh[2] : sh[3];
+    const RowQuant r = row_quant(a > b ? a : b);
+    for (int k = tid * 8; k < (int)ldq; k += 2048) {
+        float f[8];
+        load_row8(x + row * ldx, k, K, f);
+        *reinterpret_cast<u32x2_t*>(q + row * ldq + k) = pack8(f, r);
+    }
+    if (tid == 0) scale[row] = r.scale;
+}
+template <typename T>
+int launch_quantize(const void* x, long ldx, int M, int K, void* q, long ldq, float* scale, hipStream_t s) {
+    const dim3 grid((unsigned)((M + 3L) / 4));
+    const T* const xt = static_cast<const T*>(x);
+    int8_t* const qt = static_cast<int8_t*>(q);
+    if (ldq <= 512) hipLaunchKernelGGL((quantize_kernel<T, 1>), grid, dim3(256), 0, s, xt, ldx, M, K, qt, ldq, scale);
+    else if (ldq <= 1024) hipLaunchKernelGGL((quantize_kernel<T, 2>), grid, dim3(256), 0, s, xt, ldx, M, K, qt, ldq, scale);
+    else if (ldq <= 2048) hipLaunchKernelGGL((quantize_kernel<T, 4>), grid, dim3(256), 0, s, xt, ldx, M, K, qt, ldq, scale);
+    else if (ldq <= 4096) hipLaunchKernelGGL((quantize_kernel<T, 8>), grid, dim3(256), 0, s, xt, ldx, M, K, qt, ldq, scale);
+    else hipLaunchKernelGGL((quantize_long_kernel<T>), dim3(M), dim3(256), 0, s, xt, ldx, K, qt, ldq, scale);
+    return ok();
+}
+
+// GELU, erf form: x Phi(x) = max(x, 0) - |x| Phi(-|x|) with Phi(-a) = 1/2 erfc(a / sqrt 2) by Abramowitz-Stegun 7.1.26 (|error| < 8e-8, no
+// cancellation).  13 instructions, two of them transcendental: the many-row kernel's epilogue is bound by them.
+__device__ __forceinline__ float gelu_i8(float x) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(x), 0.23164189f, 1.f));
+    const float e = __builtin_amdgcn_exp2f(x * (x * -0.72134752044f));
+    const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);     // halved
+    return fmaf(-fabsf(x), (poly * t) * e, fmaxf(x, 0.f));
 }
 
 // ---- product -----------------------------------------------------------------------------------------------------------------------
 struct I8Args {
     const int8_t* A; long lda; const float* sa; const int8_t* B; long ldb; const float* sb; const float* bias;
-    void* C; long ldc; int M, N, K, gelu;
+    void* C; long ldc; int M, N, K;
 };
 
-// v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k of row l & 15, k group l >> 4; result column l & 15, rows 4 (l >> 4) + e
-template <typename T>
+// eight neighbouring f32 of an array of n (WHOLE: all inside; else the last one in place of those behind it), there when the function returns:
+// a first use inside a predicated store would wait for every store issued before it, one by one
+template <bool WHOLE> __device__ __forceinline__ void load_cols(const float* __restrict__ p, int c, int n, float (&f)[8]) {
+    if constexpr (WHOLE) {
+        const u32x4_t a = *reinterpret_cast<const u32x4_a4_t*>(p + c), b = *reinterpret_cast<const u32x4_a4_t*>(p + c + 4);
+        __builtin_memcpy(f, &a, 16);
+        __builtin_memcpy(f + 4, &b, 16);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = p[c + k < n ? c + k : n - 1];
+    }
+}
+__device__ __forceinline__ void retire(float (&f)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) asm volatile("" : "+v"(f[k]));
+}
+
+// eight results of a row of which n are left (WHOLE: all of them); rows may start at any element
+template <typename T, bool WHOLE> __device__ __forceinline__ void store_cols(T* o, int n, const float (&v)[8]) {
+    if constexpr (!WHOLE) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < n) o[k] = from_f32<T>(v[k]);
+    } else if constexpr (sizeof(T) == 2) {
+        typedef bf16x8_t v_t __attribute__((aligned(2)));
+        bf16x8_t t;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = (bf16_t)v[k];
+        *reinterpret_cast<v_t*>(o) = t;
+    } else {
+        typedef f32x4_t v_t __attribute__((aligned(4)));
+        *reinterpret_cast<v_t*>(o) = f32x4_t{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<v_t*>(o + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+    }
+}
+
+// Many rows: 256x256 tiles, four waves of 128x128, one a SIMD, 256 accumulator registers each (every AGPR, pinned there as "+a" operands of
+// the MFMAs).  Operands pass through LDS in stages of 128 bytes of k: row r at 128 r, its 16-byte chunk c at c ^ ((r >> 1) & 7), which
+// spreads a fragment read (row = lane & 15, chunk = lane >> 4) over all banks; the DMA writes LDS linearly, so the XOR sits on the source
+// address of its lanes.  LDS holds three stages of A (streamed) and two of B (weights, in L2): 160 KB.
+// The stages of ALL tiles of a workgroup form one stream: while the last two stages of a tile are multiplied, the first two of the next
+// one are on their way, and they land under the epilogue, which goes from the accumulators straight to memory and leaves LDS alone.
+//   stage s: 64 MFMAs on its first 64 k (fragments X) | reads of its second 64 k (Y) | DMA: A of stage s + 2
+//            wait for stage s + 1 (only A of s + 2 may be in flight: vmcnt(8)) ; barrier
+//            64 MFMAs on Y | reads of stage s + 1's first 64 k (X) | DMA: B of stage s + 2
+// The weights ride as the MFMA's A operand, so that a lane's four results are neighbouring columns; within 32 weight rows LDS row
+// 16 j + 4 g + e holds weight row 8 g + 4 j + e, and the two MFMAs of a pair leave a lane eight neighbouring columns: a 16-byte store.
+// Measured (MI355X): 8192^3 393 us = 2,796 TOP/s (the library's integer product 2,107); 36,864 x 4,096 x 1,024 170 us, with GELU 213 us: a
+// tile's epilogue is 65,536 values of 6 (25 with GELU, counting the transcendentals' four) issue slots on 256 lanes beside 11 us of main loop.
+constexpr int kStageBytes = 256 * 128;
+template <typename T, bool GELU>
+__global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(I8Args p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int B_BASE = 3 * kStageBytes;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    const int tiles_m = (p.M + 255) / 256, tiles_n = (p.N + 255) / 256, total = tiles_m * tiles_n;
+    const int nst = p.K / 128;
+    int a_frag0, b_frag0, ydelta, offA, offB;                     // per lane; made anew for every tile (lane_constants), so that the epilogue need not carry them
+
+    const int my_tiles = (total - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;     // >= 1: the grid has no more workgroups than tiles
+    const int S = my_tiles * nst;
+    // the stage that is requested next: tile pvid, stage pst of it, into LDS stages pa / pb
+    int pvid = blockIdx.x, pst = 0, pa = 0, pb = 0;
+    const int8_t* baseA = nullptr;
+    const int8_t* baseB = nullptr;
+    int bytesA = 0, bytesB = 0;                                    // from the tile's first row to the operand's end: rows behind it are not fetched (nor their results stored)
+    // A piece is eight rows; piece i of wave w covers rows 32 i + 8 w .., so a lane's offset of piece i is that of piece 0 + 32 i rows.
+    auto lane_constants = [&]() {
+        int ln;
+        asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(ln));
+        const int row0 = wave * 8 + (ln >> 3), ch0 = ((ln & 7) ^ ((row0 >> 1) & 7)) * 16;
+        offA = row0 * (int)p.lda + ch0;
+        offB = ((((row0 >> 2) & 3) << 3) | (((row0 >> 4) & 1) << 2) | (row0 & 3)) * (int)p.ldb + ch0;
+        const int r16 = ln & 15, fo = r16 * 128 + ((((ln >> 4) ^ (r16 >> 1)) & 7) << 4);
+        a_frag0 = wm * 128 * 128 + fo;
+        b_frag0 = B_BASE + wn * 128 * 128 + fo;
+        ydelta = (fo ^ 64) - fo;
+    };
+    auto set_tile = [&](int vid) {
+        int tm, tn;
+        tile_coords(xcd_remap(vid, total), tiles_m, tiles_n, tm, tn);
+        baseA = p.A + (long)tm * 256 * p.lda;
+        baseB = p.B + (long)tn * 256 * p.ldb;
+        const long ra = (p.M - (long)tm * 256) * p.lda, rb = (p.N - (long)tn * 256) * p.ldb;
+        bytesA = (int)(ra < 0x7fffffff ? ra : 0x7fffffff);
+        bytesB = (int)(rb < 0x7fffffff ? rb : 0x7fffffff);
+    };
+#if defined(__HIP_DEVICE_COMPILE__)        // the host pass rejects the buffer-resource builtins inside templates
+#define I8_DMA(BASE, BYTES, OFF, LDS)                                                                                               \
+    {                                                                                                                               \
+        typedef __attribute__((address_space(3))) void* lds_ptr;                                                                    \
+        const __amdgpu_buffer_rsrc_t r_ = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(BASE), 0, BYTES, 0x00020000);       \
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r_, (lds_ptr)(LDS), 16, OFF, pst * 128, 0, 0);                                     \
+    }
+#else
+#define I8_DMA(BASE, BYTES, OFF, LDS) {}
+#endif
+#define I8_A(I) I8_DMA(baseA, bytesA, oa + (I) * 32 * (int)p.lda, smem + pa * kStageBytes + ((I) * 4 + wave) * 1024)
+#define I8_B(I) I8_DMA(baseB, bytesB, ob + (I) * 32 * (int)p.ldb, smem + B_BASE + pb * kStageBytes + ((I) * 4 + wave) * 1024)
+    auto advance = [&]() {
+        pa = pa == 2 ? 0 : pa + 1;
+        pb ^= 1;
+        if (++pst == nst) {
+            pst = 0;
+            pvid += gridDim.x;
+            if (pvid < total) set_tile(pvid);
+        }
+    };
+
+    Frag aX[4], bX[4], aY[4], bY[4];
+    set_tile(pvid);
+    lane_constants();
+    int oa = offA, ob = offB;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) I8_A(i)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) I8_B(i)
+    advance();
+    if (S > 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) I8_A(i)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) I8_B(i)
+        advance();
+        asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+#define I8_MMA(FA, FB, I, J)                                                                                                         \
+    _Pragma("unroll") for (int q = 0; q < 4; ++q)                                                                                    \
+        asm volatile("v_mfma_i32_16x16x64_i8 %0, %2, %1, %0" : "+a"(c[I][J][q]) : "v"(FA[I].c[q >> 1]), "v"(FB[J].c[q & 1]) : "memory");
+#define I8_MMA0(FA, FB, I, J)                                                                                                        \
+    _Pragma("unroll") for (int q = 0; q < 4; ++q)                                                                                    \
+        asm volatile("v_mfma_i32_16x16x64_i8 %0, %2, %1, 0" : "=a"(c[I][J][q]) : "v"(FA[I].c[q >> 1]), "v"(FB[J].c[q & 1]) : "memory");
+    // LEFT = stages of the stream behind this one: >= 2 steady state; 1: nothing left to request; 0: the last one
+    bool whole = false;                                           // the last tile left by the WHOLE epilogue
+    auto stage = [&](i32x4_t (&c)[4][4][4], int abuf, int bbuf, auto left_c, auto first_c) {
+        constexpr int LEFT = decltype(left_c)::value;
+        constexpr bool FIRST = decltype(first_c)::value;
+        const char* As = smem + abuf * kStageBytes + a_frag0;
+        const char* Bs = smem + bbuf * kStageBytes + b_frag0;
+        int oa = offA, ob = offB;
+        asm volatile("s_nop 1" : "+v"(oa), "+v"(ob)::"memory");     // opaque: the pieces' 16 offsets are added up here, not carried in registers
+#pragma unroll
+        for (int g = 0; g < 16; ++g) {
+            if constexpr (FIRST) { I8_MMA0(aX, bX, g >> 2, g & 3) } else { I8_MMA(aX, bX, g >> 2, g & 3) }
+            if (g < 8) bY[g >> 1].c[g & 1] = *reinterpret_cast<const u32x4_t*>(Bs + ((g >> 1) * 32 + (g & 1) * 16) * 128 + ydelta);
+            else aY[(g - 8) >> 1].c[g & 1] = *reinterpret_cast<const u32x4_t*>(As + (((g - 8) >> 1) * 32 + (g & 1) * 16) * 128 + ydelta);
+            if constexpr (LEFT >= 2) { if (!(g & 1)) I8_A(g >> 1) }
+        }
+        // vmcnt counts down in order: behind stage s + 1's pieces come, in a tile's first stage, the last tile's 32 stores of a whole bf16
+        // epilogue (its loads are back before its first store), which may stay in flight
+        if constexpr (LEFT >= 2 && FIRST && sizeof(T) == 2) {
+            if (whole) asm volatile("s_waitcnt vmcnt(40)" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        } else if constexpr (LEFT >= 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else if constexpr (LEFT == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_nop 1" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        const char* An = smem + (abuf == 2 ? 0 : abuf + 1) * kStageBytes + a_frag0;
+        const char* Bn = smem + (bbuf ^ 1) * kStageBytes + b_frag0;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) {
+            I8_MMA(aY, bY, g >> 2, g & 3)
+            if constexpr (LEFT >= 1) {
+                if (g < 8) bX[g >> 1].c[g & 1] = *reinterpret_cast<const u32x4_t*>(Bn + ((g >> 1) * 32 + (g & 1) * 16) * 128);
+                else aX[(g - 8) >> 1].c[g & 1] = *reinterpret_cast<const u32x4_t*>(An + (((g - 8) >> 1) * 32 + (g & 1) * 16) * 128);
+            }
+            if constexpr (LEFT >= 2) { if (!(g & 1)) I8_B(g >> 1) }
+        }
+        if constexpr (LEFT >= 2) advance();
+    };
+    using std::integral_constant;
+    int s = 0, abuf = 0, bbuf = 0;
+    for (int vid = blockIdx.x; vid < total; vid += gridDim.x) {
+        i32x4_t c[4][4][4];                                       // [32 rows][32 columns][quarter q = 2 (row half) + (column half)]
+        lane_constants();
+        // (read here and not kept from the last tile's last stage, which would cost the epilogue 64 registers)
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+            bX[g >> 1].c[g & 1] = *reinterpret_cast<const u32x4_t*>(smem + bbuf * kStageBytes + b_frag0 + ((g >> 1) * 32 + (g & 1) * 16) * 128);
+            aX[g >> 1].c[g & 1] = *reinterpret_cast<const u32x4_t*>(smem + abuf * kStageBytes + a_frag0 + ((g >> 1) * 32 + (g & 1) * 16) * 128);
+        }
+        auto next = [&]() {
+            ++s;
+            abuf = abuf == 2 ? 0 : abuf + 1;
+            bbuf ^= 1;
+        };
+        if (s + 2 < S) stage(c, abuf, bbuf, integral_constant<int, 2>{}, std::true_type{});
+        else if (s + 2 == S) stage(c, abuf, bbuf, integral_constant<int, 1>{}, std::true_type{});
+        else stage(c, abuf, bbuf, integral_constant<int, 0>{}, std::true_type{});
+        next();
+        const int end = s + nst - 1, full = end < S - 2 ? end : S - 2;
+        while (s < full) { stage(c, abuf, bbuf, integral_constant<int, 2>{}, std::false_type{}); next(); }
+        if (s < end && s + 2 == S) { stage(c, abuf, bbuf, integral_constant<int, 1>{}, std::false_type{}); next(); }
+        if (s < end) { stage(c, abuf, bbuf, integral_constant<int, 0>{}, std::false_type{}); next(); }
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");       // the last MFMAs' results: the compiler does not know they are still on their way
+        int tm, tn, lane_e;
+        tile_coords(xcd_remap(vid, total), tiles_m, tiles_n, tm, tn);
+        asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane_e));
+        const int mr = tm * 256 + wm * 128 + (lane_e & 15), nc = tn * 256 + wn * 128 + 8 * (lane_e >> 4);
+        auto epilogue = [&](auto whole_c) {
+            constexpr bool WHOLE = decltype(whole_c)::value;      // every row and column of the tile is stored, in whole chunks
+            float sx[8], sw[4][8], bs[4][8] = {};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sx[k] = p.sa[WHOLE || mr + 16 * k < p.M ? mr + 16 * k : p.M - 1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                load_cols<WHOLE>(p.sb, nc + 32 * j, p.N, sw[j]);
+                if (p.bias != nullptr) load_cols<WHOLE>(p.bias, nc + 32 * j, p.N, bs[j]);
+            }
+            retire(sx);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { retire(sw[j]); retire(bs[j]); }
+            __builtin_amdgcn_sched_barrier(0);
+            T* row = static_cast<T*>(p.C) + (long)mr * p.ldc + nc;
+#pragma unroll
+            for (int k = 0; k < 8; ++k, row += 16 * p.ldc) {
+                if (WHOLE || mr + 16 * k < p.M) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            v[e] = fmaf((float)c[k >> 1][j][2 * (k & 1) + (e >> 2)][e & 3] * sx[k], sw[j][e], bs[j][e]);
+                            if constexpr (GELU) v[e] = gelu_i8(v[e]);
+                        }
+                        store_cols<T, WHOLE>(row + 32 * j, p.N - nc - 32 * j, v);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            }
+        };
+        whole = tm * 256 + 256 <= p.M && tn * 256 + 256 <= p.N;
+        if (whole) epilogue(std::true_type{});
+        else epilogue(std::false_type{});
+    }
+#undef I8_MMA0
+#undef I8_MMA
+#undef I8_B
+#undef I8_A
+#undef I8_DMA
+}
+
+// Any shape: 64x64 tiles.  v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k of row l & 15, k group l >> 4; result column l & 15, rows 4 (l >> 4) + e
+template <typename T, bool GELU>
 __global__ __launch_bounds__(256) void gemm_i8_kernel(I8Args p) {
     __shared__ __attribute__((aligned(16))) int8_t sA[64 * 64], sB[64 * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -77,35 +420,54 @@ __global__ __launch_bounds__(256) void gemm_i8_kernel(I8Args p) {
         for (int e = 0; e < 4; ++e) {
             const long m = m0 + wave * 16 + 4 * (lane >> 4) + e, n = n0 + j * 16 + (lane & 15);
             if (m < p.M && n < p.N) {
-                float v = (float)acc[j][e] * p.sa[m] * p.sb[n];
-                if (p.bias) v += p.bias[n];
-                if (p.gelu) v = gelu_f(v);
+                float v = fmaf((float)acc[j][e] * p.sa[m], p.sb[n], p.bias ? p.bias[n] : 0.f);
+                if constexpr (GELU) v = gelu_i8(v);
                 static_cast<T*>(p.C)[m * p.ldc + n] = from_f32<T>(v);
             }
         }
 }
 
+// CUs of the device, a multiple of 8 (the tile walk hands every XCD its own stretch of the tile list)
+int cu_count() {
+    int dev = 0, v = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v < 8) return 256;
+    return v & ~7;
+}
+
+template <typename T, bool GELU>
+int launch_product(const I8Args& p, hipStream_t s) {
+    const long tiles = ((long)p.M + 255) / 256 * (((long)p.N + 255) / 256);
+    if (p.M > 64 && tiles >= 128 && tiles <= 0x7fffffffL) {
+        const size_t lds = 5 * kStageBytes;
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_w4_kernel<T, GELU>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return MMSUM_ERR_HIP;
+        const int cus = cu_count();
+        hipLaunchKernelGGL((gemm_i8_w4_kernel<T, GELU>), dim3((unsigned)(tiles < cus ? tiles : cus)), dim3(256), lds, s, p);
+        return ok();
+    }
+    const dim3 grid((unsigned)((p.N + 63L) / 64), (unsigned)((p.M + 63L) / 64));
+    if (grid.y > 65535) return MMSUM_ERR_BAD_SHAPE;
+    hipLaunchKernelGGL((gemm_i8_kernel<T, GELU>), grid, dim3(256), 0, s, p);
+    return ok();
+}
+
 }  // namespace
 
 extern "C" int mmsum_quantize_i8(int dtype, const void* x, long ldx, int M, int K, void* q, long ldq, float* scale, void* stream) {
-    if (M <= 0 || K <= 0 || ldx < K || ldq < K || ldq % 64 || ldq > 0x7fffffc0L) return MMSUM_ERR_BAD_SHAPE;
+    if (M <= 0 || K <= 0 || ldx < K || ldq < K || ldq % 128 || ldq > 0x7fffffc0L) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
     if (((uintptr_t)q & 15) || ((uintptr_t)x & (dtype == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == MMSUM_BF16) hipLaunchKernelGGL((quantize_kernel<bf16_t>), dim3(M), dim3(256), 0, s, (const bf16_t*)x, ldx, K, (int8_t*)q, ldq, scale);
-    else hipLaunchKernelGGL((quantize_kernel<float>), dim3(M), dim3(256), 0, s, (const float*)x, ldx, K, (int8_t*)q, ldq, scale);
-    return ok();
+    if (dtype == MMSUM_BF16) return launch_quantize<bf16_t>(x, ldx, M, K, q, ldq, scale, s);
+    return launch_quantize<float>(x, ldx, M, K, q, ldq, scale, s);
 }
 
 extern "C" int mmsum_gemm_i8(const void* qx, long ldx, const float* sx, const void* qw, long ldw, const float* sw, const float* bias, int dtype_out, void* y, long ldy,
                              int M, int N, int K, int gelu, void* stream) {
-    if (M <= 0 || N <= 0 || K <= 0 || K % 64 || K > 131072 || ldx < K || ldw < K || ldx % 16 || ldw % 16 || ldy < N) return MMSUM_ERR_BAD_SHAPE;
+    if (M <= 0 || N <= 0 || K <= 0 || K % 128 || K > 131072 || ldx < K || ldw < K || ldx % 16 || ldw % 16 || ldx > 0x3fffff || ldw > 0x3fffff || ldy < N) return MMSUM_ERR_BAD_SHAPE;
     if (dtype_out != MMSUM_BF16 && dtype_out != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
     if ((((uintptr_t)qx | (uintptr_t)qw) & 15) || ((uintptr_t)y & (dtype_out == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
-    I8Args p = {static_cast<const int8_t*>(qx), ldx, sx, static_cast<const int8_t*>(qw), ldw, sw, bias, y, ldy, M, N, K, gelu};
-    const dim3 grid((unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64));
-    if (grid.y > 65535) return MMSUM_ERR_BAD_SHAPE;
-    if (dtype_out == MMSUM_BF16) hipLaunchKernelGGL((gemm_i8_kernel<bf16_t>), grid, dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL((gemm_i8_kernel<float>), grid, dim3(256), 0, (hipStream_t)stream, p);
-    return ok();
+    I8Args p = {static_cast<const int8_t*>(qx), ldx, sx, static_cast<const int8_t*>(qw), ldw, sw, bias, y, ldy, M, N, K};
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype_out == MMSUM_BF16) return gelu ? launch_product<bf16_t, true>(p, s) : launch_product<bf16_t, false>(p, s);
+    return gelu ? launch_product<float, true>(p, s) : launch_product<float, false>(p, s);
 }
