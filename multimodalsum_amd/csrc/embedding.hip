@@ -20,10 +20,11 @@ template <> struct Vec<float, 4> { typedef u32x4_t type; };
 template <> struct Vec<bf16_t, 1> { typedef bf16_t type; };
 template <> struct Vec<float, 1> { typedef float type; };
 
+constexpr int kFwdRows = 8;
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const int64_t* __restrict__ ids, const T* __restrict__ E, long lde, T* __restrict__ y, long ldy, long n,
                                                         int V, int D, float scale, int tpr_log2) {
-    constexpr int ROWS = 4;
+    constexpr int ROWS = kFwdRows;
     const int tpr = 1 << tpr_log2, rpb = 256 >> tpr_log2;
     const int c0 = ((int)threadIdx.x & (tpr - 1)) * VEC;
     const long r0 = (long)blockIdx.x * (rpb * ROWS) + (threadIdx.x >> tpr_log2);
@@ -44,7 +45,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const int64_t* __restric
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) t[k] = from_f32<T>(to_f32(t[k]) * scale);
                 __builtin_memcpy(&v[j], t, sizeof(t));
-                *reinterpret_cast<typename Vec<T, VEC>::type*>(y + (r0 + j * rpb) * ldy + c) = v[j];
+                __builtin_nontemporal_store(v[j], reinterpret_cast<typename Vec<T, VEC>::type*>(y + (r0 + j * rpb) * ldy + c));
             }
     }
 }
@@ -78,13 +79,24 @@ __device__ __forceinline__ int wave_rank(volatile int* cnt, uint32_t d, bool act
     return base + before;
 }
 
+// The rows that no id names have to be zero.  Sorting is a chain of short launches that leave the memory idle, so all of dE is cleared in
+// them, by workgroups behind the sorting ones, and the sums write the named rows over it afterwards.
+struct ZeroFill { float* p; long n; int first, blocks; };          // workgroups first .. first + blocks - 1 clear n floats (blocks 0: none)
+template <int NT> __device__ __forceinline__ void zero_fill(const ZeroFill& z) {
+    const long quads = ((uintptr_t)z.p & 15) == 0 ? z.n / 4 : 0;
+    const long t = (long)((int)blockIdx.x - z.first) * NT + threadIdx.x, step = (long)z.blocks * NT;
+    for (long i = t; i < quads; i += step) reinterpret_cast<f32x4_t*>(z.p)[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (long i = quads * 4 + t; i < z.n; i += step) z.p[i] = 0.f;
+}
+
 constexpr int kSub = 1024;               // elements a workgroup ranks at a time (four rounds of its four waves)
 constexpr int kMaxTiles = 256;
 
 // hist[tile][256]: digits of every tile
 template <bool FIRST>
 __global__ __launch_bounds__(256) void sort_hist_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys, int n, int tile, int V, int64_t pad_id, int shift,
-                                                        int* __restrict__ hist) {
+                                                        int* __restrict__ hist, ZeroFill z) {
+    if ((int)blockIdx.x >= z.first) return zero_fill<256>(z);
     __shared__ int h[256];
     h[threadIdx.x] = 0;
     __syncthreads();
@@ -98,14 +110,20 @@ __global__ __launch_bounds__(256) void sort_hist_kernel(const int64_t* __restric
 template <bool FIRST>
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys, const int* __restrict__ pos, int n, int tile,
                                                            int tiles, int V, int64_t pad_id, int shift, const int* __restrict__ hist, uint32_t* __restrict__ okeys,
-                                                           int* __restrict__ opos) {
+                                                           int* __restrict__ opos, ZeroFill z) {
+    if ((int)blockIdx.x >= z.first) return zero_fill<256>(z);
     __shared__ int cnt[4][256], wbase[4][256], scan[256];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int total = 0, before = 0;
-    for (int t = 0; t < tiles; ++t) {
-        const int v = hist[t * 256 + tid];
-        before += t < (int)blockIdx.x ? v : 0;
-        total += v;
+    for (int t0 = 0; t0 < tiles; t0 += 16) {                       // 16 requests at a time: one by one this chain was most of the kernel
+        int v[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) v[u] = t0 + u < tiles ? hist[(t0 + u) * 256 + tid] : 0;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            before += t0 + u < (int)blockIdx.x ? v[u] : 0;
+            total += v[u];
+        }
     }
     scan[tid] = total;
     __syncthreads();
@@ -153,7 +171,8 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const int64_t* __rest
 
 // the whole sort of up to 4096 ids in one workgroup's LDS
 constexpr int kSmall = 4096;
-__global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restrict__ ids, int n, int V, int64_t pad_id, int bits, uint32_t* __restrict__ okeys, int* __restrict__ opos) {
+__global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restrict__ ids, int n, int V, int64_t pad_id, int bits, uint32_t* __restrict__ okeys, int* __restrict__ opos, ZeroFill z) {
+    if ((int)blockIdx.x >= z.first) return zero_fill<1024>(z);
     __shared__ uint32_t lk[2][kSmall];
     __shared__ uint16_t lp[2][kSmall];
     __shared__ int cnt[16][256];
@@ -202,23 +221,44 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restr
     for (int i = tid; i < n; i += 1024) { okeys[i] = lk[cur][i]; opos[i] = lp[cur][i]; }
 }
 
+// up to 512 ids: an element's place is the number of elements in front of it
+constexpr int kTiny = 512;
+__global__ __launch_bounds__(kTiny) void sort_tiny_kernel(const int64_t* __restrict__ ids, int n, int V, int64_t pad_id, uint32_t* __restrict__ okeys, int* __restrict__ opos, ZeroFill z) {
+    if ((int)blockIdx.x >= z.first) return zero_fill<kTiny>(z);
+    __shared__ __attribute__((aligned(16))) uint32_t lk[kTiny];
+    const int i = threadIdx.x;
+    const uint32_t key = i < n ? key_of(ids[i], V, pad_id) : 0xffffffffu;
+    lk[i] = key;
+    __syncthreads();
+    int rank = 0;
+    for (int j = 0; j < n; j += 4) {
+        const u32x4_t k = *reinterpret_cast<const u32x4_t*>(lk + j);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) rank += k[u] < key || (k[u] == key && j + u < i);
+    }
+    if (i < n) { okeys[rank] = key; opos[rank] = i; }
+}
+
 // ---- sums --------------------------------------------------------------------------------------------------------------------------
-// A wave sums a stretch of kStretch sorted positions over 512 columns (eight a lane).  A token whose positions all lie in the stretch is
+// A wave sums a stretch of 8 or 32 sorted positions over 512 columns (eight a lane).  A token whose positions all lie in the stretch is
 // finished; a token that crosses its ends leaves partial sums: part[stretch][0] of the one that began before it, part[stretch][1] of the
 // one that begins in it and goes on (stretch_join_kernel adds those up).
-constexpr int kStretch = 32, kCols = 512;
+constexpr int kCols = 512;
+// positions of a stretch: few of them while that is what keeps the card busy, more where the partial sums' traffic counts
+int stretch_of(long n) { return n <= 8192 ? 8 : 32; }
 
+// eight columns of a lane: VEC: neighbours, else 64 apart
 template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* __restrict__ row, int c, int D, int lane, float (&f)[8]) {
     if constexpr (VEC) {
         if (c < D) {
             if constexpr (sizeof(T) == 2) {
                 T t[8];
-                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(row + c);
+                const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row + c));
                 __builtin_memcpy(t, &v, 16);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) f[k] = to_f32(t[k]);
             } else {
-                const f32x4_t a = *reinterpret_cast<const f32x4_t*>(row + c), b = *reinterpret_cast<const f32x4_t*>(row + c + 4);
+                const f32x4_t a = __builtin_nontemporal_load(reinterpret_cast<const f32x4_t*>(row + c)), b = __builtin_nontemporal_load(reinterpret_cast<const f32x4_t*>(row + c + 4));
 #pragma unroll
                 for (int k = 0; k < 4; ++k) { f[k] = a[k]; f[4 + k] = b[k]; }
             }
@@ -229,25 +269,35 @@ template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* _
             if (c + k * 64 < D) f[k] = to_f32(row[c + k * 64]);
     }
 }
-// column of element k of a lane: VEC: eight neighbours; else: strided by 64 lanes
-template <bool VEC> __device__ __forceinline__ int col_of(int c, int k) { return VEC ? c + k : c + k * 64; }
 template <bool VEC> __device__ __forceinline__ void store8(float* __restrict__ row, int c, int D, const float (&f)[8], float scale, bool accumulate) {
+    if constexpr (VEC) {
+        if (c < D) {
+            f32x4_t* const o = reinterpret_cast<f32x4_t*>(row + c);
+            f32x4_t a = {scale * f[0], scale * f[1], scale * f[2], scale * f[3]}, b = {scale * f[4], scale * f[5], scale * f[6], scale * f[7]};
+            if (accumulate) { a += o[0]; b += o[1]; }
+            o[0] = a;
+            o[1] = b;
+        }
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const int cc = col_of<VEC>(c, k);
-        if (cc < D) row[cc] = accumulate ? row[cc] + scale * f[k] : scale * f[k];
+        for (int k = 0; k < 8; ++k) {
+            const int cc = c + k * 64;
+            if (cc < D) row[cc] = accumulate ? row[cc] + scale * f[k] : scale * f[k];
+        }
     }
 }
 
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void stretch_sum_kernel(const T* __restrict__ dy, long lddy, const uint32_t* __restrict__ keys, const int* __restrict__ pos, int n, int V, int D,
+__global__ __launch_bounds__(256) void stretch_sum_kernel(const T* __restrict__ dy, long lddy, const uint32_t* __restrict__ keys, const int* __restrict__ pos, int n, int sl, int V, int D,
                                                           float scale, int accumulate, float* __restrict__ part, float* __restrict__ dE) {
     const int lane = threadIdx.x & 63;
-    const long st = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long lo = st * kStretch;
+    // the column blocks of a stretch on neighbouring waves: the rows' halves are asked for together
+    const int cols = (D + kCols - 1) / kCols;
+    const long idx = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long st = idx / cols, lo = st * sl;
     if (lo >= n) return;
-    const int len = (int)(n - lo < kStretch ? n - lo : kStretch);
-    const int col0 = blockIdx.y * kCols, c = VEC ? col0 + lane * 8 : col0 + lane;
+    const int len = (int)(n - lo < sl ? n - lo : sl);
+    const int col0 = (int)(idx - st * cols) * kCols, c = VEC ? col0 + lane * 8 : col0 + lane;
     const int Dc = VEC ? D : (D < col0 + kCols ? D : col0 + kCols);
     // the stretch's keys and positions ride on the lanes; lanes 62 / 63 hold the neighbours in front and behind
     uint32_t k = (uint32_t)V;
@@ -255,17 +305,24 @@ __global__ __launch_bounds__(256) void stretch_sum_kernel(const T* __restrict__ 
     if (lane < len) { k = keys[lo + lane]; p = pos[lo + lane]; }
     if (lane == 62 && lo > 0) k = keys[lo - 1];
     if (lane == 63 && lo + len < n) k = keys[lo + len];
+    if ((uint32_t)__builtin_amdgcn_readlane(k, 0) >= (uint32_t)V) return;      // behind every id
+    if (k >= (uint32_t)V) p = __builtin_amdgcn_readlane(p, 0);                // requested with the others, never added
     const uint32_t kbefore = lo > 0 ? (uint32_t)__builtin_amdgcn_readlane(k, 62) : 0xffffffffu;
     const uint32_t kbehind = lo + len < n ? (uint32_t)__builtin_amdgcn_readlane(k, 63) : 0xffffffffu;
     float acc[8] = {};
     constexpr int AHEAD = 8;
-    float f[AHEAD][8];
+    float f[AHEAD][8] = {};
     bool open = false;                                             // the current token began before the stretch
     for (int i0 = 0; i0 < len; i0 += AHEAD) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            if (i0 + u < len && (uint32_t)__builtin_amdgcn_readlane(k, i0 + u) < (uint32_t)V) load8<T, VEC>(dy + (long)__builtin_amdgcn_readlane(p, i0 + u) * lddy, c, Dc, lane, f[u]);
+            load8<T, VEC>(dy + (long)__builtin_amdgcn_readlane(p, i0 + u) * lddy, c, Dc, lane, f[u]);
         }
+        // all of them back before the first store: a wait between the stores below would be for the stores (one row at a time, 25 us of it at 1,152 ids)
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(f[u][e]));
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int i = i0 + u;
@@ -287,63 +344,61 @@ __global__ __launch_bounds__(256) void stretch_sum_kernel(const T* __restrict__ 
     }
 }
 
-// A token that begins in stretch st and goes on: part[st][1] + part[st + 1][0] + ... in order.  Four waves take every fourth stretch, so
-// that a token of many stretches is read four at a time; their sums are added in wave order.
-__global__ __launch_bounds__(256) void stretch_join_kernel(const uint32_t* __restrict__ keys, int n, int V, int D, float scale, int accumulate, const float* __restrict__ part,
+// A token that begins in stretch st and goes on: part[st][1] + part[st + 1][0] + ... in order.  One workgroup a stretch, a thread four
+// columns (VEC: as one vector), up to AHEAD stretches requested at a time: the most frequent tokens of a text (a few per cent of it, over a
+// hundred stretches) are the kernel's tail.
+template <bool VEC>
+__global__ __launch_bounds__(256) void stretch_join_kernel(const uint32_t* __restrict__ keys, int n, int sl, int V, int D, float scale, int accumulate, const float* __restrict__ part,
                                                            float* __restrict__ dE) {
-    __shared__ float sh[4][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long st = blockIdx.x, end = (st + 1) * kStretch;          // end < n: the grid leaves the last stretch out
-    const uint32_t key = keys[end - 1];
-    if (key >= (uint32_t)V || keys[end] != key) return;
-    if (keys[st * kStretch] == key && st > 0 && keys[st * kStretch - 1] == key) return;      // began earlier
-    // last stretch of the token: the first position behind it, by bisection
-    long a = end, b = n;
-    while (a < b) {
-        const long mid = (a + b) / 2;
-        if (keys[mid] == key) a = mid + 1;
-        else b = mid;
-    }
-    const long last = (a - 1) / kStretch;
-    const int c = blockIdx.y * 256 + lane * 4;
-    float acc[4] = {};
-    for (long q = st + wave; q <= last; q += 4) {
-        const float* row = part + (q * 2 + (q == st ? 1 : 0)) * D;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < D) acc[e] += row[c + e];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sh[wave][lane * 4 + e] = acc[e];
-    __syncthreads();
-    const int col = blockIdx.y * 256 + threadIdx.x;
-    if (col < D) {
-        const float s = scale * ((sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]));
-        float* const o = dE + (long)key * D + col;
-        *o = accumulate ? *o + s : s;
-    }
-}
-
-// rows of the table that no token of the batch names: zeros.  A wave takes 16 neighbouring rows, its lanes bisect the sorted keys for them.
-__global__ __launch_bounds__(256) void absent_rows_kernel(const uint32_t* __restrict__ keys, int n, int V, int D, float* __restrict__ dE) {
+    constexpr int AHEAD = 16;
     const int lane = threadIdx.x & 63;
-    const long v0 = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16;
-    if (v0 >= V) return;
-    const uint32_t v = (uint32_t)(v0 + (lane & 15));
-    int a = 0, b = n;
-    while (a < b) {
-        const int mid = (int)(((long)a + b) / 2);
-        if (keys[mid] < v) a = mid + 1;
-        else b = mid;
+    const long st = blockIdx.x, begin = st * sl, end = begin + sl;      // end < n: the grid leaves the last stretch out
+    // five keys at once: the last of the stretch and the first behind it, the first and the one in front, the next stretch's last
+    const uint32_t key = keys[end - 1], behind = keys[end], first = keys[begin], front = keys[begin > 0 ? begin - 1 : 0];
+    long b = end + sl < n ? end + sl : n;
+    const uint32_t far = keys[b - 1];
+    if (key >= (uint32_t)V || behind != key || (begin > 0 && first == key && front == key)) return;      // nothing goes on, or it began earlier
+    long last = st + 1;
+    if (far == key && b < n) {                                     // beyond the next stretch, perhaps: the token's last stretch in [lo, lo + len), 64 probes a step
+        long lo = st + 1, len = (n + sl - 1) / sl - lo;
+        while (len > 1) {
+            const long step = (len + 63) / 64, q = lo + (lane + 1) * step;           // does the token reach stretch q?
+            const uint64_t reach = __ballot(q < lo + len && keys[q * sl < n ? q * sl : n - 1] == key);
+            const int r = __popcll(reach);                                           // sorted: the lanes that say yes come first
+            const long nlo = lo + r * step;
+            len = lo + len - nlo < step ? lo + len - nlo : step;
+            lo = nlo;
+        }
+        last = lo;
     }
-    const uint64_t absent = __ballot(!(a < n && keys[a] == v));
-    for (int r = 0; r < 16 && v0 + r < V; ++r) {
-        if (!((absent >> r) & 1)) continue;
-        float* const row = dE + (v0 + r) * D;
-        if (D % 4 == 0 && ((uintptr_t)dE & 15) == 0) {
-            for (int c = lane * 4; c < D; c += 256) *reinterpret_cast<f32x4_t*>(row + c) = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int c = (int)threadIdx.x * 4; c < D; c += 1024) {
+        f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+        for (long q0 = st; q0 <= last; q0 += AHEAD) {
+            f32x4_t f[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                f[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                if (q0 + u <= last) {
+                    const float* const row = part + ((q0 + u) * 2 + (q0 + u == st ? 1 : 0)) * D;
+                    if constexpr (VEC) f[u] = *reinterpret_cast<const f32x4_t*>(row + c);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < D) f[u][e] = row[c + e];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) s += f[u];
+        }
+        float* const o = dE + (long)key * D + c;
+        if constexpr (VEC) {
+            f32x4_t r = s * scale;
+            if (accumulate) r += *reinterpret_cast<f32x4_t*>(o);
+            *reinterpret_cast<f32x4_t*>(o) = r;
         } else {
-            for (int c = lane; c < D; c += 64) row[c] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < D) o[e] = accumulate ? o[e] + scale * s[e] : scale * s[e];
         }
     }
 }
@@ -355,7 +410,7 @@ int embed_fwd_t(const int64_t* ids, const void* E, long lde, void* y, long ldy, 
     const int steps = vec ? D / VEC : D;
     int lg = 0;
     while ((1 << lg) < steps && lg < 8) ++lg;
-    const long blocks = (n + 4 * (256 >> lg) - 1) / (4 * (256 >> lg));
+    const long blocks = (n + kFwdRows * (256 >> lg) - 1) / (kFwdRows * (256 >> lg));
     if (blocks > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
     if (vec) hipLaunchKernelGGL((embed_fwd_kernel<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, ids, (const T*)E, lde, (T*)y, ldy, n, V, D, scale, lg);
     else hipLaunchKernelGGL((embed_fwd_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, s, ids, (const T*)E, lde, (T*)y, ldy, n, V, D, scale, lg);
@@ -380,37 +435,55 @@ int embed_bwd_t(const void* dy, long lddy, const int64_t* ids, int n, int V, int
     float* part = reinterpret_cast<float*>(ws + 4 * nb + kMaxTiles * 256 * 4);
     int bits = 0;
     while (bits < 32 && ((uint32_t)V >> bits) != 0) ++bits;
-    if (n <= kSmall) {
-        hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(1024), 0, s, ids, n, V, pad_id, bits, k0, p0);
+    const long cells = accumulate ? 0 : (long)V * D;
+    auto fill = [&](int first, int step, int steps) {                // the step-th part of the clearing, about 64 KB a workgroup
+        ZeroFill z = {nullptr, 0, first, 0};
+        const long per = ((cells + steps - 1) / steps + 3) & ~3L, lo = step * per, cnt = lo >= cells ? 0 : (cells - lo < per ? cells - lo : per);
+        if (cnt > 0) {
+            z.p = dE + lo;
+            z.n = cnt;
+            const long want = (cnt + 16383) / 16384;
+            z.blocks = (int)(want < 1024 ? want : 1024);
+        }
+        return z;
+    };
+    if (n <= kTiny) {
+        const ZeroFill z = fill(1, 0, 1);
+        hipLaunchKernelGGL(sort_tiny_kernel, dim3(1 + z.blocks), dim3(kTiny), 0, s, ids, n, V, pad_id, k0, p0, z);
+    } else if (n <= kSmall) {
+        const ZeroFill z = fill(1, 0, 1);
+        hipLaunchKernelGGL(sort_small_kernel, dim3(1 + z.blocks), dim3(1024), 0, s, ids, n, V, pad_id, bits, k0, p0, z);
     } else {
         const SortPlan sp = sort_plan(n);
-        for (int shift = 0; shift < bits; shift += 8) {
+        const int steps = (bits + 7) / 8;
+        for (int shift = 0, step = 0; shift < bits; shift += 8, ++step) {
+            const ZeroFill z0 = {nullptr, 0, sp.tiles, 0}, z1 = fill(sp.tiles, step, steps);      // beside the scatters, the longer ones
+            const dim3 g0(sp.tiles), g1(sp.tiles + z1.blocks);
             if (shift == 0) {
-                hipLaunchKernelGGL((sort_hist_kernel<true>), dim3(sp.tiles), dim3(256), 0, s, ids, nullptr, n, sp.tile, V, pad_id, shift, hist);
-                hipLaunchKernelGGL((sort_scatter_kernel<true>), dim3(sp.tiles), dim3(256), 0, s, ids, nullptr, nullptr, n, sp.tile, sp.tiles, V, pad_id, shift, hist, k0, p0);
+                hipLaunchKernelGGL((sort_hist_kernel<true>), g0, dim3(256), 0, s, ids, nullptr, n, sp.tile, V, pad_id, shift, hist, z0);
+                hipLaunchKernelGGL((sort_scatter_kernel<true>), g1, dim3(256), 0, s, ids, nullptr, nullptr, n, sp.tile, sp.tiles, V, pad_id, shift, hist, k0, p0, z1);
             } else {
-                hipLaunchKernelGGL((sort_hist_kernel<false>), dim3(sp.tiles), dim3(256), 0, s, ids, k0, n, sp.tile, V, pad_id, shift, hist);
-                hipLaunchKernelGGL((sort_scatter_kernel<false>), dim3(sp.tiles), dim3(256), 0, s, ids, k0, p0, n, sp.tile, sp.tiles, V, pad_id, shift, hist, k1, p1);
+                hipLaunchKernelGGL((sort_hist_kernel<false>), g0, dim3(256), 0, s, ids, k0, n, sp.tile, V, pad_id, shift, hist, z0);
+                hipLaunchKernelGGL((sort_scatter_kernel<false>), g1, dim3(256), 0, s, ids, k0, p0, n, sp.tile, sp.tiles, V, pad_id, shift, hist, k1, p1, z1);
                 uint32_t* tk = k0; k0 = k1; k1 = tk;
                 int* tp = p0; p0 = p1; p1 = tp;
             }
         }
     }
-    const long stretches = ((long)n + kStretch - 1) / kStretch;
-    const unsigned cols = (unsigned)((D + kCols - 1) / kCols);
-    const bool vec = D % 8 == 0 && lddy % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)dy & 15) == 0;
-    const dim3 grid((unsigned)((stretches + 3) / 4), cols);
-    if (vec) hipLaunchKernelGGL((stretch_sum_kernel<T, true>), grid, dim3(256), 0, s, (const T*)dy, lddy, k0, p0, n, V, D, scale, accumulate, part, dE);
-    else hipLaunchKernelGGL((stretch_sum_kernel<T, false>), grid, dim3(256), 0, s, (const T*)dy, lddy, k0, p0, n, V, D, scale, accumulate, part, dE);
-    const long joins = ((long)n - 1) / kStretch;                    // stretches with another one behind them
-    if (joins > 0) hipLaunchKernelGGL(stretch_join_kernel, dim3((unsigned)joins, (unsigned)((D + 255) / 256)), dim3(256), 0, s, k0, n, V, D, scale, accumulate, part, dE);
-    if (!accumulate) hipLaunchKernelGGL(absent_rows_kernel, dim3((unsigned)((V + 63L) / 64)), dim3(256), 0, s, k0, n, V, D, dE);
+    const int sl = stretch_of(n);
+    const long stretches = ((long)n + sl - 1) / sl;
+    const long waves = stretches * ((D + kCols - 1) / kCols);
+    const bool vec = D % 8 == 0 && lddy % (16 / (int)sizeof(T)) == 0 && (((uintptr_t)dy | (uintptr_t)dE) & 15) == 0;
+    const dim3 grid((unsigned)((waves + 3) / 4));
+    if (vec) hipLaunchKernelGGL((stretch_sum_kernel<T, true>), grid, dim3(256), 0, s, (const T*)dy, lddy, k0, p0, n, sl, V, D, scale, accumulate, part, dE);
+    else hipLaunchKernelGGL((stretch_sum_kernel<T, false>), grid, dim3(256), 0, s, (const T*)dy, lddy, k0, p0, n, sl, V, D, scale, accumulate, part, dE);
+    const long joins = ((long)n - 1) / sl;                    // stretches with another one behind them
+    if (joins > 0 && vec) hipLaunchKernelGGL((stretch_join_kernel<true>), dim3((unsigned)joins), dim3(256), 0, s, k0, n, sl, V, D, scale, accumulate, part, dE);
+    else if (joins > 0) hipLaunchKernelGGL((stretch_join_kernel<false>), dim3((unsigned)joins), dim3(256), 0, s, k0, n, sl, V, D, scale, accumulate, part, dE);
     return ok();
 }
 
-__global__ __launch_bounds__(256) void zero_kernel(float* __restrict__ p, long n) {
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) p[i] = 0.f;
-}
+__global__ __launch_bounds__(256) void zero_kernel(ZeroFill z) { zero_fill<256>(z); }
 
 }  // namespace
 
@@ -423,7 +496,7 @@ extern "C" int mmsum_embed_fwd(int dtype, const int64_t* ids, const void* E, lon
 
 extern "C" long mmsum_embed_bwd_workspace(long n, int D) {
     if (n < 0 || n > 0x3fffffffL || D <= 0) return 0;
-    return 4 * align16(n * 4) + kMaxTiles * 256 * 4 + (n + kStretch - 1) / kStretch * 2 * D * (long)sizeof(float);
+    return 4 * align16(n * 4) + kMaxTiles * 256 * 4 + (n + stretch_of(n) - 1) / stretch_of(n) * 2 * D * (long)sizeof(float);
 }
 extern "C" int mmsum_embed_bwd(int dtype, const void* dy, long lddy, const int64_t* ids, long n, int V, int D, float scale, int64_t pad_id, int accumulate, float* dE,
                                void* workspace, void* stream) {
@@ -433,7 +506,7 @@ extern "C" int mmsum_embed_bwd(int dtype, const void* dy, long lddy, const int64
     if (((uintptr_t)workspace & 15) || ((uintptr_t)dE & 3) || ((uintptr_t)dy & (dtype == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
     hipStream_t s = (hipStream_t)stream;
     if (n == 0) {
-        if (!accumulate) hipLaunchKernelGGL(zero_kernel, dim3(2048), dim3(256), 0, s, dE, (long)V * D);
+        if (!accumulate) hipLaunchKernelGGL(zero_kernel, dim3(1024), dim3(256), 0, s, ZeroFill{dE, (long)V * D, 0, 1024});
         return ok();
     }
     if (dtype == MMSUM_BF16) return embed_bwd_t<bf16_t>(dy, lddy, ids, (int)n, V, D, scale, pad_id, accumulate, dE, static_cast<char*>(workspace), s);
