@@ -467,6 +467,11 @@ int mmsum_quantize_i8(int dtype, const void* x, long ldx, int M, int K, void* q,
  * 128, at most 131,072; pitches in bytes, multiples of 16 below 4 MiB; qx, qw 16-byte aligned. */
 int mmsum_gemm_i8(const void* qx, long ldx, const float* sx, const void* qw, long ldw, const float* sw, const float* bias, int dtype_out, void* y, long ldy,
                   int M, int N, int K, int gelu, void* stream);
+/* Both steps: x [M, K] of `dtype`, quantised on the way; qw [N, ldw >= K padded to 128] as mmsum_quantize_i8 leaves it.
+ * workspace: mmsum_linear_i8_workspace bytes, 16-byte aligned, any contents. */
+long mmsum_linear_i8_workspace(int M, int K);
+int mmsum_linear_i8(int dtype, const void* x, long ldx, const void* qw, long ldw, const float* sw, const float* bias, int dtype_out, void* y, long ldy, int M,
+                    int N, int K, int gelu, void* workspace, void* stream);
 
 #pragma GCC visibility pop
 #ifdef __cplusplus

@@ -137,6 +137,8 @@ SIGNATURES = {
     "mmsum_embed_bwd": (c_int, [c_int, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_float, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
     "mmsum_quantize_i8": (c_int, [c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_long, c_void_p, c_void_p]),
     "mmsum_gemm_i8": (c_int, [c_void_p, c_long, c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_int, c_void_p, c_long, c_int, c_int, c_int, c_int, c_void_p]),
+    "mmsum_linear_i8_workspace": (c_long, [c_int, c_int]),
+    "mmsum_linear_i8": (c_int, [c_int, c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_int, c_void_p, c_long] + [c_int] * 4 + [c_void_p, c_void_p]),
 }
 
 

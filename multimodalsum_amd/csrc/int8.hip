@@ -427,11 +427,109 @@ __global__ __launch_bounds__(256) void gemm_i8_kernel(I8Args p) {
         }
 }
 
+// Few rows (a decode step): the weights go past the matrix cores once.  A workgroup owns 16 NB columns, its four waves every fourth 64 bytes
+// of k; a wave asks for U steps of weights and activations together, straight into the MFMA's registers, and the four partial sums
+// meet in LDS.  Integer sums: the order does not matter.
+// FUSED: the workgroup quantises the rows itself, into LDS, first -- cheaper than a launch of its own while rows and workgroups are few.
+// Bound: HBM / latency.
+template <typename T, bool GELU, int MB, int NB, bool FUSED, typename X>
+__global__ __launch_bounds__(256) void gemm_i8_few_kernel(I8Args p, const X* __restrict__ x, long ldx, int Kx) {
+    constexpr int U = NB == 1 ? 4 : 2, PITCH = 16 * NB + 4;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int* const part = reinterpret_cast<int*>(smem);                 // [4][16 MB][PITCH]
+    float* const rs = reinterpret_cast<float*>(smem + 4 * 16 * MB * PITCH * 4);
+    char* const xq = smem + 4 * 16 * MB * PITCH * 4 + 64 * MB;      // FUSED: rows of K + 16 bytes
+    const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const long n0 = (long)blockIdx.x * (16 * NB);
+    const int xpitch = p.K + 16;
+    const int steps = p.K / 64;
+    const int8_t* wrow[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) wrow[j] = p.B + (n0 + 16 * j + r16 < p.N ? n0 + 16 * j + r16 : p.N - 1) * p.ldb + kg * 16;
+    i32x4_t b[U][NB];
+    auto load_weights = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int st = s0 + 4 * u < steps ? s0 + 4 * u : s0 < steps ? s0 : 0;      // behind the end: any step, not multiplied
+#pragma unroll
+            for (int j = 0; j < NB; ++j) b[u][j] = *reinterpret_cast<const i32x4_t*>(wrow[j] + (long)st * 64);
+        }
+    };
+    load_weights(wave);                                             // on their way while the rows are quantised
+    if constexpr (FUSED) {
+        for (int m = wave; m < p.M; m += 4) {
+            uint32_t top = 0;
+            for (int k = lane * 8; k < Kx; k += 512) {
+                float f[8];
+                load_row8(x + m * ldx, k, Kx, f);
+                top = top8(top, f);
+            }
+            const RowQuant r = row_quant(wave_top(top));
+            for (int k = lane * 8; k < p.K; k += 512) {
+                float f[8];
+                load_row8(x + m * ldx, k, Kx, f);
+                *reinterpret_cast<u32x2_t*>(xq + m * xpitch + k) = pack8(f, r);
+            }
+            if (lane == 0) rs[m] = r.scale;
+        }
+        __syncthreads();
+    } else if (tid < p.M) rs[tid] = p.sa[tid];
+    i32x4_t acc[MB][NB] = {};
+    for (int s0 = wave; s0 < steps; s0 += 4 * U) {
+        if (s0 != wave) load_weights(s0);
+        i32x4_t a[U][MB];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int st = s0 + 4 * u < steps ? s0 + 4 * u : s0;
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const int m = 16 * i + r16 < p.M ? 16 * i + r16 : p.M - 1;
+                if constexpr (FUSED) a[u][i] = *reinterpret_cast<const i32x4_t*>(xq + m * xpitch + st * 64 + kg * 16);
+                else a[u][i] = *reinterpret_cast<const i32x4_t*>(p.A + m * p.lda + st * 64 + kg * 16);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + 4 * u < steps)
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[u][j], a[u][i], acc[i][j], 0, 0, 0);
+    }
+    // weights as the A operand: a lane holds columns 4 kg .. + 3 of row r16
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) *reinterpret_cast<i32x4_t*>(part + (wave * 16 * MB + 16 * i + r16) * PITCH + 16 * j + 4 * kg) = acc[i][j];
+    __syncthreads();
+    for (int o = tid; o < p.M * 16 * NB; o += 256) {
+        const int m = o / (16 * NB), c = o % (16 * NB);
+        const long n = n0 + c;
+        if (n >= p.N) continue;
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sum += part[(w * 16 * MB + m) * PITCH + c];
+        float v = fmaf((float)sum * rs[m], p.sb[n], p.bias ? p.bias[n] : 0.f);
+        if constexpr (GELU) v = gelu_i8(v);
+        static_cast<T*>(p.C)[m * p.ldc + n] = from_f32<T>(v);
+    }
+}
+
 // CUs of the device, a multiple of 8 (the tile walk hands every XCD its own stretch of the tile list)
 int cu_count() {
     int dev = 0, v = 0;
     if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v < 8) return 256;
     return v & ~7;
+}
+
+template <typename T, bool GELU, int MB, int NB, bool FUSED, typename X>
+int launch_few(const I8Args& p, const X* x, long ldx, int Kx, hipStream_t s) {
+    const size_t lds = 4 * 16 * MB * (16 * NB + 4) * 4 + 64 * MB + (FUSED ? (size_t)p.M * (p.K + 16) : 0);
+    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_few_kernel<T, GELU, MB, NB, FUSED, X>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+        return MMSUM_ERR_HIP;
+    hipLaunchKernelGGL((gemm_i8_few_kernel<T, GELU, MB, NB, FUSED, X>), dim3((unsigned)((p.N + 16L * NB - 1) / (16 * NB))), dim3(256), lds, s, p, x, ldx, Kx);
+    return ok();
 }
 
 template <typename T, bool GELU>
@@ -444,10 +542,31 @@ int launch_product(const I8Args& p, hipStream_t s) {
         hipLaunchKernelGGL((gemm_i8_w4_kernel<T, GELU>), dim3((unsigned)(tiles < cus ? tiles : cus)), dim3(256), lds, s, p);
         return ok();
     }
+    if (p.M <= 64) {
+        // wide workgroups where there are still enough of them for every CU: they read the activations less often
+        const bool wide = p.N >= 32768;
+        if (p.M <= 16) return wide ? launch_few<T, GELU, 1, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 1, 1, false, float>(p, nullptr, 0, 0, s);
+        if (p.M <= 32) return wide ? launch_few<T, GELU, 2, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 2, 1, false, float>(p, nullptr, 0, 0, s);
+        return wide ? launch_few<T, GELU, 4, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 4, 1, false, float>(p, nullptr, 0, 0, s);
+    }
     const dim3 grid((unsigned)((p.N + 63L) / 64), (unsigned)((p.M + 63L) / 64));
     if (grid.y > 65535) return MMSUM_ERR_BAD_SHAPE;
     hipLaunchKernelGGL((gemm_i8_kernel<T, GELU>), grid, dim3(256), 0, s, p);
     return ok();
+}
+
+// Quantisation and product.  In one launch for up to 16 rows of up to 4,096 values and few columns: there the launch costs more than every
+// workgroup's quantising all rows.
+template <typename T, bool GELU>
+int launch_linear(int dtype, const void* x, long ldx, I8Args p, int Kx, hipStream_t s) {
+    if (p.M <= 16 && p.K <= 4096 && p.N <= 4096) {
+        if (dtype == MMSUM_BF16) return launch_few<T, GELU, 1, 1, true, bf16_t>(p, static_cast<const bf16_t*>(x), ldx, Kx, s);
+        return launch_few<T, GELU, 1, 1, true, float>(p, static_cast<const float*>(x), ldx, Kx, s);
+    }
+    int8_t* const q = const_cast<int8_t*>(p.A);
+    float* const scale = const_cast<float*>(p.sa);
+    const int rc = dtype == MMSUM_BF16 ? launch_quantize<bf16_t>(x, ldx, p.M, Kx, q, p.K, scale, s) : launch_quantize<float>(x, ldx, p.M, Kx, q, p.K, scale, s);
+    return rc == MMSUM_OK ? launch_product<T, GELU>(p, s) : rc;
 }
 
 }  // namespace
@@ -470,4 +589,21 @@ extern "C" int mmsum_gemm_i8(const void* qx, long ldx, const float* sx, const vo
     hipStream_t s = (hipStream_t)stream;
     if (dtype_out == MMSUM_BF16) return gelu ? launch_product<bf16_t, true>(p, s) : launch_product<bf16_t, false>(p, s);
     return gelu ? launch_product<float, true>(p, s) : launch_product<float, false>(p, s);
+}
+
+extern "C" long mmsum_linear_i8_workspace(int M, int K) { return M <= 0 || K <= 0 || K > 131072 ? 0 : M * ((K + 127L) / 128 * 128 + 4L); }
+extern "C" int mmsum_linear_i8(int dtype, const void* x, long ldx, const void* qw, long ldw, const float* sw, const float* bias, int dtype_out, void* y, long ldy, int M,
+                               int N, int K, int gelu, void* workspace, void* stream) {
+    if (M <= 0 || N <= 0 || K <= 0 || K > 131072 || ldx < K || ldw < (K + 127L) / 128 * 128 || ldw % 16 || ldw > 0x3fffff || ldy < N) return MMSUM_ERR_BAD_SHAPE;
+    if ((dtype != MMSUM_BF16 && dtype != MMSUM_F32) || (dtype_out != MMSUM_BF16 && dtype_out != MMSUM_F32)) return MMSUM_ERR_BAD_DTYPE;
+    if (workspace == nullptr) return MMSUM_ERR_WORKSPACE;
+    if (((uintptr_t)x & (dtype == MMSUM_BF16 ? 1 : 3)) || (((uintptr_t)qw | (uintptr_t)workspace) & 15) || ((uintptr_t)y & (dtype_out == MMSUM_BF16 ? 1 : 3)))
+        return MMSUM_ERR_BAD_ALIGN;
+    const int Kp = (K + 127) / 128 * 128;
+    int8_t* const q = static_cast<int8_t*>(workspace);
+    const float* const scale = reinterpret_cast<const float*>(q + (long)M * Kp);
+    I8Args p = {q, Kp, scale, static_cast<const int8_t*>(qw), ldw, sw, bias, y, ldy, M, N, Kp};
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype_out == MMSUM_BF16) return gelu ? launch_linear<bf16_t, true>(dtype, x, ldx, p, K, s) : launch_linear<bf16_t, false>(dtype, x, ldx, p, K, s);
+    return gelu ? launch_linear<float, true>(dtype, x, ldx, p, K, s) : launch_linear<float, false>(dtype, x, ldx, p, K, s);
 }

@@ -79,19 +79,27 @@ template <int NT> __device__ __forceinline__ float block_sum(float v, float* sh)
 // What the policy loss takes per token besides the logits
 struct PolicyArgs {
     const float* old_logp; const float* ref_logp; const float* adv;
-    const int* counts;              // counted tokens: of kCountParts stretches of the batch (token mean) or of every sequence (sequence mean)
+    const int64_t* labels; int V;
+    const int* counts;              // counted tokens: of kCountParts stretches of the batch (token mean) or of every sequence (sequence mean); NULL: counted here
     int adv_per_token, seq_mean, N, T;
     float lo, hi, kl_coef;
     float* terms;                   // [3][R]: weighted loss, KL estimate, clipped indicator of every row
 };
 constexpr int kCountParts = 64;
 
+// 1 / (the tokens the mean is over); whole waves come here together, a wave's rows are of one sequence or `row` is the lane's own with counts
 __device__ __forceinline__ float policy_weight(const PolicyArgs& p, int row, int lane) {
-    if (p.seq_mean) return 1.f / (fmaxf((float)p.counts[row / p.T], 1.f) * (float)p.N);
-    int n = p.counts[lane];
+    const int seq = row / p.T;
+    int n = 0;
+    if (p.counts == nullptr) {
+        const long lo = p.seq_mean ? (long)seq * p.T : 0, hi = p.seq_mean ? lo + p.T : (long)p.N * p.T;
+        for (long i = lo + lane; i < hi; i += 64) { const int64_t y = p.labels[i]; n += y >= 0 && y < p.V; }
+    } else if (p.seq_mean) {
+        return 1.f / (fmaxf((float)p.counts[seq], 1.f) * (float)p.N);
+    } else n = p.counts[lane];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
-    return 1.f / fmaxf((float)n, 1.f);
+    return 1.f / (fmaxf((float)n, 1.f) * (p.seq_mean ? (float)p.N : 1.f));
 }
 // loss = max(-A r, -A clip(r, lo, hi)) + kl (e^d - d - 1) with r = exp(log p - old), d = ref - log p; returns dL / d log p.
 // The bounded branch carries no gradient; the KL estimate (non-negative, unbiased under the sampling policy) gives 1 - e^d.
@@ -345,27 +353,56 @@ __device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1
 
 // Pair i = sequences (i, P + i): h = beta ((S_i - ref_i) - (S_{P+i} - ref_{P+i})), loss_i = (1 - e) softplus(-h) + e softplus(h),
 // d loss_i / d h = e - sigmoid(-h).  coef[n] = d (mean loss) / d log p of every counted token of sequence n.
-__global__ __launch_bounds__(256) void pair_kernel(const float* logp, const int64_t* labels, const float* ref, int P, int T, int V, float beta, float smoothing,
-                                                   int average, int pair0, int pairs, float* seq, float* margins, float* pair_loss, float* coef) {
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (i >= pairs) return;
-    const int p = pair0 + i;
-    float sc, sr;
+// loss (may be NULL): the mean over the pairs, written by a single workgroup of 16 waves that takes them in turn; else pair_loss is left for a mean.
+struct PairArgs {
+    const float* logp; const int64_t* labels; const float* ref;
+    int P, T, V, average;
+    float beta, smoothing;
+    float* seq; float* margins; float* pair_loss; float* coef; float* loss;
+};
+struct PairTerms { float sc, sr, h, dc, dr; };
+__device__ __forceinline__ PairTerms pair_terms(const PairArgs& a, int p, int lane) {
+    PairTerms t;
     int nc, nr;
-    sequence_sum(logp, labels, p, T, V, lane, sc, nc);
-    sequence_sum(logp, labels, P + p, T, V, lane, sr, nr);
-    if (lane != 0) return;
-    const float ic = average ? 1.f / fmaxf((float)nc, 1.f) : 1.f, ir = average ? 1.f / fmaxf((float)nr, 1.f) : 1.f;
-    sc *= ic;
-    sr *= ir;
-    const float h = beta * ((sc - (ref ? ref[p] : 0.f)) - (sr - (ref ? ref[P + p] : 0.f)));
-    const float dh = (smoothing - 1.f / (1.f + expf(h))) * beta / (float)P;
-    seq[p] = sc;
-    seq[P + p] = sr;
-    margins[p] = h;
-    pair_loss[p] = (smoothing == 0.f) ? softplus(-h) : (1.f - smoothing) * softplus(-h) + smoothing * softplus(h);
-    coef[p] = dh * ic;
-    coef[P + p] = -dh * ir;
+    sequence_sum(a.logp, a.labels, p, a.T, a.V, lane, t.sc, nc);
+    sequence_sum(a.logp, a.labels, a.P + p, a.T, a.V, lane, t.sr, nr);
+    const float ic = a.average ? 1.f / fmaxf((float)nc, 1.f) : 1.f, ir = a.average ? 1.f / fmaxf((float)nr, 1.f) : 1.f;
+    t.sc *= ic;
+    t.sr *= ir;
+    t.h = a.beta * ((t.sc - (a.ref ? a.ref[p] : 0.f)) - (t.sr - (a.ref ? a.ref[a.P + p] : 0.f)));
+    const float dh = (a.smoothing - 1.f / (1.f + expf(t.h))) * a.beta / (float)a.P;
+    t.dc = dh * ic;
+    t.dr = -dh * ir;
+    return t;
+}
+__device__ __forceinline__ float pair_loss_of(const PairArgs& a, float h) {
+    return a.smoothing == 0.f ? softplus(-h) : (1.f - a.smoothing) * softplus(-h) + a.smoothing * softplus(h);
+}
+__global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
+    __shared__ float sh[16];
+    const int lane = threadIdx.x & 63, waves = blockDim.x / 64;
+    float mean = 0.f;
+    for (int p = blockIdx.x * waves + (threadIdx.x >> 6); p < a.P; p += gridDim.x * waves) {
+        const PairTerms t = pair_terms(a, p, lane);
+        const float l = pair_loss_of(a, t.h);
+        mean += l;
+        if (lane == 0) {
+            a.seq[p] = t.sc;
+            a.seq[a.P + p] = t.sr;
+            a.margins[p] = t.h;
+            a.pair_loss[p] = l;
+            a.coef[p] = t.dc;
+            a.coef[a.P + p] = t.dr;
+        }
+    }
+    if (a.loss != nullptr) {                                       // one workgroup of 16 waves
+        if (lane == 0) sh[threadIdx.x >> 6] = mean;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < 16; ++w) mean += sh[w];
+            *a.loss = mean / (float)a.P;
+        }
+    }
 }
 
 // out[j] = scale * sum of x[j * n .. (j + 1) * n)
@@ -476,8 +513,14 @@ extern "C" int mmsum_preference_pairs(const float* logp, const int64_t* labels, 
                                       float* seq, float* margins, float* pair_loss, float* coef, float* loss, void* stream) {
     if (P <= 0 || T <= 0 || V <= 0 || 2L * P * T > 0x7fffffffL || !(smoothing >= 0.f && smoothing <= 1.f)) return MMSUM_ERR_BAD_SHAPE;
     hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(pair_kernel, dim3((P + 3) / 4), dim3(256), 0, s, logp, labels, ref, P, T, V, beta, smoothing, average, 0, P, seq, margins, pair_loss, coef);
-    hipLaunchKernelGGL(rows_mean_kernel, dim3(1), dim3(1024), 0, s, pair_loss, (long)P, 1.f / (float)P, loss);
+    PairArgs a = {logp, labels, ref, P, T, V, average, beta, smoothing, seq, margins, pair_loss, coef, loss};
+    if ((long)P * T <= 32768) {                                    // a single workgroup is done before a second launch would begin
+        hipLaunchKernelGGL(pair_kernel, dim3(1), dim3(1024), 0, s, a);
+    } else {
+        a.loss = nullptr;
+        hipLaunchKernelGGL(pair_kernel, dim3((P + 3) / 4), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(rows_mean_kernel, dim3(1), dim3(1024), 0, s, pair_loss, (long)P, 1.f / (float)P, loss);
+    }
     return ok();
 }
 
@@ -504,11 +547,14 @@ extern "C" int mmsum_preference_loss(int dtype, const void* logits, long ld, con
 extern "C" long mmsum_policy_workspace(int N, int T) {
     return N <= 0 || T <= 0 ? 0 : 3L * N * T * (long)sizeof(float) + (long)(N > kCountParts ? N : kCountParts) * (long)sizeof(int);
 }
-static int policy_setup(PolicyArgs& p, const float* old_logp, const float* ref_logp, const float* adv, int adv_per_token, int N, int T, float clip_low,
+// Rows of the logits count their sequence (or the small batch) themselves, under the latency of the row: a launch less
+static bool rows_count(int N, int T, int seq_mean) { return seq_mean ? T <= 2048 : (long)N * T <= 1024; }
+static int policy_setup(PolicyArgs& p, const int64_t* labels, int V, const float* old_logp, const float* ref_logp, const float* adv, int adv_per_token, int N, int T, float clip_low,
                         float clip_high, float kl_coef, int seq_mean, void* workspace) {
     if (!(clip_low >= 0.f) || !(clip_high >= 0.f) || kl_coef != kl_coef) return MMSUM_ERR_BAD_SHAPE;
     if (workspace == nullptr) return MMSUM_ERR_WORKSPACE;
     if ((uintptr_t)workspace & 15) return MMSUM_ERR_BAD_ALIGN;
+    p.labels = labels; p.V = V;
     p.old_logp = old_logp; p.ref_logp = ref_logp; p.adv = adv;
     p.terms = static_cast<float*>(workspace);
     p.counts = reinterpret_cast<int*>(p.terms + 3L * N * T);
@@ -521,7 +567,7 @@ extern "C" int mmsum_policy_terms(const float* logp, const int64_t* labels, cons
                                   int T, int V, float clip_low, float clip_high, float kl_coef, int seq_mean, float* out, float* coef, void* workspace, void* stream) {
     if (N <= 0 || T <= 0 || V <= 0 || (long)N * T > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
     PolicyArgs p = {};
-    int rc = policy_setup(p, old_logp, ref_logp, adv, adv_per_token, N, T, clip_low, clip_high, kl_coef, seq_mean, workspace);
+    int rc = policy_setup(p, labels, V, old_logp, ref_logp, adv, adv_per_token, N, T, clip_low, clip_high, kl_coef, seq_mean, workspace);
     hipStream_t s = (hipStream_t)stream;
     const long R = (long)N * T;
     if (rc == MMSUM_OK) rc = launch_counts(labels, N, T, V, seq_mean, const_cast<int*>(p.counts), s);
@@ -538,10 +584,11 @@ extern "C" int mmsum_policy_loss(int dtype, const void* logits, long ld, const i
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
     if (bad_align(dtype, logits) || bad_align(dtype, dlogits)) return MMSUM_ERR_BAD_ALIGN;
     PolicyArgs p = {};
-    int rc = policy_setup(p, old_logp, ref_logp, adv, adv_per_token, N, T, clip_low, clip_high, kl_coef, seq_mean, workspace);
+    int rc = policy_setup(p, labels, V, old_logp, ref_logp, adv, adv_per_token, N, T, clip_low, clip_high, kl_coef, seq_mean, workspace);
     hipStream_t s = (hipStream_t)stream;
     const int R = N * T;
-    if (rc == MMSUM_OK) rc = launch_counts(labels, N, T, V, seq_mean, const_cast<int*>(p.counts), s);
+    if (rows_count(N, T, seq_mean)) p.counts = nullptr;
+    else if (rc == MMSUM_OK) rc = launch_counts(labels, N, T, V, seq_mean, const_cast<int*>(p.counts), s);
     if (rc != MMSUM_OK) return rc;
     if (dtype == MMSUM_BF16) {
         RowArgs<bf16_t> a = row_args<bf16_t>(logits, ld, labels, V, logp, nullptr, R);

@@ -39,7 +39,6 @@ class Int8Linear(nn.Module):
         rows = x.reshape(-1, self.in_features)
         if self.in_features > 1 and rows.stride(1) != 1:
             rows = rows.contiguous()
-        q, scale = kn.quantize_rows(rows)
         y = torch.empty(rows.shape[0], self.out_features, dtype=self.out_dtype or x.dtype, device=x.device)
-        kn.gemm_i8(q, scale, self.qweight, self.scale, y, self.bias, self.gelu)
+        kn.linear_i8(rows, self.qweight, self.scale, y, self.bias, self.gelu)
         return y.reshape(*x.shape[:-1], self.out_features)

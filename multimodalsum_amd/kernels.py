@@ -587,50 +587,53 @@ def gemm_pair(xs, x2s, ws, outs, biases):
 # their workspaces from the allocator call by call (nothing is shared between streams or captured graphs) and launch on the device that the
 # tensors live on, whichever is current.
 # ---------------------------------------------------------------------------------------------------------------------------------
-def _need(ok, message):
+def _need(ok, message, *args):
     if not ok:
-        raise ValueError(message)
+        raise ValueError(message % args)
 
 
 def _device(*tensors):
-    dev = None
+    index = -1
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()
+        if i < 0:
             raise RuntimeError("libmmsum_hip kernels need device tensors (no CPU fallback exists)")
-        if dev is None:
-            dev = t.device
-        _need(t.device == dev, "tensors on different devices: %s and %s" % (dev, t.device))
-    return dev
+        if index < 0:
+            index = i
+        _need(i == index, "tensors on different devices: %d and %d", index, i)
+    return torch.device("cuda", index)
 
 
 def _launch(name, device, *args):
-    if device.index == torch.cuda.current_device():
-        rc = getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream)
+    fn, index = getattr(lib, name), device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            rc = getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream)
-    check(rc, name)
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)
 
 
 def _rows_of(t, what):
     """[N, T, V] with unit inner stride and one row pitch -> (N, T, V, pitch)."""
-    _need(t.dim() == 3, "%s: [N, T, V] expected, got %s" % (what, tuple(t.shape)))
+    _need(t.dim() == 3, "%s: [N, T, V] expected, got %s", what, t.shape)
     _dt(t)
     N, T, V = t.shape
-    _need(N > 0 and T > 0 and V > 0, "%s: empty (%s)" % (what, tuple(t.shape)))
-    _need(V == 1 or t.stride(2) == 1, "%s: unit inner stride expected" % what)
+    _need(N > 0 and T > 0 and V > 0, "%s: empty (%s)", what, t.shape)
+    _need(V == 1 or t.stride(2) == 1, "%s: unit inner stride expected", what)
     ld = t.stride(1) if T > 1 else (t.stride(0) if N > 1 else V)
-    _need(ld >= V and (N == 1 or t.stride(0) == T * ld), "%s: rows of one pitch expected (strides %s)" % (what, tuple(t.stride())))
-    _need(N * T < 2 ** 31, "%s: too many rows" % what)
+    _need(ld >= V and (N == 1 or t.stride(0) == T * ld), "%s: rows of one pitch expected (strides %s)", what, t.stride())
+    _need(N * T < 2 ** 31, "%s: too many rows", what)
     return N, T, V, ld
 
 
 def _labels_of(labels, N, T):
     if labels.dtype != torch.int64:
         raise TypeError("labels: int64 expected, got %s" % labels.dtype)
-    _need(labels.shape == (N, T), "labels: shape %s expected, got %s" % ((N, T), tuple(labels.shape)))
+    _need(labels.shape == (N, T), "labels: shape %s expected, got %s", (N, T), labels.shape)
     return labels.contiguous()
 
 
@@ -639,13 +642,19 @@ def _f32_of(t, shape, what):
         return None
     if t.dtype != torch.float32:
         raise TypeError("%s: float32 expected, got %s" % (what, t.dtype))
-    _need(tuple(t.shape) == tuple(shape), "%s: shape %s expected, got %s" % (what, tuple(shape), tuple(t.shape)))
+    _need(t.shape == shape, "%s: shape %s expected, got %s", what, shape, t.shape)
     return t.contiguous()
 
 
 def _span(t):
     n = 1 + sum((s - 1) * abs(st) for s, st in zip(t.shape, t.stride())) if t.numel() else 0
     return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _apart(x, out):
+    if x.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
+        a, b = _span(x), _span(out)
+        _need(a[0] >= b[1] or b[0] >= a[1], "out overlaps the input")
 
 
 def _dlogits_of(dlogits, logits, N, T, V, ld):
@@ -657,7 +666,7 @@ def _dlogits_of(dlogits, logits, N, T, V, ld):
     if dlogits.dtype != logits.dtype:
         raise TypeError("dlogits: %s expected, got %s" % (logits.dtype, dlogits.dtype))
     n, t, W, ldd = _rows_of(dlogits, "dlogits")
-    _need((n, t) == (N, T) and W >= V, "dlogits: [%d, %d, >= %d] expected, got %s" % (N, T, V, tuple(dlogits.shape)))
+    _need((n, t) == (N, T) and W >= V, "dlogits: [%d, %d, >= %d] expected, got %s", N, T, V, dlogits.shape)
     a, b = _span(logits), _span(dlogits)
     _need(a[0] >= b[1] or b[0] >= a[1] or (a[0] == b[0] and ld == ldd), "dlogits overlaps the logits without being them")
     return dlogits, ldd, W
@@ -702,8 +711,8 @@ def sequence_logprob(logp, labels, V, average=False):
 
 
 def _pairs_of(N, ref, smoothing):
-    _need(N % 2 == 0, "preference loss: [chosen; rejected] sequences expected, got an odd number (%d)" % N)
-    _need(0.0 <= smoothing <= 1.0, "label_smoothing: 0 .. 1 expected, got %r" % (smoothing,))
+    _need(N % 2 == 0, "preference loss: [chosen; rejected] sequences expected, got an odd number (%d)", N)
+    _need(0.0 <= smoothing <= 1.0, "label_smoothing: 0 .. 1 expected, got %r", smoothing)
     return N // 2, _f32_of(ref, (N,), "ref_logps")
 
 
@@ -734,7 +743,7 @@ def preference_loss(logits, labels, ref, beta, smoothing, average, dlogits=None)
 
 
 def _policy_of(N, T, old, adv, ref, clip_low, clip_high, kl_coef, reduction):
-    _need(reduction in ("token", "sequence"), "reduction: 'token' or 'sequence' expected, got %r" % (reduction,))
+    _need(reduction in ("token", "sequence"), "reduction: 'token' or 'sequence' expected, got %r", reduction)
     _need(clip_low >= 0.0 and clip_high >= 0.0, "clip_low, clip_high: not negative")
     _need(kl_coef == kl_coef and (kl_coef == 0.0 or ref is not None), "kl_coef without ref_logps")
     return _f32_of(old, (N, T), "old_logps"), _f32_of(adv, (N,) if adv.dim() == 1 else (N, T), "advantages"), _f32_of(ref, (N, T), "ref_logps")
@@ -774,9 +783,9 @@ def _ids_of(ids):
 
 
 def _pitch2(t, what):
-    _need(t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1), "%s: [rows, columns] with unit inner stride expected" % what)
+    _need(t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1), "%s: [rows, columns] with unit inner stride expected", what)
     ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    _need(ld >= t.shape[1], "%s: overlapping rows" % what)
+    _need(ld >= t.shape[1], "%s: overlapping rows", what)
     return ld
 
 
@@ -797,14 +806,14 @@ def embed_bwd(dy, ids, V, scale=1.0, pad_id=None, out=None, accumulate=False):
     """out f32 [V, D] (+)= scale * sum of dy rows by id (pad_id and ids outside 0 .. V-1: none)."""
     flat = _ids_of(ids).contiguous()
     D, n = dy.shape[-1], flat.numel()
-    _need(dy.shape[:-1] == ids.shape, "dy: shape %s expected, got %s" % ((*ids.shape, D), tuple(dy.shape)))
-    _need(V > 0 and D > 0 and n < 2 ** 30, "embed_bwd: %d ids into [%d, %d]" % (n, V, D))
+    _need(dy.shape[:-1] == ids.shape, "dy: shape %s expected, got %s", (*ids.shape, D), dy.shape)
+    _need(V > 0 and D > 0 and n < 2 ** 30, "embed_bwd: %d ids into [%d, %d]", n, V, D)
     dy = dy.reshape(-1, D)
     if n and D > 1 and dy.stride(1) != 1:
         dy = dy.contiguous()
     lddy = _pitch2(dy, "dy") if n else D
     _need(not accumulate or out is not None, "accumulate without out")
-    _need(out is None or (out.dtype == torch.float32 and out.shape == (V, D) and out.is_contiguous()), "out: packed float32 [%d, %d] expected" % (V, D))
+    _need(out is None or (out.dtype == torch.float32 and out.shape == (V, D) and out.is_contiguous()), "out: packed float32 [%d, %d] expected", V, D)
     _dt(dy)
     dev = _device(dy, ids, out)
     if out is None:
@@ -821,7 +830,7 @@ def quantize_rows(x):
     """x [M, K] -> (q int8 [M, Kp] = 127 x / max |x| of the row, ties to even, Kp = K padded with zeros; scale f32 [M] = max |x| / 127)."""
     ldx = _pitch2(x, "x")
     M, K = x.shape
-    _need(0 < K <= 131072, "quantize_rows: K = %d, 1 .. 131072 expected" % K)
+    _need(0 < K <= 131072, "quantize_rows: K = %d, 1 .. 131072 expected", K)
     _dt(x)
     dev = _device(x)
     Kp = -(-K // I8_K_STEP) * I8_K_STEP
@@ -838,11 +847,30 @@ def gemm_i8(qx, sx, qw, sw, out, bias=None, gelu=False):
         if t.dtype != torch.int8:
             raise TypeError("%s: int8 expected, got %s" % (what, t.dtype))
     _need(qw.shape[1] == K and K % I8_K_STEP == 0 and 0 < K <= 131072, "gemm_i8: operands as quantize_rows leaves them expected")
-    _need(out.shape == (M, N), "out: shape %s expected, got %s" % ((M, N), tuple(out.shape)))
+    _need(out.shape == (M, N), "out: shape %s expected, got %s", (M, N), out.shape)
     sx, sw, bias = _f32_of(sx, (M,), "sx"), _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias")
     ldx, ldw, ldy = _pitch2(qx, "qx"), _pitch2(qw, "qw"), _pitch2(out, "out")
     _dt(out)
     dev = _device(qx, sx, qw, sw, out, bias)
     if M and N:
         _launch("mmsum_gemm_i8", dev, _p(qx), ldx, _p(sx), _p(qw), ldw, _p(sw), _p(bias), _dt(out), _p(out), ldy, M, N, K, int(bool(gelu)))
+    return out
+
+
+def linear_i8(x, qw, sw, out, bias=None, gelu=False):
+    """quantize_rows and gemm_i8 in one call: out [M, N] = x [M, K] . W^T (+ bias) (GELU), W as quantize_rows left it."""
+    (M, K), N = x.shape, qw.shape[0]
+    if qw.dtype != torch.int8:
+        raise TypeError("qw: int8 expected, got %s" % qw.dtype)
+    _need(0 < K <= 131072 and qw.shape[1] == -(-K // I8_K_STEP) * I8_K_STEP, "linear_i8: weights as quantize_rows leaves them expected")
+    _need(out.shape == (M, N), "out: shape %s expected, got %s", (M, N), out.shape)
+    sw, bias = _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias")
+    ldx, ldw, ldy = _pitch2(x, "x"), _pitch2(qw, "qw"), _pitch2(out, "out")
+    dt, dto = _dt(x), _dt(out)
+    dev = _device(x, qw, sw, out, bias)
+    _apart(x, out)
+    if M:
+        ws = torch.empty(M * (qw.shape[1] + 4), dtype=torch.uint8, device=dev)
+        _launch("mmsum_linear_i8", dev, dt, x.data_ptr(), ldx, qw.data_ptr(), ldw, sw.data_ptr(), None if bias is None else bias.data_ptr(), dto, out.data_ptr(), ldy, M, N, K,
+                int(bool(gelu)), ws.data_ptr())
     return out

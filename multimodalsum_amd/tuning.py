@@ -133,7 +133,9 @@ class _EmbeddingFn(torch.autograd.Function):
 def scaled_embedding(ids, table, scale=1.0, padding_idx=None):
     """scale * table[ids] (f32 or bf16 table, int64 ids of any shape; ids outside the table give zero rows), differentiable with respect to the table
     (padding_idx: no gradient)."""
-    return _EmbeddingFn.apply(ids, table, float(scale), padding_idx)
+    if table.requires_grad and torch.is_grad_enabled():
+        return _EmbeddingFn.apply(ids, table, float(scale), padding_idx)
+    return kn.embed_fwd(ids, table, float(scale))
 
 
 class ScaledEmbedding(nn.Module):
