@@ -125,7 +125,6 @@ template <typename T> struct RowArgs {
     const T* logits; long ld; const int64_t* labels; int V;
     float* logp; float* stats;      // stats [R][2] = {m, s}; may be NULL
     T* dlogits; long ldd; int W;
-    int row0, n0, row1;             // block b works on row row0 + b, from the n0-th on row1 + (b - n0)
     PolicyArgs pol;
 };
 
@@ -133,13 +132,18 @@ template <typename T, int NT> __device__ __forceinline__ void zero_cols(T* d, in
     for (int c = lo + (int)threadIdx.x; c < hi; c += NT) d[c] = from_f32<T>(0.f);
 }
 
+// between two sweeps: the compiler may not carry the unpacked values over
+template <int MAXC> __device__ __forceinline__ void keep_packed(u32x4_t (&reg)[MAXC]) {
+#pragma unroll
+    for (int i = 0; i < MAXC; ++i) asm volatile("" : "+v"(reg[i]));
+}
+
 // One workgroup a row, the row in MAXC 16-byte chunks per thread: requested together, kept as loaded (packed), swept for the maximum,
 // for the sum and, for the policy loss, for the gradient.
 template <typename T, int NT, int MAXC, bool POLICY>
-__global__ __launch_bounds__(NT) void row_kernel(RowArgs<T> a) {
+__global__ __launch_bounds__(NT, NT == 512 && !POLICY ? 6 : 4) void row_kernel(RowArgs<T> a) {
     __shared__ float sh[2][NT / 64];
-    const int tid = threadIdx.x, b = blockIdx.x;
-    const int row = b < a.n0 ? a.row0 + b : a.row1 + (b - a.n0);
+    const int tid = threadIdx.x, row = blockIdx.x;
     const int64_t y = a.labels[row];
     T* const d = POLICY ? a.dlogits + (long)row * a.ldd : nullptr;
     if (y < 0 || y >= a.V) {
@@ -171,7 +175,9 @@ __global__ __launch_bounds__(NT) void row_kernel(RowArgs<T> a) {
         unpack<T>(reg[i], f);
 #pragma unroll
         for (int k = 0; k < kPer<T>; ++k) m = fmaxf(m, f[k]);
+        __builtin_amdgcn_sched_barrier(0);
     }
+    keep_packed(reg);
     m = block_max<NT>(m, sh[0]);
     float s = 0.f;
 #pragma unroll
@@ -183,6 +189,7 @@ __global__ __launch_bounds__(NT) void row_kernel(RowArgs<T> a) {
         s += part;
         __builtin_amdgcn_sched_barrier(0);
     }
+    keep_packed(reg);
     s = block_sum<NT>(s, sh[1]);
     const float lp = (xy - m) - logf(s);
     if (tid == 0) {
@@ -225,8 +232,7 @@ template <typename T, bool POLICY>
 __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs<T> a) {
     constexpr int NT = 1024;
     __shared__ float sh[2][NT / 64];
-    const int tid = threadIdx.x, b = blockIdx.x;
-    const int row = b < a.n0 ? a.row0 + b : a.row1 + (b - a.n0);
+    const int tid = threadIdx.x, row = blockIdx.x;
     const int64_t y = a.labels[row];
     T* const d = POLICY ? a.dlogits + (long)row * a.ldd : nullptr;
     const long R = (long)a.pol.N * a.pol.T;
@@ -277,54 +283,6 @@ __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs<T> a) {
         }
         zero_cols<T, NT>(d, a.V, a.W);
     }
-}
-
-// Gradient of the logits from the row statistics: coef[row / rows_per_coef] (* *alpha) ([v == y] - exp(x - m) / s).
-// A row whose factor is zero is not read.
-template <typename T>
-__global__ __launch_bounds__(256) void logprob_bwd_kernel(const T* logits, long ld, const int64_t* __restrict__ labels, const float* __restrict__ stats,
-                                                          const float* __restrict__ coef, int rows_per_coef, const float* __restrict__ alpha, T* dlogits,
-                                                          long ldd, int W, int V, int row0, int n0, int row1) {
-    constexpr int NT = 256, U = 4;
-    const int tid = threadIdx.x, b = blockIdx.x;
-    const int row = b < n0 ? row0 + b : row1 + (b - n0);
-    const int64_t y = labels[row];
-    T* const d = dlogits + (long)row * ldd;
-    float c0 = 0.f;
-    if (y >= 0 && y < V) c0 = coef[row / rows_per_coef];
-    if (alpha != nullptr) c0 *= *alpha;
-    if (c0 == 0.f || y < 0 || y >= V) {
-        const float z[kPer<T>] = {};
-        for (long c = (long)tid * kPer<T>; c < W; c += NT * kPer<T>) store_chunk(d, (int)c, W, z);
-        return;
-    }
-    const T* x = logits + (long)row * ld;
-    const float m = stats[2 * (long)row], cs = -c0 / stats[2 * (long)row + 1];
-    for (long c0i = (long)tid * kPer<T>; c0i < V; c0i += (long)U * NT * kPer<T>) {
-        u32x4_t reg[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long c = c0i + (long)u * NT * kPer<T>;
-            if (c < V) reg[u] = load_chunk(x, (int)c, V);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long c = c0i + (long)u * NT * kPer<T>;
-            if (c < V) {
-                float f[kPer<T>];
-                unpack<T>(reg[u], f);
-#pragma unroll
-                for (int k = 0; k < kPer<T>; ++k) f[k] = cs * row_exp<T>(f[k] - m);
-                if (y >= c && y < c + kPer<T>) {
-#pragma unroll
-                    for (int k = 0; k < kPer<T>; ++k)
-                        if (c + k == y) f[k] += c0;
-                }
-                store_chunk(d, (int)c, V, f);
-            }
-        }
-    }
-    zero_cols<T, NT>(d, V, W);
 }
 
 // out[n] = sum (or mean) of a sequence's counted log-probabilities; one wave a sequence, lanes stride over its tokens
@@ -405,6 +363,87 @@ __global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
     }
 }
 
+// Gradient of the logits from the row statistics: coef[row / rows_per_coef] (* *alpha) ([v == y] - exp(x - m) / s).
+// A row whose factor is zero is not read.
+// PAIRS: the preference loss's c; every workgroup takes its pair's sums itself (2 T numbers from the caches, under the latency of its first
+// logits), the one on the pair's first row leaves the pair's results.
+template <typename T, bool PAIRS>
+__global__ __launch_bounds__(256) void logprob_bwd_kernel(const T* logits, long ld, const int64_t* __restrict__ labels, const float* __restrict__ stats,
+                                                          const float* __restrict__ coef, int rows_per_coef, const float* __restrict__ alpha, T* dlogits,
+                                                          long ldd, int W, int V, PairArgs pairs) {
+    constexpr int NT = 256, U = 4;
+    const int tid = threadIdx.x, row = gridDim.x - 1 - blockIdx.x;
+    const int64_t y = labels[row];
+    T* const d = dlogits + (long)row * ldd;
+    const T* x = logits + (long)row * ld;
+    const bool counted = y >= 0 && y < V;
+    u32x4_t reg[U];
+    auto request = [&](long c0i) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long c = c0i + (long)u * NT * kPer<T>;
+            if (c < V) reg[u] = load_chunk(x, (int)c, V);
+        }
+    };
+    float c0 = 0.f;
+    if constexpr (PAIRS) {
+        if (counted) request((long)tid * kPer<T>);
+        const int seq = row / pairs.T, p = seq < pairs.P ? seq : seq - pairs.P;
+        if (counted || row == p * pairs.T) {
+            const PairTerms t = pair_terms(pairs, p, tid & 63);
+            if (counted) c0 = seq < pairs.P ? t.dc : t.dr;
+            if (row == p * pairs.T && tid == 0) {
+                pairs.seq[p] = t.sc;
+                pairs.seq[pairs.P + p] = t.sr;
+                pairs.margins[p] = t.h;
+                pairs.pair_loss[p] = pair_loss_of(pairs, t.h);
+            }
+        }
+    } else if (counted) {
+        c0 = coef[row / rows_per_coef];
+        if (alpha != nullptr) c0 *= *alpha;
+    }
+    if (c0 == 0.f) {
+        const float z[kPer<T>] = {};
+        for (long c = (long)tid * kPer<T>; c < W; c += NT * kPer<T>) store_chunk(d, (int)c, W, z);
+        return;
+    }
+    const float m = stats[2 * (long)row], cs = -c0 / stats[2 * (long)row + 1];
+    for (long c0i = (long)tid * kPer<T>; c0i < V; c0i += (long)U * NT * kPer<T>) {
+        if (!PAIRS || c0i != (long)tid * kPer<T>) request(c0i);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long c = c0i + (long)u * NT * kPer<T>;
+            if (c < V) {
+                float f[kPer<T>];
+                unpack<T>(reg[u], f);
+#pragma unroll
+                for (int k = 0; k < kPer<T>; ++k) f[k] = cs * row_exp<T>(f[k] - m);
+                if (y >= c && y < c + kPer<T>) {
+#pragma unroll
+                    for (int k = 0; k < kPer<T>; ++k)
+                        if (c + k == y) f[k] += c0;
+                }
+                store_chunk(d, (int)c, V, f);
+            }
+        }
+    }
+    zero_cols<T, NT>(d, V, W);
+}
+
+// the mean over the pairs in the order of a single workgroup's pair_kernel
+__global__ void pair_mean_kernel(const float* __restrict__ pair_loss, int P, float* __restrict__ loss) {
+    __shared__ float sh[16];
+    float mean = 0.f;
+    for (int p = threadIdx.x; p < P; p += 16) mean += pair_loss[p];
+    sh[threadIdx.x] = mean;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) mean += sh[w];
+        *loss = mean / (float)P;
+    }
+}
+
 // out[j] = scale * sum of x[j * n .. (j + 1) * n)
 __global__ __launch_bounds__(1024) void rows_mean_kernel(const float* __restrict__ x, long n, float scale, float* __restrict__ out) {
     __shared__ float sh[16];
@@ -462,20 +501,33 @@ bool bad_rows(long R, int V, long ld) { return R <= 0 || R > 0x7fffffffL || V <=
 bool bad_align(int dtype, const void* p) { return ((uintptr_t)p & (dtype == MMSUM_BF16 ? 1 : 3)) != 0; }
 
 template <typename T>
-RowArgs<T> row_args(const void* logits, long ld, const int64_t* labels, int V, float* logp, float* stats, int R) {
+RowArgs<T> row_args(const void* logits, long ld, const int64_t* labels, int V, float* logp, float* stats) {
     RowArgs<T> a = {};
     a.logits = static_cast<const T*>(logits); a.ld = ld; a.labels = labels; a.V = V; a.logp = logp; a.stats = stats;
-    a.n0 = R;
     return a;
 }
 
 template <typename T>
 int launch_bwd(const void* logits, long ld, const int64_t* labels, const float* stats, const float* coef, int rows_per_coef, const float* alpha, void* dlogits,
-               long ldd, int W, int V, int row0, int n0, int row1, int blocks, hipStream_t s) {
-    hipLaunchKernelGGL((logprob_bwd_kernel<T>), dim3(blocks), dim3(256), 0, s, static_cast<const T*>(logits), ld, labels, stats, coef, rows_per_coef, alpha,
-                       static_cast<T*>(dlogits), ldd, W, V, row0, n0, row1);
+               long ldd, int W, int V, int R, hipStream_t s) {
+    hipLaunchKernelGGL((logprob_bwd_kernel<T, false>), dim3(R), dim3(256), 0, s, static_cast<const T*>(logits), ld, labels, stats, coef, rows_per_coef, alpha,
+                       static_cast<T*>(dlogits), ldd, W, V, PairArgs{});
     return ok();
 }
+
+// Statistics, then the gradient from the last row to the first: the rows read last are still in the 256 MB memory-side cache.
+template <typename T>
+int preference_rows(const void* logits, long ld, void* dlogits, long ldd, int W, float* stats, const PairArgs& pairs, hipStream_t s) {
+    const int R = 2 * pairs.P * pairs.T;
+    const RowArgs<T> a = row_args<T>(logits, ld, pairs.labels, pairs.V, const_cast<float*>(pairs.logp), stats);
+    const int rc = launch_rows<T, false>(a, R, s);
+    if (rc != MMSUM_OK) return rc;
+    hipLaunchKernelGGL((logprob_bwd_kernel<T, true>), dim3(R), dim3(256), 0, s, a.logits, ld, pairs.labels, stats, nullptr, 1, nullptr, static_cast<T*>(dlogits), ldd, W, pairs.V,
+                       pairs);
+    return ok();
+}
+
+bool single_pairs(int P, int T) { return (long)P * T <= 32768; }      // a single workgroup is done before a second launch would begin
 
 long count_slots(int N, int seq_mean) { return seq_mean ? N : kCountParts; }
 int launch_counts(const int64_t* labels, int N, int T, int V, int seq_mean, int* counts, hipStream_t s) {
@@ -490,8 +542,8 @@ extern "C" int mmsum_token_logprob(int dtype, const void* logits, long ld, const
     if (bad_rows(R, V, ld)) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
     if (bad_align(dtype, logits)) return MMSUM_ERR_BAD_ALIGN;
-    if (dtype == MMSUM_BF16) return launch_rows<bf16_t, false>(row_args<bf16_t>(logits, ld, labels, V, logp, stats, R), R, (hipStream_t)stream);
-    return launch_rows<float, false>(row_args<float>(logits, ld, labels, V, logp, stats, R), R, (hipStream_t)stream);
+    if (dtype == MMSUM_BF16) return launch_rows<bf16_t, false>(row_args<bf16_t>(logits, ld, labels, V, logp, stats), R, (hipStream_t)stream);
+    return launch_rows<float, false>(row_args<float>(logits, ld, labels, V, logp, stats), R, (hipStream_t)stream);
 }
 
 extern "C" int mmsum_token_logprob_bwd(int dtype, const void* logits, long ld, const int64_t* labels, const float* stats, const float* coef, int rows_per_coef,
@@ -499,8 +551,8 @@ extern "C" int mmsum_token_logprob_bwd(int dtype, const void* logits, long ld, c
     if (bad_rows(R, V, ld) || rows_per_coef <= 0 || W < V || W > 0x7fffffff - 16384 || ldd < W) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
     if (bad_align(dtype, logits) || bad_align(dtype, dlogits)) return MMSUM_ERR_BAD_ALIGN;
-    if (dtype == MMSUM_BF16) return launch_bwd<bf16_t>(logits, ld, labels, stats, coef, rows_per_coef, alpha, dlogits, ldd, W, V, 0, R, 0, R, (hipStream_t)stream);
-    return launch_bwd<float>(logits, ld, labels, stats, coef, rows_per_coef, alpha, dlogits, ldd, W, V, 0, R, 0, R, (hipStream_t)stream);
+    if (dtype == MMSUM_BF16) return launch_bwd<bf16_t>(logits, ld, labels, stats, coef, rows_per_coef, alpha, dlogits, ldd, W, V, R, (hipStream_t)stream);
+    return launch_bwd<float>(logits, ld, labels, stats, coef, rows_per_coef, alpha, dlogits, ldd, W, V, R, (hipStream_t)stream);
 }
 
 extern "C" int mmsum_sequence_logprob(const float* logp, const int64_t* labels, int N, int T, int V, int average, float* out, void* stream) {
@@ -514,7 +566,7 @@ extern "C" int mmsum_preference_pairs(const float* logp, const int64_t* labels, 
     if (P <= 0 || T <= 0 || V <= 0 || 2L * P * T > 0x7fffffffL || !(smoothing >= 0.f && smoothing <= 1.f)) return MMSUM_ERR_BAD_SHAPE;
     hipStream_t s = (hipStream_t)stream;
     PairArgs a = {logp, labels, ref, P, T, V, average, beta, smoothing, seq, margins, pair_loss, coef, loss};
-    if ((long)P * T <= 32768) {                                    // a single workgroup is done before a second launch would begin
+    if (single_pairs(P, T)) {
         hipLaunchKernelGGL(pair_kernel, dim3(1), dim3(1024), 0, s, a);
     } else {
         a.loss = nullptr;
@@ -537,10 +589,19 @@ extern "C" int mmsum_preference_loss(int dtype, const void* logits, long ld, con
     float* const stats = logp + R;
     float* const pair_loss = stats + 2L * R;
     float* const coef = pair_loss + P;
-    int rc = mmsum_token_logprob(dtype, logits, ld, labels, logp, stats, R, V, stream);
-    if (rc == MMSUM_OK) rc = mmsum_preference_pairs(logp, labels, ref, P, T, V, beta, smoothing, average, seq, margins, pair_loss, coef, loss, stream);
-    if (rc == MMSUM_OK) rc = mmsum_token_logprob_bwd(dtype, logits, ld, labels, stats, coef, T, nullptr, dlogits, ldd, W, R, V, stream);
-    return rc;
+    hipStream_t s = (hipStream_t)stream;
+    if (T > 1024) {                                                // long sequences: the pairs once, not in every row's workgroup
+        int rc = mmsum_token_logprob(dtype, logits, ld, labels, logp, stats, R, V, stream);
+        if (rc == MMSUM_OK) rc = mmsum_preference_pairs(logp, labels, ref, P, T, V, beta, smoothing, average, seq, margins, pair_loss, coef, loss, stream);
+        if (rc == MMSUM_OK) rc = mmsum_token_logprob_bwd(dtype, logits, ld, labels, stats, coef, T, nullptr, dlogits, ldd, W, R, V, stream);
+        return rc;
+    }
+    const PairArgs pairs = {logp, labels, ref, P, T, V, average, beta, smoothing, seq, margins, pair_loss, coef, loss};
+    int rc = dtype == MMSUM_BF16 ? preference_rows<bf16_t>(logits, ld, dlogits, ldd, W, stats, pairs, s) : preference_rows<float>(logits, ld, dlogits, ldd, W, stats, pairs, s);
+    if (rc != MMSUM_OK) return rc;
+    if (single_pairs(P, T)) hipLaunchKernelGGL(pair_mean_kernel, dim3(1), dim3(16), 0, s, pair_loss, P, loss);
+    else hipLaunchKernelGGL(rows_mean_kernel, dim3(1), dim3(1024), 0, s, pair_loss, (long)P, 1.f / (float)P, loss);
+    return ok();
 }
 
 // workspace: terms [3][NT], counts
@@ -591,11 +652,11 @@ extern "C" int mmsum_policy_loss(int dtype, const void* logits, long ld, const i
     else if (rc == MMSUM_OK) rc = launch_counts(labels, N, T, V, seq_mean, const_cast<int*>(p.counts), s);
     if (rc != MMSUM_OK) return rc;
     if (dtype == MMSUM_BF16) {
-        RowArgs<bf16_t> a = row_args<bf16_t>(logits, ld, labels, V, logp, nullptr, R);
+        RowArgs<bf16_t> a = row_args<bf16_t>(logits, ld, labels, V, logp, nullptr);
         a.dlogits = static_cast<bf16_t*>(dlogits); a.ldd = ldd; a.W = W; a.pol = p;
         rc = launch_rows<bf16_t, true>(a, R, s);
     } else {
-        RowArgs<float> a = row_args<float>(logits, ld, labels, V, logp, nullptr, R);
+        RowArgs<float> a = row_args<float>(logits, ld, labels, V, logp, nullptr);
         a.dlogits = static_cast<float*>(dlogits); a.ldd = ldd; a.W = W; a.pol = p;
         rc = launch_rows<float, true>(a, R, s);
     }
