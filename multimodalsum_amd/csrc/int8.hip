@@ -392,39 +392,114 @@ __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(I8Args p) {
 #undef I8_DMA
 }
 
-// Any shape: 64x64 tiles.  v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k of row l & 15, k group l >> 4; result column l & 15, rows 4 (l >> 4) + e
-template <typename T, bool GELU>
-__global__ __launch_bounds__(256) void gemm_i8_kernel(I8Args p) {
-    __shared__ __attribute__((aligned(16))) int8_t sA[64 * 64], sB[64 * 64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const long m0 = (long)blockIdx.y * 64, n0 = (long)blockIdx.x * 64;
-    i32x4_t acc[4] = {};
-    for (int k0 = 0; k0 < p.K; k0 += 64) {
-        const int r = tid >> 2, ch = tid & 3;
-        const long am = m0 + r < p.M ? m0 + r : p.M - 1, bn = n0 + r < p.N ? n0 + r : p.N - 1;
-        const u32x4_t va = *reinterpret_cast<const u32x4_t*>(p.A + am * p.lda + k0 + ch * 16), vb = *reinterpret_cast<const u32x4_t*>(p.B + bn * p.ldb + k0 + ch * 16);
-        __syncthreads();
-        *reinterpret_cast<u32x4_t*>(sA + r * 64 + ch * 16) = va;
-        *reinterpret_cast<u32x4_t*>(sB + r * 64 + ch * 16) = vb;
-        __syncthreads();
-        const i32x4_t a = *reinterpret_cast<const i32x4_t*>(sA + (wave * 16 + (lane & 15)) * 64 + (lane >> 4) * 16);
+// Between the two: 64x64 tiles, one a workgroup of 2x2 waves, the stages in a ring that runs NST - 1 of them ahead of the products (64 KB of
+// LDS: two workgroups a CU hide each other's waits).  Operand rows, swizzle and the order of the weight rows as above.
+template <typename T, bool GELU, int BM, int BN, int WM, int WN, int NST>
+__global__ __launch_bounds__(WM* WN * 64) void gemm_i8_ring_kernel(I8Args p) {
+    constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 128, PA = BM / 8 / NW, PB = BN / 8 / NW, PPW = PA + PB;
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && (32 % (8 * NW) == 0 || (8 * NW) % 32 == 0), "whole pieces for every wave");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
+    int tm, tn;
+    tile_coords(xcd_remap(blockIdx.x, gridDim.x), tiles_m, tiles_n, tm, tn);
+    const int nst = p.K / 128;
+    const long ra = (p.M - (long)tm * BM) * p.lda, rb = (p.N - (long)tn * BN) * p.ldb;
+    const int bytesA = (int)(ra < 0x7fffffff ? ra : 0x7fffffff), bytesB = (int)(rb < 0x7fffffff ? rb : 0x7fffffff);
+    const int8_t* const baseA = p.A + (long)tm * BM * p.lda;
+    const int8_t* const baseB = p.B + (long)tn * BN * p.ldb;
+    int offA[PA], offB[PB];                                        // piece i of a wave: rows 8 (NW i + wave) .. + 7
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const i32x4_t b = *reinterpret_cast<const i32x4_t*>(sB + (j * 16 + (lane & 15)) * 64 + (lane >> 4) * 16);
-            acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc[j], 0, 0, 0);
-        }
+    for (int i = 0; i < PA; ++i) {
+        const int row = (i * NW + wave) * 8 + (lane >> 3);
+        offA[i] = row * (int)p.lda + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int i = 0; i < PB; ++i) {
+        const int row = (i * NW + wave) * 8 + (lane >> 3), wrow = (row & ~31) | (((row >> 2) & 3) << 3) | (((row >> 4) & 1) << 2) | (row & 3);
+        offB[i] = wrow * (int)p.ldb + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+    }
+    auto issue = [&](int st) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        typedef __attribute__((address_space(3))) void* lds_ptr;
+        const __amdgpu_buffer_rsrc_t da = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(baseA), 0, bytesA, 0x00020000);
+        const __amdgpu_buffer_rsrc_t db = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(baseB), 0, bytesB, 0x00020000);
+        char* const slot = smem + st % NST * STAGE;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const long m = m0 + wave * 16 + 4 * (lane >> 4) + e, n = n0 + j * 16 + (lane & 15);
-            if (m < p.M && n < p.N) {
-                float v = fmaf((float)acc[j][e] * p.sa[m], p.sb[n], p.bias ? p.bias[n] : 0.f);
-                if constexpr (GELU) v = gelu_i8(v);
-                static_cast<T*>(p.C)[m * p.ldc + n] = from_f32<T>(v);
+        for (int i = 0; i < PA; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (lds_ptr)(slot + (i * NW + wave) * 1024), 16, offA[i], st * 128, 0, 0);
+#pragma unroll
+        for (int i = 0; i < PB; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_ptr)(slot + BM * 128 + (i * NW + wave) * 1024), 16, offB[i], st * 128, 0, 0);
+#endif
+    };
+    const int r16 = lane & 15, fo = r16 * 128 + ((((lane >> 4) ^ (r16 >> 1)) & 7) << 4);
+    i32x4_t c[TM][TN][4] = {};
+#pragma unroll
+    for (int st = 0; st < NST - 1; ++st)
+        if (st < nst) issue(st);
+    for (int st = 0; st < nst; ++st) {
+        const int ahead = nst - 1 - st;                            // stages requested behind this one, NST - 2 of them at most
+        if (ahead >= NST - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * PPW) : "memory");
+        else if (NST > 3 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PPW) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        const char* const A = smem + st % NST * STAGE + wm * (TM * 32) * 128 + fo;
+        const char* const B = smem + st % NST * STAGE + BM * 128 + wn * (TN * 32) * 128 + fo;
+        const int yd = (fo ^ 64) - fo;
+        i32x4_t a[2][TM][2], b[2][TN][2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) a[y][i][h] = *reinterpret_cast<const i32x4_t*>(A + (i * 32 + h * 16) * 128 + y * yd);
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) b[y][j][h] = *reinterpret_cast<const i32x4_t*>(B + (j * 32 + h * 16) * 128 + y * yd);
+        }
+        if (st + NST - 1 < nst) issue(st + NST - 1);               // into the slot of stage st - 1: every wave is past its products
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) c[i][j][q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[y][j][q & 1], a[y][i][q >> 1], c[i][j][q], 0, 0, 0);
+    }
+    const int mr = tm * BM + wm * (TM * 32) + r16, nc = tn * BN + wn * (TN * 32) + 8 * (lane >> 4);
+    auto epilogue = [&](auto whole_c) {
+        constexpr bool WHOLE = decltype(whole_c)::value;
+        float sx[2 * TM], sw[TN][8], bs[TN][8] = {};
+#pragma unroll
+        for (int k = 0; k < 2 * TM; ++k) sx[k] = p.sa[WHOLE || mr + 16 * k < p.M ? mr + 16 * k : p.M - 1];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            load_cols<WHOLE>(p.sb, nc + 32 * j, p.N, sw[j]);
+            if (p.bias != nullptr) load_cols<WHOLE>(p.bias, nc + 32 * j, p.N, bs[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) { retire(sw[j]); retire(bs[j]); }
+        T* row = static_cast<T*>(p.C) + (long)mr * p.ldc + nc;
+#pragma unroll
+        for (int k = 0; k < 2 * TM; ++k, row += 16 * p.ldc) {
+            if (WHOLE || mr + 16 * k < p.M) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        v[e] = fmaf((float)c[k >> 1][j][2 * (k & 1) + (e >> 2)][e & 3] * sx[k], sw[j][e], bs[j][e]);
+                        if constexpr (GELU) v[e] = gelu_i8(v[e]);
+                    }
+                    store_cols<T, WHOLE>(row + 32 * j, p.N - nc - 32 * j, v);
+                }
             }
         }
+    };
+    if (tm * BM + BM <= p.M && tn * BN + BN <= p.N) epilogue(std::true_type{});
+    else epilogue(std::false_type{});
 }
 
 // Few rows (a decode step): the weights go past the matrix cores once.  A workgroup owns 16 NB columns, its four waves every fourth 64 bytes
@@ -532,16 +607,19 @@ int launch_few(const I8Args& p, const X* x, long ldx, int Kx, hipStream_t s) {
     return ok();
 }
 
+template <typename T, bool GELU, int BM, int BN, int WM, int WN, int NST>
+int launch_ring(const I8Args& p, hipStream_t s) {
+    const long tiles = (p.M + (long)BM - 1) / BM * ((p.N + (long)BN - 1) / BN);
+    if (tiles > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    const size_t lds = (size_t)NST * (BM + BN) * 128;
+    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_ring_kernel<T, GELU, BM, BN, WM, WN, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+        return MMSUM_ERR_HIP;
+    hipLaunchKernelGGL((gemm_i8_ring_kernel<T, GELU, BM, BN, WM, WN, NST>), dim3((unsigned)tiles), dim3(WM * WN * 64), lds, s, p);
+    return ok();
+}
+
 template <typename T, bool GELU>
 int launch_product(const I8Args& p, hipStream_t s) {
-    const long tiles = ((long)p.M + 255) / 256 * (((long)p.N + 255) / 256);
-    if (p.M > 64 && tiles >= 128 && tiles <= 0x7fffffffL) {
-        const size_t lds = 5 * kStageBytes;
-        if (hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_w4_kernel<T, GELU>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return MMSUM_ERR_HIP;
-        const int cus = cu_count();
-        hipLaunchKernelGGL((gemm_i8_w4_kernel<T, GELU>), dim3((unsigned)(tiles < cus ? tiles : cus)), dim3(256), lds, s, p);
-        return ok();
-    }
     if (p.M <= 64) {
         // wide workgroups where there are still enough of them for every CU: they read the activations less often
         const bool wide = p.N >= 32768;
@@ -549,9 +627,15 @@ int launch_product(const I8Args& p, hipStream_t s) {
         if (p.M <= 32) return wide ? launch_few<T, GELU, 2, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 2, 1, false, float>(p, nullptr, 0, 0, s);
         return wide ? launch_few<T, GELU, 4, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 4, 1, false, float>(p, nullptr, 0, 0, s);
     }
-    const dim3 grid((unsigned)((p.N + 63L) / 64), (unsigned)((p.M + 63L) / 64));
-    if (grid.y > 65535) return MMSUM_ERR_BAD_SHAPE;
-    hipLaunchKernelGGL((gemm_i8_kernel<T, GELU>), grid, dim3(256), 0, s, p);
+    // 256x256 tiles from about half a round of the CUs on, unless most of a tile is behind the edge (us, 64x64 | 256x256, bf16 out):
+    // 1152x4096x1024 (80 tiles) 14 | 29, 2304x4096x1024 (144) 22 | 20, 9216x1024x4096 (144) 58 | 49, 18432x4096x1024 142 | 88; 128x50265x1024 (197) 21 | 31
+    const long t256 = (p.M + 255L) / 256 * ((p.N + 255L) / 256);
+    if (t256 < 144 || p.M < 192 || p.N < 192) return launch_ring<T, GELU, 64, 64, 2, 2, 4>(p, s);
+    const int cus = cu_count();
+    const size_t lds = 5 * kStageBytes;
+    if (t256 > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_w4_kernel<T, GELU>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return MMSUM_ERR_HIP;
+    hipLaunchKernelGGL((gemm_i8_w4_kernel<T, GELU>), dim3((unsigned)(t256 < cus ? t256 : cus)), dim3(256), lds, s, p);
     return ok();
 }
 

@@ -34,11 +34,11 @@ class Int8Linear(nn.Module):
     def forward(self, x):
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("Int8Linear is for inference: no gradient (use torch.no_grad() or detach the input)")
-        if x.dim() < 1 or x.shape[-1] != self.in_features:
-            raise ValueError("x: [..., %d] expected, got %s" % (self.in_features, tuple(x.shape)))
-        rows = x.reshape(-1, self.in_features)
-        if self.in_features > 1 and rows.stride(1) != 1:
+        K = self.in_features
+        if x.dim() < 1 or x.shape[-1] != K:
+            raise ValueError("x: [..., %d] expected, got %s" % (K, tuple(x.shape)))
+        rows = x if x.dim() == 2 else x.reshape(-1, K)
+        if K > 1 and rows.stride(1) != 1:
             rows = rows.contiguous()
-        y = torch.empty(rows.shape[0], self.out_features, dtype=self.out_dtype or x.dtype, device=x.device)
-        kn.linear_i8(rows, self.qweight, self.scale, y, self.bias, self.gelu)
-        return y.reshape(*x.shape[:-1], self.out_features)
+        y = kn.linear_i8(rows, self.qweight, self.scale, None, self.bias, self.gelu, self.out_dtype)
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)

@@ -857,19 +857,24 @@ def gemm_i8(qx, sx, qw, sw, out, bias=None, gelu=False):
     return out
 
 
-def linear_i8(x, qw, sw, out, bias=None, gelu=False):
-    """quantize_rows and gemm_i8 in one call: out [M, N] = x [M, K] . W^T (+ bias) (GELU), W as quantize_rows left it."""
+def linear_i8(x, qw, sw, out=None, bias=None, gelu=False, out_dtype=None):
+    """quantize_rows and gemm_i8 in one call: out [M, N] = x [M, K] . W^T (+ bias) (GELU), W as quantize_rows left it; out None: a new one of
+    out_dtype (None: x's)."""
     (M, K), N = x.shape, qw.shape[0]
     if qw.dtype != torch.int8:
         raise TypeError("qw: int8 expected, got %s" % qw.dtype)
     _need(0 < K <= 131072 and qw.shape[1] == -(-K // I8_K_STEP) * I8_K_STEP, "linear_i8: weights as quantize_rows leaves them expected")
-    _need(out.shape == (M, N), "out: shape %s expected, got %s", (M, N), out.shape)
     sw, bias = _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias")
-    ldx, ldw, ldy = _pitch2(x, "x"), _pitch2(qw, "qw"), _pitch2(out, "out")
-    dt, dto = _dt(x), _dt(out)
+    ldx, ldw, dt = _pitch2(x, "x"), _pitch2(qw, "qw"), _dt(x)
     dev = _device(x, qw, sw, out, bias)
-    _apart(x, out)
-    if M:
+    if out is None:
+        out, ldy = torch.empty(M, N, dtype=out_dtype or x.dtype, device=dev), N
+    else:
+        _need(out.shape == (M, N), "out: shape %s expected, got %s", (M, N), out.shape)
+        ldy = _pitch2(out, "out")
+        _apart(x, out)
+    dto = _dt(out)
+    if M and N:
         ws = torch.empty(M * (qw.shape[1] + 4), dtype=torch.uint8, device=dev)
         _launch("mmsum_linear_i8", dev, dt, x.data_ptr(), ldx, qw.data_ptr(), ldw, sw.data_ptr(), None if bias is None else bias.data_ptr(), dto, out.data_ptr(), ldy, M, N, K,
                 int(bool(gelu)), ws.data_ptr())

@@ -394,7 +394,7 @@ def test_quantize_rows(M, K, dt):
 
 I8 = [(1, 17, 16), (1, 1, 1), (3, 64, 100), (8, 1024, 1024), (16, 50, 4096), (17, 129, 257), (32, 5001, 1024), (33, 1024, 2000), (65, 200, 64), (128, 512, 512), (129, 1000, 640),
       (257, 255, 384), (1152, 1024, 1024), (1300, 2051, 128), (700, 4096, 1024),
-      (4100, 2100, 384), (33000, 70, 128), (300, 33001, 256), (2048, 4096, 1024), (8200, 1028, 128)]
+      (4100, 2100, 384), (33000, 70, 128), (300, 33001, 256), (2048, 4096, 1024), (8200, 1028, 128), (2500, 4100, 1024), (40000, 256, 512)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
