@@ -1,6 +1,6 @@
 // Embedding lookup with scaling, y[i] = scale E[ids[i]], and the table's gradient dE[v] = scale sum of dy[i] over ids[i] == v.
 //
-// The gradient goes by SORTED tokens: a stable radix sort brings equal ids together in batch order, fixed stretches of the sorted list
+// The gradient goes by SORTED tokens: a stable radix sort (few ids: every workgroup picks and sorts its own) brings equal ids together in batch order, fixed stretches of the sorted list
 // are summed each by one wave, and a token's stretches are added in order -- no floating-point atomics, so a gradient is the same bit
 // for bit on every run, and a frequent token (padding excluded, still a few percent of a text) is summed by many waves at once.
 // Ids outside 0 .. V-1 read as zero rows and leave no gradient, and so does pad_id in the gradient.
@@ -221,22 +221,136 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restr
     for (int i = tid; i < n; i += 1024) { okeys[i] = lk[cur][i]; opos[i] = lp[cur][i]; }
 }
 
-// up to 512 ids: an element's place is the number of elements in front of it
-constexpr int kTiny = 512;
-__global__ __launch_bounds__(kTiny) void sort_tiny_kernel(const int64_t* __restrict__ ids, int n, int V, int64_t pad_id, uint32_t* __restrict__ okeys, int* __restrict__ opos, ZeroFill z) {
-    if ((int)blockIdx.x >= z.first) return zero_fill<kTiny>(z);
-    __shared__ __attribute__((aligned(16))) uint32_t lk[kTiny];
-    const int i = threadIdx.x;
-    const uint32_t key = i < n ? key_of(ids[i], V, pad_id) : 0xffffffffu;
-    lk[i] = key;
-    __syncthreads();
-    int rank = 0;
-    for (int j = 0; j < n; j += 4) {
-        const u32x4_t k = *reinterpret_cast<const u32x4_t*>(lk + j);
+// ---- up to 2048 ids: one launch ----------------------------------------------------------------------------------------------------
+// A workgroup takes neighbouring rows of the table (16 KB of them) at a time.  It reads every id, keeps the positions that name its rows (in batch
+// order), sorts them by row by counting the entries in front of each, and writes its rows whole: sums or zeros.  A row is summed by tpr threads of
+// four columns (VEC = 1: one), its positions in order, eight requested at a time.  Reading all ids in every workgroup is cheap while they
+// are few (1,152 ids: 9 KB a workgroup, once); the launches and waits of the sort are not.
+constexpr int kFew = 2048, kRowsMax = 256;
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void embed_bwd_few_kernel(const T* __restrict__ dy, long lddy, const int64_t* __restrict__ ids, int n, int V, int D, float scale, int64_t pad_id,
+                                                            int accumulate, float* __restrict__ dE, int rows, int tpr_log2) {
+    __shared__ __attribute__((aligned(16))) uint32_t list[kFew];       // (row in the workgroup's range) << 16 | position, in batch order
+    __shared__ uint16_t sorted[kFew];                                  // positions by row
+    __shared__ int start[kRowsMax + 1], wsum[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int64_t all[kFew / 256];                                           // requested together
 #pragma unroll
-        for (int u = 0; u < 4; ++u) rank += k[u] < key || (k[u] == key && j + u < i);
+    for (int i = 0; i < kFew / 256; ++i) all[i] = i * 256 + tid < n ? ids[i * 256 + tid] : -1;
+    for (long v0 = (long)blockIdx.x * rows; v0 < V; v0 += (long)gridDim.x * rows) {      // the ids stay in registers from one stretch of rows to the next
+    const int here = (int)(V - v0 < rows ? V - v0 : rows);
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < kFew / 256; ++i) any |= all[i] >= v0 && all[i] < v0 + here && all[i] != pad_id;
+    if (!__syncthreads_or(any)) {                                      // none of the rows is named: most workgroups of a large table
+        if (accumulate) continue;
+        float* const z = dE + v0 * D;
+        const long cells = (long)here * D, quads = ((uintptr_t)z & 15) == 0 ? cells / 4 : 0;
+        for (long i = tid; i < quads; i += 256) reinterpret_cast<f32x4_t*>(z)[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (long i = quads * 4 + tid; i < cells; i += 256) z[i] = 0.f;
+        continue;
     }
-    if (i < n) { okeys[rank] = key; opos[rank] = i; }
+    start[tid] = 0;
+    int L = 0;
+#pragma unroll
+    for (int i = 0; i < kFew / 256; ++i) {
+        const int i0 = i * 256;
+        if (i0 >= n) break;
+        const int64_t id = all[i];
+        const bool mine = id >= v0 && id < v0 + here && id != pad_id;
+        const uint64_t m = __ballot(mine);
+        __syncthreads();                                              // wsum of the last round is read
+        if (lane == 0) wsum[wave] = __popcll(m);
+        __syncthreads();
+        int at = L + __popcll(m & ((1ull << lane) - 1));
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            at += w < wave ? wsum[w] : 0;
+            L += wsum[w];
+        }
+        if (mine) list[at] = (uint32_t)(id - v0) << 16 | (uint32_t)(i0 + tid);
+    }
+    if (tid < 4 && L + tid < kFew) list[L + tid] = 0xffffffffu;        // the counting below reads four at a time
+    __syncthreads();
+    for (int i = tid; i < L; i += 256) {
+        const uint32_t e = list[i];
+        int rank = 0;                                                  // entries order by (row, position), all different
+        for (int j = 0; j < L; j += 4) {
+            const u32x4_t q = *reinterpret_cast<const u32x4_t*>(list + j);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) rank += q[u] < e;
+        }
+        sorted[rank] = (uint16_t)(e & 0xffffu);
+        atomicAdd(&start[e >> 16], 1);                                 // counts: whole numbers
+    }
+    __syncthreads();
+    {                                                                  // counts -> starts
+        const int c = start[tid];
+        int s = c;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(s, o);
+            s += lane >= o ? v : 0;
+        }
+        if (lane == 63) wsum[wave] = s;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) s += w < wave ? wsum[w] : 0;
+        start[tid] = s - c;
+        if (tid == 255) start[256] = s;
+        __syncthreads();
+    }
+    constexpr int AHEAD = 8;
+    const int tpr = 1 << tpr_log2, groups = 256 >> tpr_log2;
+    for (int r = tid >> tpr_log2; r < here; r += groups) {
+        const int lo = start[r], hi = start[r + 1];
+        if (accumulate && lo == hi) continue;
+        for (int c = (tid & (tpr - 1)) * VEC; c < D; c += tpr * VEC) {
+            float acc[VEC] = {};
+            for (int i0 = lo; i0 < hi; i0 += AHEAD) {
+                float f[AHEAD][VEC];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const T* const src = dy + (long)sorted[i0 + u < hi ? i0 + u : lo] * lddy + c;
+                    if constexpr (VEC == 1) f[u][0] = to_f32(*src);
+                    else if constexpr (sizeof(T) == 2) {
+                        const bf16x4_t t = *reinterpret_cast<const bf16x4_t*>(src);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) f[u][k] = (float)t[k];
+                    } else {
+                        const f32x4_t t = *reinterpret_cast<const f32x4_t*>(src);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) f[u][k] = t[k];
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) acc[k] += i0 + u < hi ? f[u][k] : 0.f;
+            }
+            float* const o = dE + (v0 + r) * D + c;
+            if constexpr (VEC == 1) *o = accumulate ? *o + scale * acc[0] : scale * acc[0];
+            else {
+                f32x4_t s = {scale * acc[0], scale * acc[1], scale * acc[2], scale * acc[3]};
+                if (accumulate) s += *reinterpret_cast<f32x4_t*>(o);
+                *reinterpret_cast<f32x4_t*>(o) = s;
+            }
+        }
+    }
+    }
+}
+template <typename T>
+int embed_bwd_few(const void* dy, long lddy, const int64_t* ids, int n, int V, int D, float scale, int64_t pad_id, int accumulate, float* dE, hipStream_t s) {
+    const bool vec = D % 4 == 0 && lddy % 4 == 0 && ((uintptr_t)dy & (4 * sizeof(T) - 1)) == 0 && ((uintptr_t)dE & 15) == 0;
+    const long want = 4096 / D;                                        // 16 KB: the rows of a text's most frequent tokens are neighbours, and the tail
+    const int rows = want < 1 ? 1 : want > kRowsMax ? kRowsMax : (int)want, steps = vec ? D / 4 : D;
+    int lg = 0;
+    while ((1 << lg) < steps && lg < 8) ++lg;
+    const long ranges = (V + (long)rows - 1) / rows;
+    const dim3 grid((unsigned)(ranges < 2048 ? ranges : 2048));        // eight a CU
+    if (vec) hipLaunchKernelGGL((embed_bwd_few_kernel<T, 4>), grid, dim3(256), 0, s, (const T*)dy, lddy, ids, n, V, D, scale, pad_id, accumulate, dE, rows, lg);
+    else hipLaunchKernelGGL((embed_bwd_few_kernel<T, 1>), grid, dim3(256), 0, s, (const T*)dy, lddy, ids, n, V, D, scale, pad_id, accumulate, dE, rows, lg);
+    return ok();
 }
 
 // ---- sums --------------------------------------------------------------------------------------------------------------------------
@@ -426,6 +540,7 @@ long align16(long b) { return (b + 15) & ~15L; }
 
 template <typename T>
 int embed_bwd_t(const void* dy, long lddy, const int64_t* ids, int n, int V, int D, float scale, int64_t pad_id, int accumulate, float* dE, char* ws, hipStream_t s) {
+    if (n <= kFew) return embed_bwd_few<T>(dy, lddy, ids, n, V, D, scale, pad_id, accumulate, dE, s);
     const long nb = align16((long)n * 4);
     uint32_t* k0 = reinterpret_cast<uint32_t*>(ws);
     int* p0 = reinterpret_cast<int*>(ws + nb);
@@ -447,10 +562,7 @@ int embed_bwd_t(const void* dy, long lddy, const int64_t* ids, int n, int V, int
         }
         return z;
     };
-    if (n <= kTiny) {
-        const ZeroFill z = fill(1, 0, 1);
-        hipLaunchKernelGGL(sort_tiny_kernel, dim3(1 + z.blocks), dim3(kTiny), 0, s, ids, n, V, pad_id, k0, p0, z);
-    } else if (n <= kSmall) {
+    if (n <= kSmall) {
         const ZeroFill z = fill(1, 0, 1);
         hipLaunchKernelGGL(sort_small_kernel, dim3(1 + z.blocks), dim3(1024), 0, s, ids, n, V, pad_id, bits, k0, p0, z);
     } else {
