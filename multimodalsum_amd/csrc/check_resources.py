@@ -1,4 +1,4 @@
-"""Build-time guard (csrc/Makefile runs it on the compiler's -Rpass-analysis=kernel-resource-usage remarks of gemm_fast.hip).
+"""Build-time guard (csrc/Makefile runs it on the compiler's -Rpass-analysis=kernel-resource-usage remarks of gemm_fast.hip and int8.hip).
 
 gemm_tn_w4_kernel keeps its 256 accumulators in AGPRs that it names in inline asm (gemm_tn_w4_acc.inc); the compiler does not
 know they are live between the zero-fill and the read-out, so it must never need an AGPR or a scratch slot of its own in that
@@ -19,9 +19,11 @@ LIMITS = {                    # kernel-name substring -> (max arch VGPRs, max sc
     # accumulator layout and spills a few more registers in that epilogue; more specific entries win
     "gemm_nt_w4_kernelILi0ELi3E": (256, 96, 24),
 }
+INT8_LIMITS = {"gemm_i8_w4_kernel": (256, 0, 0)}             # int8.hip: the same pipeline on 8-bit operands, "+a" accumulators
 
 
 def main(path):
+    LIMITS = INT8_LIMITS if "int8" in path else globals()["LIMITS"]
     text = open(path).read()
     blocks = re.split(r"remark: Function Name: ", text)[1:]
     seen, bad = set(), []

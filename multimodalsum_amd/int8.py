@@ -38,7 +38,7 @@ class Int8Linear(nn.Module):
         if x.dim() < 1 or x.shape[-1] != K:
             raise ValueError("x: [..., %d] expected, got %s" % (K, tuple(x.shape)))
         rows = x if x.dim() == 2 else x.reshape(-1, K)
-        if K > 1 and rows.stride(1) != 1:
+        if (K > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < K):
             rows = rows.contiguous()
         y = kn.linear_i8(rows, self.qweight, self.scale, None, self.bias, self.gelu, self.out_dtype)
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)

@@ -809,7 +809,7 @@ def embed_bwd(dy, ids, V, scale=1.0, pad_id=None, out=None, accumulate=False):
     _need(dy.shape[:-1] == ids.shape, "dy: shape %s expected, got %s", (*ids.shape, D), dy.shape)
     _need(V > 0 and D > 0 and n < 2 ** 30, "embed_bwd: %d ids into [%d, %d]", n, V, D)
     dy = dy.reshape(-1, D)
-    if n and D > 1 and dy.stride(1) != 1:
+    if n and ((D > 1 and dy.stride(1) != 1) or (n > 1 and dy.stride(0) < D)):        # a gradient that is one row, repeated, among them
         dy = dy.contiguous()
     lddy = _pitch2(dy, "dy") if n else D
     _need(not accumulate or out is not None, "accumulate without out")

@@ -139,7 +139,7 @@ def pref_plain(own, keep, ref, beta, eps, average):
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("average", [False, True])
 @pytest.mark.parametrize("eps", [0.0, 0.1])
-@pytest.mark.parametrize("size", [(2, 1, 5), (4, 7, 1009), (6, 33, 2050), (4, 5, 50265)])
+@pytest.mark.parametrize("size", [(2, 1, 5), (4, 7, 1009), (6, 33, 2050), (4, 5, 50265), (2, 1100, 5), (66, 1000, 3)])
 def test_preference_loss(size, eps, average, dt):
     import multimodalsum_amd as mm
     from multimodalsum_amd import kernels as kn
@@ -197,7 +197,7 @@ def policy_plain(own, keep, old, adv, ref, lo, hi, kl_coef, reduction):
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("reduction", ["token", "sequence"])
 @pytest.mark.parametrize("kl_coef", [0.0, 0.1])
-@pytest.mark.parametrize("size", [(1, 1, 5), (5, 7, 1009), (3, 70, 300), (3, 4, 50265), (2, 2, 110003)])
+@pytest.mark.parametrize("size", [(1, 1, 5), (5, 7, 1009), (3, 70, 300), (3, 4, 50265), (2, 2, 110003), (2, 2100, 7)])
 def test_policy_loss(size, kl_coef, reduction, dt):
     import multimodalsum_amd as mm
     N, T, V = size
@@ -278,7 +278,7 @@ def test_gradient_against_differences():
 # embedding
 # ---------------------------------------------------------------------------------------------------------------------------------
 EMB = [(1, 1, 1), (7, 5, 3), (21, 1009, 256), (1000, 50, 100), (4097, 70000, 64), (5000, 300, 777), (300, 50265, 1024), (12000, 1, 40), (9000, 255, 512), (4096, 256, 8),
-       (40000, 2, 520)]
+       (40000, 2, 520), (2500, 4000, 16), (300000, 1000, 8)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
@@ -324,6 +324,18 @@ def test_embedding(case, dt):
     t = table.clone().requires_grad_(True)
     mm.scaled_embedding(ids.view(1, n), t, scale, pad).backward(dy.view(1, n, D))
     assert torch.equal(t.grad, d.to(dt))
+
+
+def test_repeated_rows():
+    """A gradient that is one row for every position (sum over positions) and activations that are one row for every token: strides of zero."""
+    import multimodalsum_amd as mm
+    table = torch.randn(50, 24, device="cuda", requires_grad=True)
+    ids = torch.arange(100, device="cuda") % 50
+    v = torch.randn(24, device="cuda")
+    (mm.scaled_embedding(ids, table, 3.0).sum(0) * v).sum().backward()
+    assert torch.equal(table.grad, (v * 2 * 3.0).expand(50, 24))
+    lin = mm.Int8Linear(torch.randn(20, 24, device="cuda"))
+    assert torch.equal(lin(v.expand(7, 24)), lin(v).expand(7, 20))
 
 
 def test_embedding_without_ids_and_module():
@@ -491,7 +503,7 @@ def all_ops(s):
     q = mm.policy_loss_and_grad(s["x"], s["labels"], s["old"], s["adv"], s["old"], kl_coef=0.1)
     y = mm.scaled_embedding(s["ids"], s["table"], 2.0)
     d = mm.scaled_embedding_grad(s["dy"], s["ids"], s["table"].shape[0], 2.0)
-    return [seq, tok, *p, *q, y, d, s["lin"](s["act"]), s["lin"](s["act"][:5])]
+    return [seq, tok, *p, *q, y, d, s["lin"](s["act"]), s["lin"](s["act"][:5]), s["lin2"](s["act2"])]
 
 
 def op_state(seed, n=5000):
@@ -500,7 +512,8 @@ def op_state(seed, n=5000):
     g = torch.Generator().manual_seed(seed)
     return dict(x=torch.nan_to_num(x), labels=labels, ref=torch.randn(4, generator=g).cuda(), old=torch.randn(4, 8, generator=g).cuda() - 3, adv=torch.randn(4, generator=g).cuda(),
                 ids=torch.randint(0, 700, (n,), generator=g).cuda(), table=torch.randn(700, 64, generator=g).cuda(), dy=torch.randn(n, 64, generator=g).cuda(),
-                lin=mm.Int8Linear(torch.randn(300, 256, generator=g).cuda()), act=torch.randn(150, 256, generator=g).cuda())
+                lin=mm.Int8Linear(torch.randn(300, 256, generator=g).cuda()), act=torch.randn(150, 256, generator=g).cuda(),
+                lin2=mm.Int8Linear(torch.randn(1024, 384, generator=g).cuda()), act2=torch.randn(9216, 384, generator=g).cuda())
 
 
 def test_graph_replay():
