@@ -45,7 +45,7 @@ template <typename T> __device__ __forceinline__ void store_chunk(T* d, int c, i
     if (c + kPer<T> <= V) {
         u32x4_t r;
         __builtin_memcpy(&r, t, 16);
-        *reinterpret_cast<typename Chunk<T>::type*>(d + c) = r;
+        __builtin_nontemporal_store(r, reinterpret_cast<typename Chunk<T>::type*>(d + c));
     } else {
 #pragma unroll
         for (int k = 0; k < kPer<T>; ++k)

@@ -300,8 +300,9 @@ def test_embedding(case, dt):
     want = torch.where(ok[:, None], table.double()[torch.where(ok, ids, torch.zeros_like(ids))] * scale, 0.0)
     assert ((y.double() - want).abs() <= want.abs() * half_step(dt) + H * want.abs()).all()
     live = ok & (ids != pad) if pad is not None else ok
-    want = torch.zeros(V, D, dtype=torch.float64, device="cuda").index_add_(0, ids[live], dy[live].double()) * scale
-    mass = torch.zeros(V, D, dtype=torch.float64, device="cuda").index_add_(0, ids[live], dy[live].double().abs()) * scale
+    il, dl = ids[live].cpu(), dy[live].double().cpu()
+    want = torch.zeros(V, D, dtype=torch.float64).index_add_(0, il, dl).cuda() * scale
+    mass = torch.zeros(V, D, dtype=torch.float64).index_add_(0, il, dl.abs()).cuda() * scale
     # chains of at most 32 inside a stretch, then a quarter of the stretches in a row, 2 + 1 more: each adds H of the partial sums
     tol = mass * H * (32 + n / 128 + 8)
     d = mm.scaled_embedding_grad(dy, ids, V, scale, padding_idx=pad)
@@ -494,6 +495,55 @@ def test_preference_step_with_a_frozen_8bit_model():
     assert (loss.double() - want).abs() < 1e-4 and (emb.weight.grad.double() - w.grad).abs().max() < 1e-4 * w.grad.abs().max()
     exact = torch.log_softmax((h @ w.t()).detach(), -1).gather(-1, labels.clamp(min=0)[..., None])[..., 0] * keep
     assert (ref.double() - exact.sum(1)).abs().max() < 0.05 * exact.sum(1).abs().max()      # 8 bits: a few per cent of a score
+
+
+def test_tuning_the_summariser():
+    """The framework's decoder under both losses: the parameters' gradients equal those of the same losses written in torch on the same logits."""
+    import multimodalsum_amd as mm
+    from multimodalsum_amd.modules import BartForEncConditionalGeneration, init_formula
+    from multimodalsum_amd.selftest import tiny_config
+    cfg = tiny_config()
+
+    def fresh():
+        m = BartForEncConditionalGeneration(cfg, device="cuda:0", dtype=torch.float32, deterministic=True)
+        init_formula(m)
+        m._engine.mark_weights_changed()
+        return m.train()
+
+    g = torch.Generator().manual_seed(2)
+    hid = (torch.randn(4, 2, 6, cfg.d_model, generator=g) * 0.5).cuda()
+    labels = torch.randint(4, cfg.vocab_size, (4, 9), generator=g).cuda()
+    labels[1, 6:] = cfg.pad_token_id
+    counted = torch.where(labels == cfg.pad_token_id, torch.full_like(labels, -100), labels)
+    rd = torch.zeros(4, 1, device="cuda")
+    with torch.no_grad():
+        first = fresh()(hid, rd, labels=labels)[0]
+        ref, old = mm.sequence_logprobs(first, counted)
+    ref, old, rtok, adv = ref - torch.arange(4.0, device="cuda"), old - 0.1, old + 0.2, torch.tensor([1.0, -0.5, 0.3, -2.0], device="cuda")
+
+    def in_torch(kind, logits):
+        keep = counted >= 0
+        lp = torch.log_softmax(logits.double(), -1).gather(-1, counted.clamp(min=0)[..., None])[..., 0] * keep
+        if kind == "pref":
+            r = lp.sum(1) - ref.double()
+            return -torch.nn.functional.logsigmoid(0.5 * (r[:2] - r[2:])).mean()
+        ratio, d = (lp - old.double()).exp(), (rtok.double() - lp)
+        a = adv.double()[:, None]
+        t = torch.maximum(-a * ratio, -a * ratio.clamp(0.8, 1.2)) + 0.1 * (d.exp() - d - 1)
+        return (t * keep).sum() / keep.sum()
+
+    pref, pol = mm.PreferenceLoss(beta=0.5), mm.ClippedPolicyLoss(kl_coef=0.1)
+    for kind, loss in (("pref", lambda x: pref(x, counted, ref)), ("pol", lambda x: pol(x, counted, old, adv, rtok))):
+        results = []
+        for f in (loss, lambda x: in_torch(kind, x)):
+            model = fresh()
+            value = f(model(hid, rd, labels=labels)[0])
+            value.backward()
+            results.append((value.detach().double(), {n: p.grad.clone() for n, p in model.named_parameters() if p.grad is not None}))
+        (v1, g1), (v2, g2) = results
+        assert (v1 - v2).abs() < 1e-5 * (1 + v2.abs()) and g1.keys() == g2.keys() and len(g1) > 10
+        for n in g1:                                                # f32 gradients of one model from logits' gradients that agree to f32
+            assert (g1[n] - g2[n]).abs().max() <= 1e-4 * g2[n].abs().max() + 1e-7, n
 
 
 def all_ops(s):
