@@ -7,7 +7,9 @@
 //
 // Bound: HBM.  The policy loss knows c as soon as the row's own log p is known, so its kernel reads the logits once and writes the
 // gradient once, the row waiting in registers in between.  The preference loss needs the sums over both summaries of a pair first:
-// statistics (read), pairs, gradient (read, write).
+// statistics (read), gradient (read, write), every workgroup of the second taking its pair's sums itself.
+// Measured (MI355X, 50,265 bf16 logits): scoring 72 x 141 rows 177 us (4.8 TB/s), policy loss 72 x 128 rows 315 us (5.4 TB/s), preference loss
+// of 36 pairs x 128 rows 419 us (4.1 TB/s of what has to move, 5.9 with the second reading).
 // Everything is summed in f32, in an order that depends on the sizes alone.
 #include "mmsum_device.h"
 #include "mmsum_kernels.h"
@@ -22,9 +24,12 @@ template <> struct Chunk<bf16_t> { typedef u32x4_t type __attribute__((aligned(2
 template <> struct Chunk<float> { typedef u32x4_t type __attribute__((aligned(4))); };
 template <typename T> constexpr int kPer = 16 / (int)sizeof(T);
 
-// columns [c, c + kPer) of a row, -inf behind V (adds nothing to a maximum or a sum of exponentials)
-template <typename T> __device__ __forceinline__ u32x4_t load_chunk(const T* x, int c, int V) {
-    if (c + kPer<T> <= V) return *reinterpret_cast<const typename Chunk<T>::type*>(x + c);
+// columns [c, c + kPer) of a row, -inf behind V (adds nothing to a maximum or a sum of exponentials); LAST: read past the caches
+template <typename T, bool LAST = false> __device__ __forceinline__ u32x4_t load_chunk(const T* x, int c, int V) {
+    if (c + kPer<T> <= V) {
+        if constexpr (LAST) return __builtin_nontemporal_load(reinterpret_cast<const typename Chunk<T>::type*>(x + c));
+        else return *reinterpret_cast<const typename Chunk<T>::type*>(x + c);
+    }
     T t[kPer<T>];
 #pragma unroll
     for (int k = 0; k < kPer<T>; ++k) t[k] = c + k < V ? x[c + k] : from_f32<T>(-INFINITY);
@@ -38,6 +43,7 @@ template <typename T> __device__ __forceinline__ void unpack(const u32x4_t& r, f
 #pragma unroll
     for (int k = 0; k < kPer<T>; ++k) f[k] = to_f32(t[k]);
 }
+// past the caches: a gradient of the logits' size would push out what the second reading finds there (477 -> 430 us)
 template <typename T> __device__ __forceinline__ void store_chunk(T* d, int c, int V, const float (&g)[kPer<T>]) {
     T t[kPer<T>];
 #pragma unroll
@@ -125,6 +131,7 @@ template <typename T> struct RowArgs {
     const T* logits; long ld; const int64_t* labels; int V;
     float* logp; float* stats;      // stats [R][2] = {m, s}; may be NULL
     T* dlogits; long ldd; int W;
+    int past;                       // rows below it are read past the caches
     PolicyArgs pol;
 };
 
@@ -163,8 +170,13 @@ __global__ __launch_bounds__(NT, NT == 512 && !POLICY ? 6 : 4) void row_kernel(R
     }
     const T* x = a.logits + (long)row * a.ld;                       // no __restrict__: d may be x
     u32x4_t reg[MAXC];
+    if (POLICY || row < a.past) {
 #pragma unroll
-    for (int i = 0; i < MAXC; ++i) reg[i] = load_chunk(x, (i * NT + tid) * kPer<T>, a.V);
+        for (int i = 0; i < MAXC; ++i) reg[i] = load_chunk<T, true>(x, (i * NT + tid) * kPer<T>, a.V);
+    } else {
+#pragma unroll
+        for (int i = 0; i < MAXC; ++i) reg[i] = load_chunk<T>(x, (i * NT + tid) * kPer<T>, a.V);
+    }
     const float xy = to_f32(x[y]);                                   // read before any thread writes: d may be x
     float w = 0.f;
     if constexpr (POLICY) w = policy_weight(a.pol, row, tid & 63);
@@ -382,7 +394,7 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(const T* logits, long 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long c = c0i + (long)u * NT * kPer<T>;
-            if (c < V) reg[u] = load_chunk(x, (int)c, V);
+            if (c < V) reg[u] = load_chunk<T, true>(x, (int)c, V);
         }
     };
     float c0 = 0.f;
@@ -518,8 +530,12 @@ int launch_bwd(const void* logits, long ld, const int64_t* labels, const float* 
 // Statistics, then the gradient from the last row to the first: the rows read last are still in the 256 MB memory-side cache.
 template <typename T>
 int preference_rows(const void* logits, long ld, void* dlogits, long ldd, int W, float* stats, const PairArgs& pairs, hipStream_t s) {
+    RowArgs<T> a = row_args<T>(logits, ld, pairs.labels, pairs.V, const_cast<float*>(pairs.logp), stats);
     const int R = 2 * pairs.P * pairs.T;
-    const RowArgs<T> a = row_args<T>(logits, ld, pairs.labels, pairs.V, const_cast<float*>(pairs.logp), stats);
+    // all rows but the last 400 MB are read past the caches, which leaves those to the second reading (36 pairs of 128 x 50,265: 428 -> 419 us;
+    // pairs in separate launches of 110 .. 480 MB: 487 .. 411 us)
+    const long keep = (400L << 20) / (ld * (long)sizeof(T));
+    a.past = keep < R ? R - (int)keep : 0;
     const int rc = launch_rows<T, false>(a, R, s);
     if (rc != MMSUM_OK) return rc;
     hipLaunchKernelGGL((logprob_bwd_kernel<T, true>), dim3(R), dim3(256), 0, s, a.logits, ld, pairs.labels, stats, nullptr, 1, nullptr, static_cast<T*>(dlogits), ldd, W, pairs.V,
