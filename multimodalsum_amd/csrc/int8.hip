@@ -439,10 +439,12 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_i8_ring_kernel(I8Args p) {
         if (st < nst) issue(st);
     for (int st = 0; st < nst; ++st) {
         const int ahead = nst - 1 - st;                            // stages requested behind this one, NST - 2 of them at most
-        if (ahead >= NST - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * PPW) : "memory");
-        else if (NST > 3 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PPW) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // (lgkmcnt: this wave's reads of stage st - 1 are back; its slot is requested into behind the barrier)
+        if (ahead >= NST - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * PPW) : "memory");
+        else if (NST > 3 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PPW) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");                               // no read of the stage above its barrier
         const char* const A = smem + st % NST * STAGE + wm * (TM * 32) * 128 + fo;
         const char* const B = smem + st % NST * STAGE + BM * 128 + wn * (TN * 32) * 128 + fo;
         const int yd = (fo ^ 64) - fo;
