@@ -455,8 +455,8 @@ def test_int8_linear_extremes_and_shapes():
     for M, N in ((5, 40), (100, 200), (2500, 4100)):
         a, b = torch.randint(-127, 128, (M, 384), dtype=torch.int8, generator=g).cuda(), torch.randint(-127, 128, (N, 512), dtype=torch.int8, generator=g).cuda()
         one = torch.ones(max(M, N), device="cuda")
-        y = kn.gemm_i8(a[:, 128:], one[:M], b[:, 128:384], one[:N], torch.empty(M, N, device="cuda"))
-        assert torch.equal(y.double(), torch.mm(a[:, 128:].double(), b[:, 128:384].double().t().contiguous()))      # sums below 2^24
+        got = kn.gemm_i8(a[:, 128:], one[:M], b[:, 128:384], one[:N], torch.empty(M, N, device="cuda"))
+        assert torch.equal(got.double(), torch.mm(a[:, 128:].double(), b[:, 128:384].double().t().contiguous()))      # sums below 2^24
     # columns and rows behind the result stay as they were
     q, s = kn.quantize_rows(x[1])
     out = torch.full((8, 60), float("nan"), device="cuda")
