@@ -455,7 +455,7 @@ int mmsum_policy_loss(int dtype, const void* logits, long ld, const int64_t* lab
 int mmsum_embed_fwd(int dtype, const int64_t* ids, const void* E, long lde, void* y, long ldy, long n, int V, int D, float scale, void* stream);
 /* dE[v] (+)= scale sum of dy[i] over ids[i] == v, f32 [V, D] packed, written whole unless `accumulate` (then only rows that ids name change).  By
  * sorted tokens, without floating-point atomics: reproducible.  ids outside 0 .. V-1 and pad_id (-1: none) leave no gradient.
- * workspace: mmsum_embed_bwd_workspace bytes; n < 2^30. */
+ * workspace: mmsum_embed_bwd_workspace bytes (0: none needed); n < 2^30. */
 long mmsum_embed_bwd_workspace(long n, int D);
 int mmsum_embed_bwd(int dtype, const void* dy, long lddy, const int64_t* ids, long n, int V, int D, float scale, int64_t pad_id, int accumulate, float* dE,
                     void* workspace, void* stream);

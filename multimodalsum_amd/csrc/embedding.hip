@@ -79,24 +79,15 @@ __device__ __forceinline__ int wave_rank(volatile int* cnt, uint32_t d, bool act
     return base + before;
 }
 
-// The rows that no id names have to be zero.  Sorting is a chain of short launches that leave the memory idle, so all of dE is cleared in
-// them, by workgroups behind the sorting ones, and the sums write the named rows over it afterwards.
-struct ZeroFill { float* p; long n; int first, blocks; };          // workgroups first .. first + blocks - 1 clear n floats (blocks 0: none)
-template <int NT> __device__ __forceinline__ void zero_fill(const ZeroFill& z) {
-    const long quads = ((uintptr_t)z.p & 15) == 0 ? z.n / 4 : 0;
-    const long t = (long)((int)blockIdx.x - z.first) * NT + threadIdx.x, step = (long)z.blocks * NT;
-    for (long i = t; i < quads; i += step) reinterpret_cast<f32x4_t*>(z.p)[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (long i = quads * 4 + t; i < z.n; i += step) z.p[i] = 0.f;
-}
-
 constexpr int kSub = 1024;               // elements a workgroup ranks at a time (four rounds of its four waves)
 constexpr int kMaxTiles = 256;
+constexpr long kHistBytes = (long)kMaxTiles * 256 * 4;
 
-// hist[tile][256]: digits of every tile
+// hist[tile][256]: digits of every tile.  (Counting a later pass's digits with atomics while the pass in front of it places the elements
+// saves a launch and was slower: the frequent ids meet in a few counters, 14 -> 28 us at 147,456 ids.)
 template <bool FIRST>
 __global__ __launch_bounds__(256) void sort_hist_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys, int n, int tile, int V, int64_t pad_id, int shift,
-                                                        int* __restrict__ hist, ZeroFill z) {
-    if ((int)blockIdx.x >= z.first) return zero_fill<256>(z);
+                                                        int* __restrict__ hist) {
     __shared__ int h[256];
     h[threadIdx.x] = 0;
     __syncthreads();
@@ -110,8 +101,7 @@ __global__ __launch_bounds__(256) void sort_hist_kernel(const int64_t* __restric
 template <bool FIRST>
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys, const int* __restrict__ pos, int n, int tile,
                                                            int tiles, int V, int64_t pad_id, int shift, const int* __restrict__ hist, uint32_t* __restrict__ okeys,
-                                                           int* __restrict__ opos, ZeroFill z) {
-    if ((int)blockIdx.x >= z.first) return zero_fill<256>(z);
+                                                           int* __restrict__ opos) {
     __shared__ int cnt[4][256], wbase[4][256], scan[256];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int total = 0, before = 0;
@@ -171,8 +161,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const int64_t* __rest
 
 // the whole sort of up to 4096 ids in one workgroup's LDS
 constexpr int kSmall = 4096;
-__global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restrict__ ids, int n, int V, int64_t pad_id, int bits, uint32_t* __restrict__ okeys, int* __restrict__ opos, ZeroFill z) {
-    if ((int)blockIdx.x >= z.first) return zero_fill<1024>(z);
+__global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restrict__ ids, int n, int V, int64_t pad_id, int bits, uint32_t* __restrict__ okeys, int* __restrict__ opos) {
     __shared__ uint32_t lk[2][kSmall];
     __shared__ uint16_t lp[2][kSmall];
     __shared__ int cnt[16][256];
@@ -239,17 +228,17 @@ __global__ __launch_bounds__(256) void embed_bwd_few_kernel(const T* __restrict_
     for (int i = 0; i < kFew / 256; ++i) all[i] = i * 256 + tid < n ? ids[i * 256 + tid] : -1;
     for (long v0 = (long)blockIdx.x * rows; v0 < V; v0 += (long)gridDim.x * rows) {      // the ids stay in registers from one stretch of rows to the next
     const int here = (int)(V - v0 < rows ? V - v0 : rows);
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < kFew / 256; ++i) any |= all[i] >= v0 && all[i] < v0 + here && all[i] != pad_id;
-    if (!__syncthreads_or(any)) {                                      // none of the rows is named: most workgroups of a large table
-        if (accumulate) continue;
+    if (!accumulate) {                                                 // zeros first: they need no id and keep the memory busy while the ids arrive
         float* const z = dE + v0 * D;
         const long cells = (long)here * D, quads = ((uintptr_t)z & 15) == 0 ? cells / 4 : 0;
         for (long i = tid; i < quads; i += 256) reinterpret_cast<f32x4_t*>(z)[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         for (long i = quads * 4 + tid; i < cells; i += 256) z[i] = 0.f;
-        continue;
     }
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < kFew / 256; ++i) any |= all[i] >= v0 && all[i] < v0 + here && all[i] != pad_id;
+    if (!__syncthreads_or(any)) continue;                              // none of the rows is named: most stretches of a large table
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                   // the zeros are in front of the sums (other waves' too: barriers follow)
     start[tid] = 0;
     int L = 0;
 #pragma unroll
@@ -304,7 +293,7 @@ __global__ __launch_bounds__(256) void embed_bwd_few_kernel(const T* __restrict_
     const int tpr = 1 << tpr_log2, groups = 256 >> tpr_log2;
     for (int r = tid >> tpr_log2; r < here; r += groups) {
         const int lo = start[r], hi = start[r + 1];
-        if (accumulate && lo == hi) continue;
+        if (lo == hi) continue;
         for (int c = (tid & (tpr - 1)) * VEC; c < D; c += tpr * VEC) {
             float acc[VEC] = {};
             for (int i0 = lo; i0 < hi; i0 += AHEAD) {
@@ -458,12 +447,36 @@ __global__ __launch_bounds__(256) void stretch_sum_kernel(const T* __restrict__ 
     }
 }
 
+// Rows of the table that no id names: zeros.  A wave takes 16 neighbouring rows, its lanes bisect the sorted keys for them.
+__device__ __forceinline__ void clear_absent(const uint32_t* __restrict__ keys, int n, int V, int D, float* __restrict__ dE, long v0) {
+    const int lane = threadIdx.x & 63;
+    if (v0 >= V) return;
+    const uint32_t v = (uint32_t)(v0 + (lane & 15));
+    int a = 0, b = n;
+    while (a < b) {
+        const int mid = (int)(((long)a + b) / 2);
+        if (keys[mid] < v) a = mid + 1;
+        else b = mid;
+    }
+    const uint64_t absent = __ballot(!(a < n && keys[a] == v));
+    for (int r = 0; r < 16 && v0 + r < V; ++r) {
+        if (!((absent >> r) & 1)) continue;
+        float* const row = dE + (v0 + r) * D;
+        if (D % 4 == 0 && ((uintptr_t)dE & 15) == 0) {
+            for (int c = lane * 4; c < D; c += 256) *reinterpret_cast<f32x4_t*>(row + c) = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        } else {
+            for (int c = lane; c < D; c += 64) row[c] = 0.f;
+        }
+    }
+}
+
 // A token that begins in stretch st and goes on: part[st][1] + part[st + 1][0] + ... in order.  One workgroup a stretch, a thread four
 // columns (VEC: as one vector), up to AHEAD stretches requested at a time: the most frequent tokens of a text (a few per cent of it, over a
-// hundred stretches) are the kernel's tail.
+// hundred stretches) are the kernel's tail.  Workgroups from `joins` on clear the absent rows: the joins wait for memory, the clearing fills it.
 template <bool VEC>
 __global__ __launch_bounds__(256) void stretch_join_kernel(const uint32_t* __restrict__ keys, int n, int sl, int V, int D, float scale, int accumulate, const float* __restrict__ part,
-                                                           float* __restrict__ dE) {
+                                                           float* __restrict__ dE, int joins) {
+    if ((int)blockIdx.x >= joins) return clear_absent(keys, n, V, D, dE, ((long)((int)blockIdx.x - joins) * 4 + (threadIdx.x >> 6)) * 16);
     constexpr int AHEAD = 16;
     const int lane = threadIdx.x & 63;
     const long st = blockIdx.x, begin = st * sl, end = begin + sl;      // end < n: the grid leaves the last stretch out
@@ -547,36 +560,21 @@ int embed_bwd_t(const void* dy, long lddy, const int64_t* ids, int n, int V, int
     uint32_t* k1 = reinterpret_cast<uint32_t*>(ws + 2 * nb);
     int* p1 = reinterpret_cast<int*>(ws + 3 * nb);
     int* hist = reinterpret_cast<int*>(ws + 4 * nb);
-    float* part = reinterpret_cast<float*>(ws + 4 * nb + kMaxTiles * 256 * 4);
+    float* part = reinterpret_cast<float*>(ws + 4 * nb + kHistBytes);
     int bits = 0;
     while (bits < 32 && ((uint32_t)V >> bits) != 0) ++bits;
-    const long cells = accumulate ? 0 : (long)V * D;
-    auto fill = [&](int first, int step, int steps) {                // the step-th part of the clearing, about 64 KB a workgroup
-        ZeroFill z = {nullptr, 0, first, 0};
-        const long per = ((cells + steps - 1) / steps + 3) & ~3L, lo = step * per, cnt = lo >= cells ? 0 : (cells - lo < per ? cells - lo : per);
-        if (cnt > 0) {
-            z.p = dE + lo;
-            z.n = cnt;
-            const long want = (cnt + 16383) / 16384;
-            z.blocks = (int)(want < 1024 ? want : 1024);
-        }
-        return z;
-    };
     if (n <= kSmall) {
-        const ZeroFill z = fill(1, 0, 1);
-        hipLaunchKernelGGL(sort_small_kernel, dim3(1 + z.blocks), dim3(1024), 0, s, ids, n, V, pad_id, bits, k0, p0, z);
+        hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(1024), 0, s, ids, n, V, pad_id, bits, k0, p0);
     } else {
         const SortPlan sp = sort_plan(n);
-        const int steps = (bits + 7) / 8;
-        for (int shift = 0, step = 0; shift < bits; shift += 8, ++step) {
-            const ZeroFill z0 = {nullptr, 0, sp.tiles, 0}, z1 = fill(sp.tiles, step, steps);      // beside the scatters, the longer ones
-            const dim3 g0(sp.tiles), g1(sp.tiles + z1.blocks);
+        const dim3 g(sp.tiles);
+        for (int shift = 0; shift < bits; shift += 8) {
             if (shift == 0) {
-                hipLaunchKernelGGL((sort_hist_kernel<true>), g0, dim3(256), 0, s, ids, nullptr, n, sp.tile, V, pad_id, shift, hist, z0);
-                hipLaunchKernelGGL((sort_scatter_kernel<true>), g1, dim3(256), 0, s, ids, nullptr, nullptr, n, sp.tile, sp.tiles, V, pad_id, shift, hist, k0, p0, z1);
+                hipLaunchKernelGGL((sort_hist_kernel<true>), g, dim3(256), 0, s, ids, nullptr, n, sp.tile, V, pad_id, shift, hist);
+                hipLaunchKernelGGL((sort_scatter_kernel<true>), g, dim3(256), 0, s, ids, nullptr, nullptr, n, sp.tile, sp.tiles, V, pad_id, shift, hist, k0, p0);
             } else {
-                hipLaunchKernelGGL((sort_hist_kernel<false>), g0, dim3(256), 0, s, ids, k0, n, sp.tile, V, pad_id, shift, hist, z0);
-                hipLaunchKernelGGL((sort_scatter_kernel<false>), g1, dim3(256), 0, s, ids, k0, p0, n, sp.tile, sp.tiles, V, pad_id, shift, hist, k1, p1, z1);
+                hipLaunchKernelGGL((sort_hist_kernel<false>), g, dim3(256), 0, s, ids, k0, n, sp.tile, V, pad_id, shift, hist);
+                hipLaunchKernelGGL((sort_scatter_kernel<false>), g, dim3(256), 0, s, ids, k0, p0, n, sp.tile, sp.tiles, V, pad_id, shift, hist, k1, p1);
                 uint32_t* tk = k0; k0 = k1; k1 = tk;
                 int* tp = p0; p0 = p1; p1 = tp;
             }
@@ -590,12 +588,16 @@ int embed_bwd_t(const void* dy, long lddy, const int64_t* ids, int n, int V, int
     if (vec) hipLaunchKernelGGL((stretch_sum_kernel<T, true>), grid, dim3(256), 0, s, (const T*)dy, lddy, k0, p0, n, sl, V, D, scale, accumulate, part, dE);
     else hipLaunchKernelGGL((stretch_sum_kernel<T, false>), grid, dim3(256), 0, s, (const T*)dy, lddy, k0, p0, n, sl, V, D, scale, accumulate, part, dE);
     const long joins = ((long)n - 1) / sl;                    // stretches with another one behind them
-    if (joins > 0 && vec) hipLaunchKernelGGL((stretch_join_kernel<true>), dim3((unsigned)joins), dim3(256), 0, s, k0, n, sl, V, D, scale, accumulate, part, dE);
-    else if (joins > 0) hipLaunchKernelGGL((stretch_join_kernel<false>), dim3((unsigned)joins), dim3(256), 0, s, k0, n, sl, V, D, scale, accumulate, part, dE);
+    const dim3 jg((unsigned)(joins + (accumulate ? 0 : (V + 63L) / 64)));
+    if (jg.x == 0) return ok();
+    if (vec) hipLaunchKernelGGL((stretch_join_kernel<true>), jg, dim3(256), 0, s, k0, n, sl, V, D, scale, accumulate, part, dE, (int)joins);
+    else hipLaunchKernelGGL((stretch_join_kernel<false>), jg, dim3(256), 0, s, k0, n, sl, V, D, scale, accumulate, part, dE, (int)joins);
     return ok();
 }
 
-__global__ __launch_bounds__(256) void zero_kernel(ZeroFill z) { zero_fill<256>(z); }
+__global__ __launch_bounds__(256) void zero_kernel(float* __restrict__ p, long n) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) p[i] = 0.f;
+}
 
 }  // namespace
 
@@ -607,18 +609,18 @@ extern "C" int mmsum_embed_fwd(int dtype, const int64_t* ids, const void* E, lon
 }
 
 extern "C" long mmsum_embed_bwd_workspace(long n, int D) {
-    if (n < 0 || n > 0x3fffffffL || D <= 0) return 0;
-    return 4 * align16(n * 4) + kMaxTiles * 256 * 4 + (n + stretch_of(n) - 1) / stretch_of(n) * 2 * D * (long)sizeof(float);
+    if (n <= kFew || n > 0x3fffffffL || D <= 0) return 0;              // few ids need none
+    return 4 * align16(n * 4) + kHistBytes + (n + stretch_of(n) - 1) / stretch_of(n) * 2 * D * (long)sizeof(float);
 }
 extern "C" int mmsum_embed_bwd(int dtype, const void* dy, long lddy, const int64_t* ids, long n, int V, int D, float scale, int64_t pad_id, int accumulate, float* dE,
                                void* workspace, void* stream) {
     if (n < 0 || n > 0x3fffffffL || V <= 0 || V > 0x7ffffff0 || D <= 0 || lddy < D) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
-    if (n > 0 && workspace == nullptr) return MMSUM_ERR_WORKSPACE;
+    if (n > kFew && workspace == nullptr) return MMSUM_ERR_WORKSPACE;
     if (((uintptr_t)workspace & 15) || ((uintptr_t)dE & 3) || ((uintptr_t)dy & (dtype == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
     hipStream_t s = (hipStream_t)stream;
     if (n == 0) {
-        if (!accumulate) hipLaunchKernelGGL(zero_kernel, dim3(1024), dim3(256), 0, s, ZeroFill{dE, (long)V * D, 0, 1024});
+        if (!accumulate) hipLaunchKernelGGL(zero_kernel, dim3(1024), dim3(256), 0, s, dE, (long)V * D);
         return ok();
     }
     if (dtype == MMSUM_BF16) return embed_bwd_t<bf16_t>(dy, lddy, ids, (int)n, V, D, scale, pad_id, accumulate, dE, static_cast<char*>(workspace), s);

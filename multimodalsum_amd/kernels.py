@@ -818,7 +818,8 @@ def embed_bwd(dy, ids, V, scale=1.0, pad_id=None, out=None, accumulate=False):
     dev = _device(dy, ids, out)
     if out is None:
         out = torch.empty(V, D, dtype=torch.float32, device=dev)
-    ws = torch.empty(max(1, lib.mmsum_embed_bwd_workspace(n, D)), dtype=torch.uint8, device=dev)
+    nbytes = lib.mmsum_embed_bwd_workspace(n, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _launch("mmsum_embed_bwd", dev, _dt(dy), _p(dy), lddy, _p(flat), n, V, D, float(scale), -1 if pad_id is None else int(pad_id), int(bool(accumulate)), _p(out), _p(ws))
     return out
 

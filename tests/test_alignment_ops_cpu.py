@@ -35,7 +35,7 @@ def test_c_entries_refuse():
     assert lib.mmsum_embed_fwd(BF, FAKE, FAKE, 7, FAKE, 8, 4, 10, 8, 1.0, None) == -1 and lib.mmsum_embed_fwd(3, FAKE, FAKE, 8, FAKE, 8, 4, 10, 8, 1.0, None) == -2
     assert lib.mmsum_embed_fwd(0, FAKE, FAKE + 2, 8, FAKE, 8, 4, 10, 8, 1.0, None) == -3
     eb = lib.mmsum_embed_bwd
-    assert eb(BF, FAKE, 8, FAKE, 4, 10, 8, 1.0, -1, 0, FAKE, None, None) == -4 and eb(BF, FAKE, 8, FAKE, 2 ** 30, 10, 8, 1.0, -1, 0, FAKE, FAKE, None) == -1
+    assert eb(BF, FAKE, 8, FAKE, 4000, 10, 8, 1.0, -1, 0, FAKE, None, None) == -4 and eb(BF, FAKE, 8, FAKE, 2 ** 30, 10, 8, 1.0, -1, 0, FAKE, FAKE, None) == -1
     assert eb(BF, FAKE, 8, FAKE, 4, 10, 8, 1.0, -1, 0, FAKE, FAKE + 8, None) == -3 and eb(BF, FAKE, 7, FAKE, 4, 10, 8, 1.0, -1, 0, FAKE, FAKE, None) == -1
     assert lib.mmsum_quantize_i8(BF, FAKE, 8, 4, 8, FAKE, 65, FAKE, None) == -1 and lib.mmsum_quantize_i8(BF, FAKE, 8, 4, 8, FAKE + 8, 128, FAKE, None) == -3
     g8 = lib.mmsum_gemm_i8
