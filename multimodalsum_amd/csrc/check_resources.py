@@ -19,7 +19,8 @@ LIMITS = {                    # kernel-name substring -> (max arch VGPRs, max sc
     # accumulator layout and spills a few more registers in that epilogue; more specific entries win
     "gemm_nt_w4_kernelILi0ELi3E": (256, 96, 24),
 }
-INT8_LIMITS = {"gemm_i8_w4_kernel": (256, 0, 0)}             # int8.hip: the same pipeline on 8-bit operands, "+a" accumulators
+INT8_LIMITS = {"gemm_i8_w4_kernel": (256, 0, 0),             # int8.hip: the same pipeline on 8-bit operands, "+a" accumulators
+               "gemm_i8_ring_kernel": (256, 0, 0)}           # two workgroups of four waves on a CU
 
 
 def main(path):

@@ -392,12 +392,15 @@ __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(I8Args p) {
 #undef I8_DMA
 }
 
-// Between the two: 64x64 tiles, one a workgroup of 2x2 waves, the stages in a ring that runs NST - 1 of them ahead of the products (64 KB of
-// LDS: two workgroups a CU hide each other's waits).  Operand rows, swizzle and the order of the weight rows as above.
+// One tile of BM x BN a workgroup of WM x WN waves, the stages in a ring that runs NST - 1 of them ahead of the products, at most 80 KB of
+// LDS: two workgroups a CU, and the main loop of one runs under the waits and the epilogue of the other.  Operand rows, swizzle and the order
+// of the weight rows as above.  192x128 (two stages) for large products of a short sum, where the epilogue weighs; 64x64 (four) for small ones.
+// Measured (MI355X, 192x128): 36,864 x 4,096 x 1,024 178 us, with GELU 207; 36,864 x 1,024 x 4,096 127 us = 2,435 TOP/s.
 template <typename T, bool GELU, int BM, int BN, int WM, int WN, int NST>
-__global__ __launch_bounds__(WM* WN * 64) void gemm_i8_ring_kernel(I8Args p) {
+__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_i8_ring_kernel(I8Args p) {
     constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 128, PA = BM / 8 / NW, PB = BN / 8 / NW, PPW = PA + PB;
-    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && (32 % (8 * NW) == 0 || (8 * NW) % 32 == 0), "whole pieces for every wave");
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole pieces for every wave");
+    static_assert(NST * STAGE <= 81920, "two workgroups a CU");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -481,6 +484,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_i8_ring_kernel(I8Args p) {
             load_cols<WHOLE>(p.sb, nc + 32 * j, p.N, sw[j]);
             if (p.bias != nullptr) load_cols<WHOLE>(p.bias, nc + 32 * j, p.N, bs[j]);
         }
+#pragma unroll
+        for (int k = 0; k < 2 * TM; ++k) asm volatile("" : "+v"(sx[k]));
 #pragma unroll
         for (int j = 0; j < TN; ++j) { retire(sw[j]); retire(bs[j]); }
         T* row = static_cast<T*>(p.C) + (long)mr * p.ldc + nc;
@@ -612,7 +617,6 @@ int launch_few(const I8Args& p, const X* x, long ldx, int Kx, hipStream_t s) {
 template <typename T, bool GELU, int BM, int BN, int WM, int WN, int NST>
 int launch_ring(const I8Args& p, hipStream_t s) {
     const long tiles = (p.M + (long)BM - 1) / BM * ((p.N + (long)BN - 1) / BN);
-    if (tiles > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
     const size_t lds = (size_t)NST * (BM + BN) * 128;
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_ring_kernel<T, GELU, BM, BN, WM, WN, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
         return MMSUM_ERR_HIP;
@@ -623,19 +627,29 @@ int launch_ring(const I8Args& p, hipStream_t s) {
 template <typename T, bool GELU>
 int launch_product(const I8Args& p, hipStream_t s) {
     if (p.M <= 64) {
-        // wide workgroups where there are still enough of them for every CU: they read the activations less often
+        // Workgroups of 64 columns where there are still two of them for every CU: they read the activations less often (32 x 50,265 x 1,024:
+        // 16.1 us, in 16 columns 19); below that 16 columns fill more CUs
         const bool wide = p.N >= 32768;
         if (p.M <= 16) return wide ? launch_few<T, GELU, 1, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 1, 1, false, float>(p, nullptr, 0, 0, s);
         if (p.M <= 32) return wide ? launch_few<T, GELU, 2, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 2, 1, false, float>(p, nullptr, 0, 0, s);
         return wide ? launch_few<T, GELU, 4, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 4, 1, false, float>(p, nullptr, 0, 0, s);
     }
-    // 256x256 tiles from about half a round of the CUs on, unless most of a tile is behind the edge (us, 64x64 | 256x256, bf16 out):
-    // 1152x4096x1024 (80 tiles) 14 | 29, 2304x4096x1024 (144) 22 | 20, 9216x1024x4096 (144) 58 | 49, 18432x4096x1024 142 | 88; 128x50265x1024 (197) 21 | 31
-    const long t256 = (p.M + 255L) / 256 * ((p.N + 255L) / 256);
-    if (t256 < 144 || p.M < 192 || p.N < 192) return launch_ring<T, GELU, 64, 64, 2, 2, 4>(p, s);
-    const int cus = cu_count();
+    // The tile whose rounds of the CUs take the least time, in tenths of a us: so much a stage of 128 k and so much an epilogue, fitted to the
+    // three on 24 shapes (worst choice 9 % over the best).  Measured (us, 64x64 | 192x128 | 256x256, bf16 out):
+    //   36,864 x 4,096 x 1,024   318 | 178 | 184, with GELU 345 | 207 | 234        8,192 x 8,192 x 8,192    778 | 445 | 381
+    //   36,864 x 1,024 x 4,096   223 | 127 | 141 (2 1/4 rounds of 256x256)        16,384 x 4,096 x 4,096   400 | 237 | 205 (5 3/8 of 192x128)
+    //    9,216 x 1,024 x 1,024    23 |  16 |  20                                    2,048 x 2,048 x 2,048    16 |  23 |  19
+    //   256 x 50,265 x 1,024      36 |  37 |  27                                      128 x 50,265 x 1,024    21 |  27 |  22
+    // The larger tiles are not for fewer than 129 rows: their loads of the missing rows still take their turn.
+    auto up = [](long a, long b) { return (a + b - 1) / b; };
+    const long cus = cu_count(), st = p.K / 128;
+    const long t256 = up(p.M, 256) * up(p.N, 256), t192 = up(p.M, 192) * up(p.N, 128), t64 = up(p.M, 64) * up(p.N, 64);
+    if (t64 > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    const long half = up(t192, cus);                               // rounds of one workgroup a CU: two at once take 4/3 of one alone
+    const long us256 = up(t256, cus) * (14 * st + 70 + (GELU ? 50 : 0)), us192 = (2 * half + half % 2) * (11 * st + 60 + (GELU ? 20 : 0)) / 4, us64 = up(t64, 2 * cus) * (4 * st + 14);
+    if (p.M <= 128 || (us64 <= us192 && us64 <= us256)) return launch_ring<T, GELU, 64, 64, 2, 2, 4>(p, s);
+    if (us192 <= us256) return launch_ring<T, GELU, 192, 128, 2, 2, 2>(p, s);
     const size_t lds = 5 * kStageBytes;
-    if (t256 > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_w4_kernel<T, GELU>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return MMSUM_ERR_HIP;
     hipLaunchKernelGGL((gemm_i8_w4_kernel<T, GELU>), dim3((unsigned)(t256 < cus ? t256 : cus)), dim3(256), lds, s, p);
     return ok();

@@ -428,6 +428,32 @@ def test_int8_linear(M, N, K, dt):
             assert ((y.double() - want).abs() <= tol).all(), ((y.double() - want).abs() / tol).max().item()
 
 
+@pytest.mark.parametrize("M,N,K", [(2305, 2100, 384), (2500, 6500, 900), (129, 60000, 300), (573, 12001, 700), (4353, 4099, 2600), (3100, 4100, 1000), (8100, 2040, 60), (4099, 7000, 300),
+                                   (8000, 8001, 1100)])
+@pytest.mark.parametrize("out", DTYPES)
+def test_int8_product_at_tile_edges(M, N, K, out):
+    """The large tiles, several to a workgroup too, with rows, columns and k behind the last whole tile; nothing is written around the result."""
+    from multimodalsum_amd import kernels as kn
+    g = torch.Generator(device="cuda").manual_seed(M + K)
+    Kp = -(-K // kn.I8_K_STEP) * kn.I8_K_STEP
+    qx = torch.zeros(M, Kp, dtype=torch.int8, device="cuda")
+    qw = torch.zeros(N, Kp, dtype=torch.int8, device="cuda")
+    qx[:, :K] = torch.randint(-127, 128, (M, K), generator=g, device="cuda")
+    qw[:, :K] = torch.randint(-127, 128, (N, K), generator=g, device="cuda")
+    sx, sw, bias = (torch.rand(n, generator=g, device="cuda") for n in (M, N, N))
+    want = torch.mm(qx.double(), qw.double().t().contiguous()) * sx.double()[:, None] * sw.double()
+    for b, gelu in ((None, False), (bias, False), (bias, True)):
+        ref = want if b is None else want + b.double()
+        tol = (want.abs() + 1) * (8 if not gelu else 40) * H         # as for the linear layer; the bias is below 1
+        if gelu:
+            ref = 0.5 * ref * (1 + torch.erf(ref / math.sqrt(2.0)))
+        wide = torch.full((M + 2, N + 6), float("nan"), dtype=out, device="cuda")
+        kn.gemm_i8(qx, sx, qw, sw, wide[1:-1, 3:N + 3], b, gelu)
+        y = wide[1:-1, 3:N + 3].double()
+        assert ((y - ref).abs() <= tol + ref.abs() * half_step(out) + torch.finfo(out).tiny).all()
+        assert torch.isnan(wide[0]).all() and torch.isnan(wide[-1]).all() and torch.isnan(wide[:, :3]).all() and torch.isnan(wide[:, N + 3:]).all()
+
+
 def test_int8_linear_extremes_and_shapes():
     from multimodalsum_amd import Int8Linear
     g = torch.Generator().manual_seed(3)
