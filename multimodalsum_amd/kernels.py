@@ -662,7 +662,8 @@ def _dlogits_of(dlogits, logits, N, T, V, ld):
     (unless they are a narrow view of something much wider)."""
     if dlogits is None:
         ld = ld if ld - V < 256 else V
-        return torch.empty(N, T, ld, dtype=logits.dtype, device=logits.device)[:, :, :V], ld, V
+        buf = torch.empty(N, T, ld, dtype=logits.dtype, device=logits.device)
+        return buf if ld == V else buf[:, :, :V], ld, V
     if dlogits.dtype != logits.dtype:
         raise TypeError("dlogits: %s expected, got %s" % (logits.dtype, dlogits.dtype))
     n, t, W, ldd = _rows_of(dlogits, "dlogits")
@@ -818,6 +819,8 @@ def embed_bwd(dy, ids, V, scale=1.0, pad_id=None, out=None, accumulate=False):
     dev = _device(dy, ids, out)
     if out is None:
         out = torch.empty(V, D, dtype=torch.float32, device=dev)
+    else:
+        _apart(dy, out)
     nbytes = lib.mmsum_embed_bwd_workspace(n, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _launch("mmsum_embed_bwd", dev, _dt(dy), _p(dy), lddy, _p(flat), n, V, D, float(scale), -1 if pad_id is None else int(pad_id), int(bool(accumulate)), _p(out), _p(ws))

@@ -641,3 +641,14 @@ def test_two_streams():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(torch.equal(torch.nan_to_num(x.float()), torch.nan_to_num(y.float())) for x, y in zip(a, b))
+
+
+def test_results_that_overlap_what_is_read_are_refused():
+    from multimodalsum_amd import kernels as kn
+    buf = torch.zeros(20, 8, device="cuda")
+    ids = torch.tensor([1, 2], device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        kn.embed_bwd(buf[9:11], ids, 10, out=buf[:10])
+    assert torch.equal(kn.embed_bwd(buf[10:12] + 1, ids, 10, out=buf[:10])[:4, 0].cpu(), torch.tensor([0.0, 1.0, 1.0, 0.0]))
+    out = kn.embed_bwd(buf[10:12], ids, 10, out=buf[:10], accumulate=True)
+    assert out.data_ptr() == buf.data_ptr() and out.sum() == 16
