@@ -17,6 +17,7 @@ inline int ok() { return hipGetLastError() == hipSuccess ? MMSUM_OK : MMSUM_ERR_
 template <typename T, int VEC> struct Vec;
 template <> struct Vec<bf16_t, 8> { typedef u32x4_t type; };
 template <> struct Vec<float, 4> { typedef u32x4_t type; };
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 template <> struct Vec<bf16_t, 1> { typedef bf16_t type; };
 template <> struct Vec<float, 1> { typedef float type; };
 
@@ -102,42 +103,59 @@ template <bool FIRST>
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys, const int* __restrict__ pos, int n, int tile,
                                                            int tiles, int V, int64_t pad_id, int shift, const int* __restrict__ hist, uint32_t* __restrict__ okeys,
                                                            int* __restrict__ opos) {
-    __shared__ int cnt[4][256], wbase[4][256], scan[256];
+    __shared__ __attribute__((aligned(16))) int cnt[4][256], wbase[4][256];
+    __shared__ int wsum[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int total = 0, before = 0;
-    for (int t0 = 0; t0 < tiles; t0 += 16) {                       // 16 requests at a time: one by one this chain was most of the kernel
-        int v[16];
-#pragma unroll
-        for (int u = 0; u < 16; ++u) v[u] = t0 + u < tiles ? hist[(t0 + u) * 256 + tid] : 0;
-#pragma unroll
-        for (int u = 0; u < 16; ++u) {
-            before += t0 + u < (int)blockIdx.x ? v[u] : 0;
-            total += v[u];
-        }
-    }
-    scan[tid] = total;
-    __syncthreads();
-    for (int o = 1; o < 256; o <<= 1) {                           // inclusive scan over the digits
-        const int v = tid >= o ? scan[tid - o] : 0;
-        __syncthreads();
-        scan[tid] += v;
-        __syncthreads();
-    }
-    int off = scan[tid] - total + before;                          // this digit's next place
     const long lo = (long)blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n;
+    uint32_t key[4];
+    int from[4];
+    auto load = [&](long base) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const long i = base + wave * 256 + r * 64 + lane;
+            key[r] = i < hi ? (FIRST ? key_of(ids[i], V, pad_id) : keys[i]) : 0u;
+            from[r] = FIRST ? (int)i : i < hi ? pos[i] : 0;
+        }
+    };
+    load(lo);                                                      // under way beside the counts
+    // the digits' totals and what earlier tiles hold of them: a wave sums every fourth tile, four digits a lane, 16 requests at a time (all
+    // tiles after one another by the digit's own thread were most of the kernel)
+    {
+        i32x4_t sum = {0, 0, 0, 0}, front = {0, 0, 0, 0};
+        for (int t0 = wave; t0 < tiles; t0 += 64) {
+            i32x4_t v[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) v[u] = t0 + 4 * u < tiles ? *reinterpret_cast<const i32x4_t*>(hist + (t0 + 4 * u) * 256 + 4 * lane) : i32x4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                if (t0 + 4 * u < (int)blockIdx.x) front += v[u];
+                sum += v[u];
+            }
+        }
+        *reinterpret_cast<i32x4_t*>(&cnt[wave][4 * lane]) = sum;
+        *reinterpret_cast<i32x4_t*>(&wbase[wave][4 * lane]) = front;
+    }
+    __syncthreads();
+    const int total = cnt[0][tid] + cnt[1][tid] + cnt[2][tid] + cnt[3][tid], before = wbase[0][tid] + wbase[1][tid] + wbase[2][tid] + wbase[3][tid];
+    int incl = total;                                              // inclusive scan over the digits
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+        if (w < wave) incl += wsum[w];
+    int off = incl - total + before;                              // this digit's next place
     for (long base = lo; base < hi; base += kSub) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) cnt[w][tid] = 0;
         __syncthreads();
-        uint32_t key[4];
         int rank[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const long i = base + wave * 256 + r * 64 + lane;
-            const bool act = i < hi;
-            key[r] = act ? (FIRST ? key_of(ids[i], V, pad_id) : keys[i]) : 0u;
-            rank[r] = wave_rank(cnt[wave], (key[r] >> shift) & 255, act, lane);
-        }
+        for (int r = 0; r < 4; ++r) rank[r] = wave_rank(cnt[wave], (key[r] >> shift) & 255, base + wave * 256 + r * 64 + lane < hi, lane);
         __syncthreads();
         {
             int o = off;
@@ -147,14 +165,13 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const int64_t* __rest
         }
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const long i = base + wave * 256 + r * 64 + lane;
-            if (i < hi) {
+        for (int r = 0; r < 4; ++r)
+            if (base + wave * 256 + r * 64 + lane < hi) {
                 const int p = wbase[wave][(key[r] >> shift) & 255] + rank[r];
                 okeys[p] = key[r];
-                opos[p] = FIRST ? (int)i : pos[i];
+                opos[p] = from[r];
             }
-        }
+        if (base + kSub < hi) load(base + kSub);
         __syncthreads();
     }
 }
