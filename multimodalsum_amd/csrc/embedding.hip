@@ -228,96 +228,80 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restr
 }
 
 // ---- up to 2048 ids: one launch ----------------------------------------------------------------------------------------------------
-// A workgroup takes neighbouring rows of the table (16 KB of them) at a time.  It reads every id, keeps the positions that name its rows (in batch
-// order), sorts them by row by counting the entries in front of each, and writes its rows whole: sums or zeros.  A row is summed by tpr threads of
-// four columns (VEC = 1: one), its positions in order, eight requested at a time.  Reading all ids in every workgroup is cheap while they
-// are few (1,152 ids: 9 KB a workgroup, once); the launches and waits of the sort are not.
-constexpr int kFew = 2048, kRowsMax = 256;
+// A workgroup takes up to four neighbouring rows of the table (8 KB of them) and clears them at once, which needs no id and keeps the memory
+// busy while they arrive.  It reads every id, lists the positions that name a row of its own in batch order, and writes those rows' sums over
+// the zeros.  A row is summed by tpr threads of four columns (VEC = 1: one), its positions in order, eight requested at a time.  Reading all ids
+// in every workgroup is cheap while they are few (1,152 ids: 9 KB from L2); the launches and waits of a sort are not.  More rows a workgroup
+// put a text's most frequent tokens, neighbours in the table, into one.  Measured (MI355X, bf16, table 50,265 x 1,024, its clearing alone 31 us):
+// 1,152 ids 37 us (16 KB a workgroup 38, 4 KB 48); 2,048 ids 36 us (42, 58).
+constexpr int kFew = 2048, kRowsMax = 4;
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void embed_bwd_few_kernel(const T* __restrict__ dy, long lddy, const int64_t* __restrict__ ids, int n, int V, int D, float scale, int64_t pad_id,
                                                             int accumulate, float* __restrict__ dE, int rows, int tpr_log2) {
-    __shared__ __attribute__((aligned(16))) uint32_t list[kFew];       // (row in the workgroup's range) << 16 | position, in batch order
-    __shared__ uint16_t sorted[kFew];                                  // positions by row
-    __shared__ int start[kRowsMax + 1], wsum[4];
+    constexpr int R = kFew / 256;                                      // rounds of the workgroup over the ids
+    __shared__ uint16_t list[kRowsMax][kFew];                          // positions of a row
+    __shared__ int at[kRowsMax][R * 4], count[kRowsMax];               // of a round and wave: entries of a row, then those in front of them
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int64_t all[kFew / 256];                                           // requested together
-#pragma unroll
-    for (int i = 0; i < kFew / 256; ++i) all[i] = i * 256 + tid < n ? ids[i * 256 + tid] : -1;
-    for (long v0 = (long)blockIdx.x * rows; v0 < V; v0 += (long)gridDim.x * rows) {      // the ids stay in registers from one stretch of rows to the next
+    const long v0 = ((long)blockIdx.y * gridDim.x + blockIdx.x) * rows;
+    if (v0 >= V) return;
     const int here = (int)(V - v0 < rows ? V - v0 : rows);
-    if (!accumulate) {                                                 // zeros first: they need no id and keep the memory busy while the ids arrive
+    int64_t all[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) all[i] = i * 256 + tid < n ? ids[i * 256 + tid] : -1;
+    if (!accumulate) {
         float* const z = dE + v0 * D;
         const long cells = (long)here * D, quads = ((uintptr_t)z & 15) == 0 ? cells / 4 : 0;
-        for (long i = tid; i < quads; i += 256) reinterpret_cast<f32x4_t*>(z)[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (long i = tid; i < quads; i += 256) __builtin_nontemporal_store(f32x4_t{0.f, 0.f, 0.f, 0.f}, reinterpret_cast<f32x4_t*>(z) + i);
         for (long i = quads * 4 + tid; i < cells; i += 256) z[i] = 0.f;
     }
+    int row[R];                                                        // this thread's ids: the row in the workgroup's range, or -1
     bool any = false;
 #pragma unroll
-    for (int i = 0; i < kFew / 256; ++i) any |= all[i] >= v0 && all[i] < v0 + here && all[i] != pad_id;
-    if (!__syncthreads_or(any)) continue;                              // none of the rows is named: most stretches of a large table
+    for (int i = 0; i < R; ++i) {
+        row[i] = all[i] >= v0 && all[i] < v0 + here && all[i] != pad_id ? (int)(all[i] - v0) : -1;
+        any |= row[i] >= 0;
+    }
+    if (!__syncthreads_or(any)) return;                                // none of the rows is named: most stretches of a large table
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                   // the zeros are in front of the sums (other waves' too: barriers follow)
-    start[tid] = 0;
-    int L = 0;
+    int before[R];                                                     // lanes of the wave in front with the same row
 #pragma unroll
-    for (int i = 0; i < kFew / 256; ++i) {
-        const int i0 = i * 256;
-        if (i0 >= n) break;
-        const int64_t id = all[i];
-        const bool mine = id >= v0 && id < v0 + here && id != pad_id;
-        const uint64_t m = __ballot(mine);
-        __syncthreads();                                              // wsum of the last round is read
-        if (lane == 0) wsum[wave] = __popcll(m);
-        __syncthreads();
-        int at = L + __popcll(m & ((1ull << lane) - 1));
+    for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            at += w < wave ? wsum[w] : 0;
-            L += wsum[w];
+        for (int r = 0; r < kRowsMax; ++r) {
+            const uint64_t m = __ballot(row[i] == r);
+            if (row[i] == r) before[i] = __popcll(m & ((1ull << lane) - 1));
+            if (lane == 0) at[r][i * 4 + wave] = __popcll(m);
         }
-        if (mine) list[at] = (uint32_t)(id - v0) << 16 | (uint32_t)(i0 + tid);
-    }
-    if (tid < 4 && L + tid < kFew) list[L + tid] = 0xffffffffu;        // the counting below reads four at a time
     __syncthreads();
-    for (int i = tid; i < L; i += 256) {
-        const uint32_t e = list[i];
-        int rank = 0;                                                  // entries order by (row, position), all different
-        for (int j = 0; j < L; j += 4) {
-            const u32x4_t q = *reinterpret_cast<const u32x4_t*>(list + j);
+    static_assert(kRowsMax * R * 4 <= 256 && R * 4 == 32, "a half wave scans a row's counts");
+    if (tid < kRowsMax * R * 4) {
+        const int r = tid >> 5, j = tid & 31, c = at[r][j];
+        int sum = c;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) rank += q[u] < e;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up(sum, o, 32);
+            sum += j >= o ? v : 0;
         }
-        sorted[rank] = (uint16_t)(e & 0xffffu);
-        atomicAdd(&start[e >> 16], 1);                                 // counts: whole numbers
+        at[r][j] = sum - c;
+        if (j == 31) count[r] = sum;
     }
     __syncthreads();
-    {                                                                  // counts -> starts
-        const int c = start[tid];
-        int s = c;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(s, o);
-            s += lane >= o ? v : 0;
-        }
-        if (lane == 63) wsum[wave] = s;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < 4; ++w) s += w < wave ? wsum[w] : 0;
-        start[tid] = s - c;
-        if (tid == 255) start[256] = s;
-        __syncthreads();
-    }
+    for (int i = 0; i < R; ++i)
+        if (row[i] >= 0) list[row[i]][at[row[i]][i * 4 + wave] + before[i]] = (uint16_t)(i * 256 + tid);
+    __syncthreads();
     constexpr int AHEAD = 8;
     const int tpr = 1 << tpr_log2, groups = 256 >> tpr_log2;
     for (int r = tid >> tpr_log2; r < here; r += groups) {
-        const int lo = start[r], hi = start[r + 1];
-        if (lo == hi) continue;
+        const int hi = count[r];
+        if (hi == 0) continue;
         for (int c = (tid & (tpr - 1)) * VEC; c < D; c += tpr * VEC) {
             float acc[VEC] = {};
-            for (int i0 = lo; i0 < hi; i0 += AHEAD) {
+            for (int i0 = 0; i0 < hi; i0 += AHEAD) {
                 float f[AHEAD][VEC];
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u) {
-                    const T* const src = dy + (long)sorted[i0 + u < hi ? i0 + u : lo] * lddy + c;
+                    const T* const src = dy + (long)list[r][i0 + u < hi ? i0 + u : 0] * lddy + c;
                     if constexpr (VEC == 1) f[u][0] = to_f32(*src);
                     else if constexpr (sizeof(T) == 2) {
                         const bf16x4_t t = *reinterpret_cast<const bf16x4_t*>(src);
@@ -343,17 +327,15 @@ __global__ __launch_bounds__(256) void embed_bwd_few_kernel(const T* __restrict_
             }
         }
     }
-    }
 }
 template <typename T>
 int embed_bwd_few(const void* dy, long lddy, const int64_t* ids, int n, int V, int D, float scale, int64_t pad_id, int accumulate, float* dE, hipStream_t s) {
     const bool vec = D % 4 == 0 && lddy % 4 == 0 && ((uintptr_t)dy & (4 * sizeof(T) - 1)) == 0 && ((uintptr_t)dE & 15) == 0;
-    const long want = 4096 / D;                                        // 16 KB: the rows of a text's most frequent tokens are neighbours, and the tail
-    const int rows = want < 1 ? 1 : want > kRowsMax ? kRowsMax : (int)want, steps = vec ? D / 4 : D;
+    const int rows = D <= 2048 / kRowsMax ? kRowsMax : D <= 1024 ? 2 : 1, steps = vec ? D / 4 : D;
     int lg = 0;
     while ((1 << lg) < steps && lg < 8) ++lg;
-    const long ranges = (V + (long)rows - 1) / rows;
-    const dim3 grid((unsigned)(ranges < 2048 ? ranges : 2048));        // eight a CU
+    const long ranges = (V + (long)rows - 1) / rows, wide = ranges < 1 << 20 ? ranges : 1 << 20;
+    const dim3 grid((unsigned)wide, (unsigned)((ranges + wide - 1) / wide));      // (an axis has up to 2^32 threads)
     if (vec) hipLaunchKernelGGL((embed_bwd_few_kernel<T, 4>), grid, dim3(256), 0, s, (const T*)dy, lddy, ids, n, V, D, scale, pad_id, accumulate, dE, rows, lg);
     else hipLaunchKernelGGL((embed_bwd_few_kernel<T, 1>), grid, dim3(256), 0, s, (const T*)dy, lddy, ids, n, V, D, scale, pad_id, accumulate, dE, rows, lg);
     return ok();

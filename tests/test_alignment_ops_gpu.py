@@ -652,3 +652,25 @@ def test_results_that_overlap_what_is_read_are_refused():
     assert torch.equal(kn.embed_bwd(buf[10:12] + 1, ids, 10, out=buf[:10])[:4, 0].cpu(), torch.tensor([0.0, 1.0, 1.0, 0.0]))
     out = kn.embed_bwd(buf[10:12], ids, 10, out=buf[:10], accumulate=True)
     assert out.data_ptr() == buf.data_ptr() and out.sum() == 16
+
+
+@pytest.mark.parametrize("V,D,n", [(3, 1, 2048), (5, 7, 2047), (4200000, 2, 300), (1100000, 1030, 9), (64, 2050, 1000), (9, 512, 255), (2, 64, 2048)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_embedding_gradient_of_few_ids(V, D, n, accumulate):
+    """Tables of one row a workgroup to millions; one id many times; the last rows of the table."""
+    from multimodalsum_amd import kernels as kn
+    g = torch.Generator().manual_seed(V + n)
+    ids = torch.randint(max(V - 40, 0), V, (n,), generator=g)
+    ids[: n // 3] = V - 1
+    ids[n // 3] = -7
+    ids = ids.cuda()
+    dy = torch.randn(n, D, generator=g).cuda()
+    rows, at = torch.unique(ids[ids >= 0], return_inverse=True)
+    want = torch.zeros(len(rows), D, dtype=torch.float64, device="cuda").index_add_(0, at, 0.5 * dy[ids >= 0].double())
+    mag = torch.zeros_like(want).index_add_(0, at, 0.5 * dy[ids >= 0].double().abs())
+    out = torch.full((V, D), 3.0 if accumulate else float("nan"), device="cuda")
+    got = kn.embed_bwd(dy, ids, V, 0.5, out=out, accumulate=accumulate)
+    base = 3.0 if accumulate else 0.0
+    assert ((got[rows].double() - want - base).abs() <= (mag * (n + 2) + 4 * abs(base)) * H).all()      # at most n additions in a row
+    got.index_fill_(0, rows, base)
+    assert (got == base).all()
