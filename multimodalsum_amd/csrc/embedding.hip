@@ -233,7 +233,8 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restr
 // the zeros.  A row is summed by tpr threads of four columns (VEC = 1: one), its positions in order, eight requested at a time.  Reading all ids
 // in every workgroup is cheap while they are few (1,152 ids: 9 KB from L2); the launches and waits of a sort are not.  More rows a workgroup
 // put a text's most frequent tokens, neighbours in the table, into one.  Measured (MI355X, bf16, table 50,265 x 1,024, its clearing alone 31 us):
-// 1,152 ids 37 us (16 KB a workgroup 38, 4 KB 48); 2,048 ids 36 us (42, 58).
+// 1,152 ids 37 us (16 KB a workgroup 38, 4 KB 48); 2,048 ids 38 us (42, 58).  From there on by sorting (3,000 ids 59 us): with lists of 4,096 fewer
+// workgroups fit a CU, 57 us at 1,152 ids and 66 at 3,000.
 constexpr int kFew = 2048, kRowsMax = 4;
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void embed_bwd_few_kernel(const T* __restrict__ dy, long lddy, const int64_t* __restrict__ ids, int n, int V, int D, float scale, int64_t pad_id,
@@ -342,12 +343,14 @@ int embed_bwd_few(const void* dy, long lddy, const int64_t* ids, int n, int V, i
 }
 
 // ---- sums --------------------------------------------------------------------------------------------------------------------------
-// A wave sums a stretch of 8 or 32 sorted positions over 512 columns (eight a lane).  A token whose positions all lie in the stretch is
+// A wave sums a stretch of 8, 16 or 32 sorted positions over 512 columns (eight a lane).  A token whose positions all lie in the stretch is
 // finished; a token that crosses its ends leaves partial sums: part[stretch][0] of the one that began before it, part[stretch][1] of the
 // one that begins in it and goes on (stretch_join_kernel adds those up).
 constexpr int kCols = 512;
-// positions of a stretch: few of them while that is what keeps the card busy, more where the partial sums' traffic counts
-int stretch_of(long n) { return n <= 8192 ? 8 : 32; }
+// Positions of a stretch: few of them while that is what keeps the card busy, more where the partial sums' traffic and the joins' length count.
+// Whole gradient, bf16, a text's token frequencies into 50,265 x 1,024, us in stretches of 8 | 16 | 32: 3,000 ids 58 | - | 76, 9,216 69 | 73 | 83,
+// 20,000 81 | 77 | 86, 40,000 107 | 99 | 93, 147,456 293 | 200 | 172
+int stretch_of(long n) { return n <= 16384 ? 8 : n <= 32768 ? 16 : 32; }
 
 // eight columns of a lane: VEC: neighbours, else 64 apart
 template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* __restrict__ row, int c, int D, int lane, float (&f)[8]) {

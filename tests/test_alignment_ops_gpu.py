@@ -674,3 +674,22 @@ def test_embedding_gradient_of_few_ids(V, D, n, accumulate):
     assert ((got[rows].double() - want - base).abs() <= (mag * (n + 2) + 4 * abs(base)) * H).all()      # at most n additions in a row
     got.index_fill_(0, rows, base)
     assert (got == base).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [2049, 8193, 16384, 16385, 20001, 32768, 32769, 70000])
+def test_embedding_gradient_of_skewed_ids(n, dt):
+    """A text's frequencies: tokens of one position, of a stretch's length, over hundreds of stretches; padding in front and behind."""
+    from multimodalsum_amd import kernels as kn
+    V, D = 5003, 136
+    g = torch.Generator().manual_seed(n)
+    ids = torch.multinomial(1.0 / torch.arange(1, V + 1).double() ** 1.1, n, True, generator=g).cuda()
+    dy = torch.randn(n, D, generator=g).to(dt).cuda()
+    keep = ids != 1
+    want, mag = torch.zeros(V, D, dtype=torch.float64, device="cuda"), torch.zeros(V, D, dtype=torch.float64, device="cuda")
+    want.index_add_(0, ids[keep], 1.5 * dy[keep].double())
+    mag.index_add_(0, ids[keep], 1.5 * dy[keep].double().abs())
+    got = kn.embed_bwd(dy, ids, V, 1.5, 1)
+    deep = torch.bincount(ids, minlength=V)[:, None].double() + 2       # additions into one sum, the scale
+    assert ((got.double() - want).abs() <= mag * deep * H).all()
+    assert torch.equal(got, kn.embed_bwd(dy, ids, V, 1.5, 1))
