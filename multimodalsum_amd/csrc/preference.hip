@@ -297,25 +297,32 @@ __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs<T> a) {
     }
 }
 
-// out[n] = sum (or mean) of a sequence's counted log-probabilities; one wave a sequence, lanes stride over its tokens
-__device__ __forceinline__ void sequence_sum(const float* __restrict__ logp, const int64_t* __restrict__ labels, int n, int T, int V, int lane, float& sum, int& cnt) {
-    sum = 0.f;
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Sum of a sequence's counted log-probabilities; one wave a sequence, lanes stride over its tokens.  In 64 bits: a margin is the difference of
+// sums of hundreds, whose steps in f32 (2^-16 at 256) are larger than what the tokens' own rounding leaves of it.
+__device__ __forceinline__ void sequence_sum(const float* __restrict__ logp, const int64_t* __restrict__ labels, int n, int T, int V, int lane, double& sum, int& cnt) {
+    sum = 0.0;
     cnt = 0;
     for (int t = lane; t < T; t += 64) {
         const int64_t y = labels[(long)n * T + t];
         if (y >= 0 && y < V) { sum += logp[(long)n * T + t]; ++cnt; }
     }
-    sum = warp_sum(sum);
+    sum = wave_sum(sum);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) cnt += __shfl_xor(cnt, o);
 }
 __global__ __launch_bounds__(256) void sequence_sum_kernel(const float* logp, const int64_t* labels, int N, int T, int V, int average, float* out) {
     const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (n >= N) return;
-    float s;
+    double s;
     int cnt;
     sequence_sum(logp, labels, n, T, V, lane, s, cnt);
-    if (lane == 0) out[n] = average ? s / fmaxf((float)cnt, 1.f) : s;
+    if (lane == 0) out[n] = (float)(average && cnt > 1 ? s / cnt : s);
 }
 
 // log(1 + e^x) without overflow
@@ -334,12 +341,17 @@ struct PairTerms { float sc, sr, h, dc, dr; };
 __device__ __forceinline__ PairTerms pair_terms(const PairArgs& a, int p, int lane) {
     PairTerms t;
     int nc, nr;
-    sequence_sum(a.logp, a.labels, p, a.T, a.V, lane, t.sc, nc);
-    sequence_sum(a.logp, a.labels, a.P + p, a.T, a.V, lane, t.sr, nr);
+    double sc, sr;
+    sequence_sum(a.logp, a.labels, p, a.T, a.V, lane, sc, nc);
+    sequence_sum(a.logp, a.labels, a.P + p, a.T, a.V, lane, sr, nr);
+    if (a.average) {
+        sc /= nc > 1 ? nc : 1;
+        sr /= nr > 1 ? nr : 1;
+    }
     const float ic = a.average ? 1.f / fmaxf((float)nc, 1.f) : 1.f, ir = a.average ? 1.f / fmaxf((float)nr, 1.f) : 1.f;
-    t.sc *= ic;
-    t.sr *= ir;
-    t.h = a.beta * ((t.sc - (a.ref ? a.ref[p] : 0.f)) - (t.sr - (a.ref ? a.ref[a.P + p] : 0.f)));
+    t.sc = (float)sc;
+    t.sr = (float)sr;
+    t.h = (float)((double)a.beta * ((sc - (a.ref ? a.ref[p] : 0.f)) - (sr - (a.ref ? a.ref[a.P + p] : 0.f))));
     const float dh = (a.smoothing - 1.f / (1.f + expf(t.h))) * a.beta / (float)a.P;
     t.dc = dh * ic;
     t.dr = -dh * ir;
@@ -349,9 +361,9 @@ __device__ __forceinline__ float pair_loss_of(const PairArgs& a, float h) {
     return a.smoothing == 0.f ? softplus(-h) : (1.f - a.smoothing) * softplus(-h) + a.smoothing * softplus(h);
 }
 __global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
-    __shared__ float sh[16];
+    __shared__ double sh[16];
     const int lane = threadIdx.x & 63, waves = blockDim.x / 64;
-    float mean = 0.f;
+    double mean = 0.0;
     for (int p = blockIdx.x * waves + (threadIdx.x >> 6); p < a.P; p += gridDim.x * waves) {
         const PairTerms t = pair_terms(a, p, lane);
         const float l = pair_loss_of(a, t.h);
@@ -370,7 +382,7 @@ __global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
         __syncthreads();
         if (threadIdx.x == 0) {
             for (int w = 1; w < 16; ++w) mean += sh[w];
-            *a.loss = mean / (float)a.P;
+            *a.loss = (float)(mean / a.P);
         }
     }
 }
@@ -445,24 +457,29 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(const T* logits, long 
 
 // the mean over the pairs in the order of a single workgroup's pair_kernel
 __global__ void pair_mean_kernel(const float* __restrict__ pair_loss, int P, float* __restrict__ loss) {
-    __shared__ float sh[16];
-    float mean = 0.f;
+    __shared__ double sh[16];
+    double mean = 0.0;
     for (int p = threadIdx.x; p < P; p += 16) mean += pair_loss[p];
     sh[threadIdx.x] = mean;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 16; ++w) mean += sh[w];
-        *loss = mean / (float)P;
+        *loss = (float)(mean / P);
     }
 }
 
-// out[j] = scale * sum of x[j * n .. (j + 1) * n)
-__global__ __launch_bounds__(1024) void rows_mean_kernel(const float* __restrict__ x, long n, float scale, float* __restrict__ out) {
-    __shared__ float sh[16];
-    float s = 0.f;
+// out[j] = sum of x[j * n .. (j + 1) * n) / per, in 64 bits (terms of either sign may leave little)
+__global__ __launch_bounds__(1024) void rows_mean_kernel(const float* __restrict__ x, long n, long per, float* __restrict__ out) {
+    __shared__ double sh[16];
+    double s = 0.0;
     for (long i = threadIdx.x; i < n; i += 1024) s += x[(long)blockIdx.x * n + i];
-    s = block_sum<1024>(s, sh);
-    if (threadIdx.x == 0) out[blockIdx.x] = s * scale;
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) s += sh[w];
+        out[blockIdx.x] = (float)(s / per);
+    }
 }
 
 // counts[i]: counted tokens of sequence i (seq) or of the i-th of kCountParts equal stretches of the batch
@@ -587,7 +604,7 @@ extern "C" int mmsum_preference_pairs(const float* logp, const int64_t* labels, 
     } else {
         a.loss = nullptr;
         hipLaunchKernelGGL(pair_kernel, dim3((P + 3) / 4), dim3(256), 0, s, a);
-        hipLaunchKernelGGL(rows_mean_kernel, dim3(1), dim3(1024), 0, s, pair_loss, (long)P, 1.f / (float)P, loss);
+        hipLaunchKernelGGL(rows_mean_kernel, dim3(1), dim3(1024), 0, s, pair_loss, (long)P, (long)P, loss);
     }
     return ok();
 }
@@ -616,7 +633,7 @@ extern "C" int mmsum_preference_loss(int dtype, const void* logits, long ld, con
     int rc = dtype == MMSUM_BF16 ? preference_rows<bf16_t>(logits, ld, dlogits, ldd, W, stats, pairs, s) : preference_rows<float>(logits, ld, dlogits, ldd, W, stats, pairs, s);
     if (rc != MMSUM_OK) return rc;
     if (single_pairs(P, T)) hipLaunchKernelGGL(pair_mean_kernel, dim3(1), dim3(16), 0, s, pair_loss, P, loss);
-    else hipLaunchKernelGGL(rows_mean_kernel, dim3(1), dim3(1024), 0, s, pair_loss, (long)P, 1.f / (float)P, loss);
+    else hipLaunchKernelGGL(rows_mean_kernel, dim3(1), dim3(1024), 0, s, pair_loss, (long)P, (long)P, loss);
     return ok();
 }
 
@@ -650,7 +667,7 @@ extern "C" int mmsum_policy_terms(const float* logp, const int64_t* labels, cons
     if (rc == MMSUM_OK) rc = launch_counts(labels, N, T, V, seq_mean, const_cast<int*>(p.counts), s);
     if (rc != MMSUM_OK) return rc;
     hipLaunchKernelGGL(policy_terms_kernel, dim3((unsigned)((R + 255) / 256)), dim3(256), 0, s, logp, labels, V, p, coef);
-    hipLaunchKernelGGL(rows_mean_kernel, dim3(3), dim3(1024), 0, s, p.terms, R, 1.f, out);
+    hipLaunchKernelGGL(rows_mean_kernel, dim3(3), dim3(1024), 0, s, p.terms, R, 1L, out);
     return ok();
 }
 
@@ -677,6 +694,6 @@ extern "C" int mmsum_policy_loss(int dtype, const void* logits, long ld, const i
         rc = launch_rows<float, true>(a, R, s);
     }
     if (rc != MMSUM_OK) return rc;
-    hipLaunchKernelGGL(rows_mean_kernel, dim3(3), dim3(1024), 0, s, p.terms, (long)R, 1.f, out);
+    hipLaunchKernelGGL(rows_mean_kernel, dim3(3), dim3(1024), 0, s, p.terms, (long)R, 1L, out);
     return ok();
 }

@@ -693,3 +693,42 @@ def test_embedding_gradient_of_skewed_ids(n, dt):
     deep = torch.bincount(ids, minlength=V)[:, None].double() + 2       # additions into one sum, the scale
     assert ((got.double() - want).abs() <= mag * deep * H).all()
     assert torch.equal(got, kn.embed_bwd(dy, ids, V, 1.5, 1))
+
+
+@pytest.mark.parametrize("average", [False, True])
+@pytest.mark.parametrize("P,T", [(1, 156), (3, 700), (40, 64), (300, 256), (1, 5000)])
+def test_margins_of_long_sequences_keep_their_digits(P, T, average):
+    """Sums of hundreds whose difference is small: the margin is the 64-bit sum of the tokens' values rounded once, by both forms of the loss."""
+    from multimodalsum_amd import kernels as kn
+    g = torch.Generator().manual_seed(P * T)
+    V = 11
+    labels = torch.randint(0, V, (2 * P, T), generator=g)
+    labels[:, -3:] = -100
+    logp = -torch.rand(2 * P, T, generator=g) * 4
+    ref = logp.masked_fill(labels < 0, 0.0).sum(1) / (T - 3 if average else 1) + torch.randn(2 * P, generator=g) * 1e-3
+    keep = (labels >= 0).double()
+    S = (logp.double() * keep).sum(1) / (T - 3 if average else 1)
+    r = S - ref.double()
+    h = 0.5 * (r[:P] - r[P:])
+    loss, margins, seq, coef = kn.preference_pairs(logp.cuda(), labels.cuda(), ref.cuda(), V, 0.5, 0.1, average)
+    assert ((margins.cpu().double() - h).abs() <= 2 * H * h.abs() + 2.0 ** -40).all()       # 64-bit sums of up to 5,000 values below 4: 2^-53 of them a step
+    assert ((seq.cpu().double() - S).abs() <= 2 * H * S.abs()).all()
+    x = torch.randn(2 * P, T, V, generator=g).cuda()
+    lp = kn.token_logprob(x, labels.cuda())
+    want = kn.preference_pairs(lp, labels.cuda(), ref.cuda(), V, 0.5, 0.1, average)
+    got = kn.preference_loss(x, labels.cuda(), ref.cuda(), 0.5, 0.1, average)
+    for a, b in zip(want[:3], got[:3]):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("N,T", [(4, 64), (16, 512), (64, 1024)])
+def test_policy_loss_of_terms_that_cancel(N, T):
+    from multimodalsum_amd import kernels as kn
+    g = torch.Generator().manual_seed(N)
+    adv = torch.randn(N, T, generator=g)
+    adv -= adv.mean()
+    logp = -torch.rand(N, T, generator=g)
+    out, coef = kn.policy_terms(logp.cuda(), torch.zeros(N, T, dtype=torch.int64).cuda(), logp.cuda(), adv.cuda(), None, 5, 0.2, 0.2, 0.0, "token")
+    want = -adv.double().mean()                                     # ratios of one, weights a power of two: every term is exact
+    assert abs(out[0].item() - want) <= 2 * H * abs(want) + 2.0 ** -50
+    assert torch.equal(coef.cpu(), -adv / (N * T))
