@@ -195,8 +195,8 @@ template <typename T, bool WHOLE> __device__ __forceinline__ void store_cols(T* 
 //            64 MFMAs on Y | reads of stage s + 1's first 64 k (X) | DMA: B of stage s + 2
 // The weights ride as the MFMA's A operand, so that a lane's four results are neighbouring columns; within 32 weight rows LDS row
 // 16 j + 4 g + e holds weight row 8 g + 4 j + e, and the two MFMAs of a pair leave a lane eight neighbouring columns: a 16-byte store.
-// Measured (MI355X): 8192^3 393 us = 2,796 TOP/s (the library's integer product 2,107); 36,864 x 4,096 x 1,024 170 us, with GELU 213 us: a
-// tile's epilogue is 65,536 values of 6 (25 with GELU, counting the transcendentals' four) issue slots on 256 lanes beside 11 us of main loop.
+// Measured (MI355X): 8192^3 381 us = 2,890 TOP/s (the library's integer product 2,107); 36,864 x 4,096 x 1,024 184 us, with GELU 234: a
+// tile's epilogue is 65,536 values of 6 (25 with GELU, counting the transcendentals' four) issue slots on 256 lanes beside 12 us of main loop.
 constexpr int kStageBytes = 256 * 128;
 template <typename T, bool GELU>
 __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(I8Args p) {
@@ -627,9 +627,9 @@ int launch_ring(const I8Args& p, hipStream_t s) {
 template <typename T, bool GELU>
 int launch_product(const I8Args& p, hipStream_t s) {
     if (p.M <= 64) {
-        // Workgroups of 64 columns where there are still two of them for every CU: they read the activations less often (32 x 50,265 x 1,024:
-        // 16.1 us, in 16 columns 19); below that 16 columns fill more CUs
-        const bool wide = p.N >= 32768;
+        // Workgroups of 64 columns read the activations less often, of 16 columns fill more CUs (us, 16 | 64 columns, K = 1,024): N = 8,192: 1 row 3.4 | 4.2,
+        // 32 rows 4.9 | 5.9; 16,384: 1 row 4.3 | 5.0, 16 rows 5.5 | 5.7, 32 rows 7.8 | 6.1; 50,265: 1 row 10.8 | 10.8, 32 rows 21.5 | 15.9
+        const bool wide = p.N >= (p.M <= 16 ? 32768 : 16384);
         if (p.M <= 16) return wide ? launch_few<T, GELU, 1, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 1, 1, false, float>(p, nullptr, 0, 0, s);
         if (p.M <= 32) return wide ? launch_few<T, GELU, 2, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 2, 1, false, float>(p, nullptr, 0, 0, s);
         return wide ? launch_few<T, GELU, 4, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 4, 1, false, float>(p, nullptr, 0, 0, s);
@@ -655,11 +655,12 @@ int launch_product(const I8Args& p, hipStream_t s) {
     return ok();
 }
 
-// Quantisation and product.  In one launch for up to 16 rows of up to 4,096 values and few columns: there the launch costs more than every
-// workgroup's quantising all rows.
+// Quantisation and product.  In one launch for up to 8,192 values: there every workgroup's quantising all rows costs no more than the launch (us,
+// two | one, N = 1,024): 1 x 1,024 4.8 | 3.5, 1 x 4,096 9.2 | 7.6, 8 x 1,024 5.2 | 5.0, 16 x 1,024 5.4 | 7.7, 8 x 4,096 10.0 | 12.9; 8 x 1,024 into 16,384
+// columns 7.4 | 7.8, into 50,265 15.9 | 19.4.
 template <typename T, bool GELU>
 int launch_linear(int dtype, const void* x, long ldx, I8Args p, int Kx, hipStream_t s) {
-    if (p.M <= 16 && p.K <= 4096 && p.N <= 4096) {
+    if (p.M <= 16 && (long)p.M * p.K <= 8192 && p.N <= 16384) {
         if (dtype == MMSUM_BF16) return launch_few<T, GELU, 1, 1, true, bf16_t>(p, static_cast<const bf16_t*>(x), ldx, Kx, s);
         return launch_few<T, GELU, 1, 1, true, float>(p, static_cast<const float*>(x), ldx, Kx, s);
     }

@@ -7,10 +7,10 @@
 //
 // Bound: HBM.  The policy loss knows c as soon as the row's own log p is known, so its kernel reads the logits once and writes the
 // gradient once, the row waiting in registers in between.  The preference loss needs the sums over both summaries of a pair first:
-// statistics (read), gradient (read, write), every workgroup of the second taking its pair's sums itself.
-// Measured (MI355X, 50,265 bf16 logits): scoring 72 x 141 rows 177 us (4.8 TB/s), policy loss 72 x 128 rows 315 us (5.4 TB/s), preference loss
-// of 36 pairs x 128 rows 419 us (4.1 TB/s of what has to move, 5.9 with the second reading).
-// Everything is summed in f32, in an order that depends on the sizes alone.
+// statistics (read), the pairs' sums and factors, gradient (read, write).
+// Measured (MI355X, 50,265 bf16 logits): scoring 72 x 141 rows 177 us (4.8 TB/s), policy loss 72 x 128 rows 309 us (5.5 TB/s), preference loss
+// of 36 pairs x 128 rows 416 us (4.1 TB/s of what has to move, 5.9 with the second reading).
+// A row is summed in f32, sequences and means in 64 bits, in an order that depends on the sizes alone.
 #include "mmsum_device.h"
 #include "mmsum_kernels.h"
 
@@ -389,41 +389,18 @@ __global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
 
 // Gradient of the logits from the row statistics: coef[row / rows_per_coef] (* *alpha) ([v == y] - exp(x - m) / s).
 // A row whose factor is zero is not read.
-// PAIRS: the preference loss's c; every workgroup takes its pair's sums itself (2 T numbers from the caches, under the latency of its first
-// logits), the one on the pair's first row leaves the pair's results.
-template <typename T, bool PAIRS>
+template <typename T>
 __global__ __launch_bounds__(256) void logprob_bwd_kernel(const T* logits, long ld, const int64_t* __restrict__ labels, const float* __restrict__ stats,
                                                           const float* __restrict__ coef, int rows_per_coef, const float* __restrict__ alpha, T* dlogits,
-                                                          long ldd, int W, int V, PairArgs pairs) {
+                                                          long ldd, int W, int V) {
     constexpr int NT = 256, U = 4;
     const int tid = threadIdx.x, row = gridDim.x - 1 - blockIdx.x;
     const int64_t y = labels[row];
     T* const d = dlogits + (long)row * ldd;
     const T* x = logits + (long)row * ld;
     const bool counted = y >= 0 && y < V;
-    u32x4_t reg[U];
-    auto request = [&](long c0i) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long c = c0i + (long)u * NT * kPer<T>;
-            if (c < V) reg[u] = load_chunk<T, true>(x, (int)c, V);
-        }
-    };
     float c0 = 0.f;
-    if constexpr (PAIRS) {
-        if (counted) request((long)tid * kPer<T>);
-        const int seq = row / pairs.T, p = seq < pairs.P ? seq : seq - pairs.P;
-        if (counted || row == p * pairs.T) {
-            const PairTerms t = pair_terms(pairs, p, tid & 63);
-            if (counted) c0 = seq < pairs.P ? t.dc : t.dr;
-            if (row == p * pairs.T && tid == 0) {
-                pairs.seq[p] = t.sc;
-                pairs.seq[pairs.P + p] = t.sr;
-                pairs.margins[p] = t.h;
-                pairs.pair_loss[p] = pair_loss_of(pairs, t.h);
-            }
-        }
-    } else if (counted) {
+    if (counted) {
         c0 = coef[row / rows_per_coef];
         if (alpha != nullptr) c0 *= *alpha;
     }
@@ -434,7 +411,12 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(const T* logits, long 
     }
     const float m = stats[2 * (long)row], cs = -c0 / stats[2 * (long)row + 1];
     for (long c0i = (long)tid * kPer<T>; c0i < V; c0i += (long)U * NT * kPer<T>) {
-        if (!PAIRS || c0i != (long)tid * kPer<T>) request(c0i);
+        u32x4_t reg[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long c = c0i + (long)u * NT * kPer<T>;
+            if (c < V) reg[u] = load_chunk<T, true>(x, (int)c, V);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long c = c0i + (long)u * NT * kPer<T>;
@@ -453,19 +435,6 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(const T* logits, long 
         }
     }
     zero_cols<T, NT>(d, V, W);
-}
-
-// the mean over the pairs in the order of a single workgroup's pair_kernel
-__global__ void pair_mean_kernel(const float* __restrict__ pair_loss, int P, float* __restrict__ loss) {
-    __shared__ double sh[16];
-    double mean = 0.0;
-    for (int p = threadIdx.x; p < P; p += 16) mean += pair_loss[p];
-    sh[threadIdx.x] = mean;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) mean += sh[w];
-        *loss = (float)(mean / P);
-    }
 }
 
 // out[j] = sum of x[j * n .. (j + 1) * n) / per, in 64 bits (terms of either sign may leave little)
@@ -514,7 +483,8 @@ __global__ __launch_bounds__(256) void policy_terms_kernel(const float* __restri
 }
 
 // Threads and chunks of a row: the smallest workgroup whose registers hold it, so that short rows keep many rows in flight on a CU
-// and a BART row (50,265 bf16 logits: 512 threads x 13 chunks, 52 registers; f32: 1024 x 13) is resident as a whole.
+// and a BART row (50,265 bf16 logits: 512 threads x 13 chunks, 52 registers; f32: 1024 x 13) is resident as a whole.  Scoring | policy loss, us, against
+// the next larger workgroup: 8,192 x 2,000 8 | 21 (35 | 53), 4,096 x 16,000 24 | 54 (55 | 175), 4,096 x 50,265 88 | 177 (207 | 289).
 template <typename T, bool POLICY>
 int launch_rows(const RowArgs<T>& a, int blocks, hipStream_t s) {
     const long chunks = ((long)a.V + kPer<T> - 1) / kPer<T>;
@@ -539,28 +509,10 @@ RowArgs<T> row_args(const void* logits, long ld, const int64_t* labels, int V, f
 template <typename T>
 int launch_bwd(const void* logits, long ld, const int64_t* labels, const float* stats, const float* coef, int rows_per_coef, const float* alpha, void* dlogits,
                long ldd, int W, int V, int R, hipStream_t s) {
-    hipLaunchKernelGGL((logprob_bwd_kernel<T, false>), dim3(R), dim3(256), 0, s, static_cast<const T*>(logits), ld, labels, stats, coef, rows_per_coef, alpha,
-                       static_cast<T*>(dlogits), ldd, W, V, PairArgs{});
+    hipLaunchKernelGGL((logprob_bwd_kernel<T>), dim3(R), dim3(256), 0, s, static_cast<const T*>(logits), ld, labels, stats, coef, rows_per_coef, alpha,
+                       static_cast<T*>(dlogits), ldd, W, V);
     return ok();
 }
-
-// Statistics, then the gradient from the last row to the first: the rows read last are still in the 256 MB memory-side cache.
-template <typename T>
-int preference_rows(const void* logits, long ld, void* dlogits, long ldd, int W, float* stats, const PairArgs& pairs, hipStream_t s) {
-    RowArgs<T> a = row_args<T>(logits, ld, pairs.labels, pairs.V, const_cast<float*>(pairs.logp), stats);
-    const int R = 2 * pairs.P * pairs.T;
-    // all rows but the last 400 MB are read past the caches, which leaves those to the second reading (36 pairs of 128 x 50,265: 428 -> 419 us;
-    // pairs in separate launches of 110 .. 480 MB: 487 .. 411 us)
-    const long keep = (400L << 20) / (ld * (long)sizeof(T));
-    a.past = keep < R ? R - (int)keep : 0;
-    const int rc = launch_rows<T, false>(a, R, s);
-    if (rc != MMSUM_OK) return rc;
-    hipLaunchKernelGGL((logprob_bwd_kernel<T, true>), dim3(R), dim3(256), 0, s, a.logits, ld, pairs.labels, stats, nullptr, 1, nullptr, static_cast<T*>(dlogits), ldd, W, pairs.V,
-                       pairs);
-    return ok();
-}
-
-bool single_pairs(int P, int T) { return (long)P * T <= 32768; }      // a single workgroup is done before a second launch would begin
 
 long count_slots(int N, int seq_mean) { return seq_mean ? N : kCountParts; }
 int launch_counts(const int64_t* labels, int N, int T, int V, int seq_mean, int* counts, hipStream_t s) {
@@ -599,7 +551,8 @@ extern "C" int mmsum_preference_pairs(const float* logp, const int64_t* labels, 
     if (P <= 0 || T <= 0 || V <= 0 || 2L * P * T > 0x7fffffffL || !(smoothing >= 0.f && smoothing <= 1.f)) return MMSUM_ERR_BAD_SHAPE;
     hipStream_t s = (hipStream_t)stream;
     PairArgs a = {logp, labels, ref, P, T, V, average, beta, smoothing, seq, margins, pair_loss, coef, loss};
-    if (single_pairs(P, T)) {
+    // one workgroup, a wave a pair, with the mean (us, this | two launches: 1 x 33 3.2 | 4.7, 16 x 128 4.5 | 5.4; in turns 36 x 32 6.4 | 5.2, 128 x 256 28 | 6.5)
+    if (P <= 16) {
         hipLaunchKernelGGL(pair_kernel, dim3(1), dim3(1024), 0, s, a);
     } else {
         a.loss = nullptr;
@@ -623,26 +576,28 @@ extern "C" int mmsum_preference_loss(int dtype, const void* logits, long ld, con
     float* const pair_loss = stats + 2L * R;
     float* const coef = pair_loss + P;
     hipStream_t s = (hipStream_t)stream;
-    if (T > 1024) {                                                // long sequences: the pairs once, not in every row's workgroup
-        int rc = mmsum_token_logprob(dtype, logits, ld, labels, logp, stats, R, V, stream);
+    // Statistics, the pairs, then the gradient from the last row to the first.  All rows but the last 400 MB are read past the caches, which leaves
+    // those to the second reading: the memory-side cache holds 256 MB (36 pairs of 128 x 50,265: 428 -> 419 us).  (Every row's workgroup of the
+    // gradient taking its pair's sums itself in place of the pairs' launch: 4 x 128 x 1,009 equal, 36 x 128 x 1,009 30 -> 52 us.)
+    const auto run = [&](auto of_type) {
+        typedef decltype(of_type) T_;
+        RowArgs<T_> a = row_args<T_>(logits, ld, labels, V, logp, stats);
+        const long keep = (400L << 20) / (ld * (long)sizeof(T_));
+        a.past = keep < R ? R - (int)keep : 0;
+        int rc = launch_rows<T_, false>(a, R, s);
         if (rc == MMSUM_OK) rc = mmsum_preference_pairs(logp, labels, ref, P, T, V, beta, smoothing, average, seq, margins, pair_loss, coef, loss, stream);
-        if (rc == MMSUM_OK) rc = mmsum_token_logprob_bwd(dtype, logits, ld, labels, stats, coef, T, nullptr, dlogits, ldd, W, R, V, stream);
-        return rc;
-    }
-    const PairArgs pairs = {logp, labels, ref, P, T, V, average, beta, smoothing, seq, margins, pair_loss, coef, loss};
-    int rc = dtype == MMSUM_BF16 ? preference_rows<bf16_t>(logits, ld, dlogits, ldd, W, stats, pairs, s) : preference_rows<float>(logits, ld, dlogits, ldd, W, stats, pairs, s);
-    if (rc != MMSUM_OK) return rc;
-    if (single_pairs(P, T)) hipLaunchKernelGGL(pair_mean_kernel, dim3(1), dim3(16), 0, s, pair_loss, P, loss);
-    else hipLaunchKernelGGL(rows_mean_kernel, dim3(1), dim3(1024), 0, s, pair_loss, (long)P, (long)P, loss);
-    return ok();
+        return rc == MMSUM_OK ? launch_bwd<T_>(logits, ld, labels, stats, coef, T, nullptr, dlogits, ldd, W, V, R, s) : rc;
+    };
+    return dtype == MMSUM_BF16 ? run(bf16_t{}) : run(float{});
 }
 
 // workspace: terms [3][NT], counts
 extern "C" long mmsum_policy_workspace(int N, int T) {
     return N <= 0 || T <= 0 ? 0 : 3L * N * T * (long)sizeof(float) + (long)(N > kCountParts ? N : kCountParts) * (long)sizeof(int);
 }
-// Rows of the logits count their sequence (or the small batch) themselves, under the latency of the row: a launch less
-static bool rows_count(int N, int T, int seq_mean) { return seq_mean ? T <= 2048 : (long)N * T <= 1024; }
+// Rows of the logits count their sequence (or the small batch) themselves, under the latency of the row: a launch less (us, V = 1,009, this | a launch:
+// token mean 3 x 57 7.2 | 9.1, 8 x 128 9.7 | 9.9, 16 x 128 13.1 | 11.4; sequence mean 4 x 128 7.4 | 8.8, 4 x 1,024 14.1 | 14.0, 4 x 4,096 56 | 31)
+static bool rows_count(int N, int T, int seq_mean) { return seq_mean ? T <= 1024 : (long)N * T <= 1024; }
 static int policy_setup(PolicyArgs& p, const int64_t* labels, int V, const float* old_logp, const float* ref_logp, const float* adv, int adv_per_token, int N, int T, float clip_low,
                         float clip_high, float kl_coef, int seq_mean, void* workspace) {
     if (!(clip_low >= 0.f) || !(clip_high >= 0.f) || kl_coef != kl_coef) return MMSUM_ERR_BAD_SHAPE;
