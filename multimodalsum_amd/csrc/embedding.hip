@@ -6,6 +6,7 @@
 // summed by many waves at once.
 // Ids outside 0 .. V-1 read as zero rows and leave no gradient, and so does pad_id in the gradient.
 // Bound: HBM (dy once, dE once).
+#include "entry_checks.h"
 #include "mmsum_device.h"
 #include "mmsum_kernels.h"
 
@@ -607,6 +608,7 @@ __global__ __launch_bounds__(256) void zero_kernel(float* __restrict__ p, long n
 
 extern "C" int mmsum_embed_fwd(int dtype, const int64_t* ids, const void* E, long lde, void* y, long ldy, long n, int V, int D, float scale, void* stream) {
     if (n <= 0 || V <= 0 || D <= 0 || lde < D || ldy < D) return MMSUM_ERR_BAD_SHAPE;
+    if (any_null(ids, E, y)) return MMSUM_ERR_BAD_ALIGN;
     if (dtype == MMSUM_BF16) return ((uintptr_t)E | (uintptr_t)y) & 1 ? MMSUM_ERR_BAD_ALIGN : embed_fwd_t<bf16_t>(ids, E, lde, y, ldy, n, V, D, scale, (hipStream_t)stream);
     if (dtype == MMSUM_F32) return ((uintptr_t)E | (uintptr_t)y) & 3 ? MMSUM_ERR_BAD_ALIGN : embed_fwd_t<float>(ids, E, lde, y, ldy, n, V, D, scale, (hipStream_t)stream);
     return MMSUM_ERR_BAD_DTYPE;
@@ -621,7 +623,7 @@ extern "C" int mmsum_embed_bwd(int dtype, const void* dy, long lddy, const int64
     if (n < 0 || n > 0x3fffffffL || V <= 0 || V > 0x7ffffff0 || D <= 0 || lddy < D) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
     if (n > kFew && workspace == nullptr) return MMSUM_ERR_WORKSPACE;
-    if (((uintptr_t)workspace & 15) || ((uintptr_t)dE & 3) || ((uintptr_t)dy & (dtype == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
+    if (dE == nullptr || (n > 0 && any_null(dy, ids)) || ((uintptr_t)workspace & 15) || ((uintptr_t)dE & 3) || ((uintptr_t)dy & (dtype == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
     hipStream_t s = (hipStream_t)stream;
     if (n == 0) {
         if (!accumulate) hipLaunchKernelGGL(zero_kernel, dim3(1024), dim3(256), 0, s, dE, (long)V * D);

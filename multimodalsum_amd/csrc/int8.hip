@@ -4,6 +4,7 @@
 // The sum is an integer and exact (127^2 K < 2^31 bounds K at 131,072); it becomes f32 (2^-24) before the two scales.  A row whose values
 // are not all finite has a scale that is not finite and gives NaN; a row of zeros gives the bias.
 // Bound: the integer matrix cores (twice the bf16 rate) for many rows, HBM (the weights once, half the bf16 bytes) for few.
+#include "entry_checks.h"
 #include "gemm_common.h"
 #include <type_traits>
 
@@ -675,7 +676,7 @@ int launch_linear(int dtype, const void* x, long ldx, I8Args p, int Kx, hipStrea
 extern "C" int mmsum_quantize_i8(int dtype, const void* x, long ldx, int M, int K, void* q, long ldq, float* scale, void* stream) {
     if (M <= 0 || K <= 0 || ldx < K || ldq < K || ldq % 128 || ldq > 0x7fffffc0L) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
-    if (((uintptr_t)q & 15) || ((uintptr_t)x & (dtype == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
+    if (any_null(x, q, scale) || ((uintptr_t)q & 15) || ((uintptr_t)x & (dtype == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == MMSUM_BF16) return launch_quantize<bf16_t>(x, ldx, M, K, q, ldq, scale, s);
     return launch_quantize<float>(x, ldx, M, K, q, ldq, scale, s);
@@ -685,7 +686,7 @@ extern "C" int mmsum_gemm_i8(const void* qx, long ldx, const float* sx, const vo
                              int M, int N, int K, int gelu, void* stream) {
     if (M <= 0 || N <= 0 || K <= 0 || K % 128 || K > 131072 || ldx < K || ldw < K || ldx % 16 || ldw % 16 || ldx > 0x3fffff || ldw > 0x3fffff || ldy < N) return MMSUM_ERR_BAD_SHAPE;
     if (dtype_out != MMSUM_BF16 && dtype_out != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
-    if ((((uintptr_t)qx | (uintptr_t)qw) & 15) || ((uintptr_t)y & (dtype_out == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
+    if (any_null(qx, sx, qw, sw, y) || (((uintptr_t)qx | (uintptr_t)qw) & 15) || ((uintptr_t)y & (dtype_out == MMSUM_BF16 ? 1 : 3))) return MMSUM_ERR_BAD_ALIGN;
     I8Args p = {static_cast<const int8_t*>(qx), ldx, sx, static_cast<const int8_t*>(qw), ldw, sw, bias, y, ldy, M, N, K};
     hipStream_t s = (hipStream_t)stream;
     if (dtype_out == MMSUM_BF16) return gelu ? launch_product<bf16_t, true>(p, s) : launch_product<bf16_t, false>(p, s);
@@ -698,7 +699,7 @@ extern "C" int mmsum_linear_i8(int dtype, const void* x, long ldx, const void* q
     if (M <= 0 || N <= 0 || K <= 0 || K > 131072 || ldx < K || ldw < (K + 127L) / 128 * 128 || ldw % 16 || ldw > 0x3fffff || ldy < N) return MMSUM_ERR_BAD_SHAPE;
     if ((dtype != MMSUM_BF16 && dtype != MMSUM_F32) || (dtype_out != MMSUM_BF16 && dtype_out != MMSUM_F32)) return MMSUM_ERR_BAD_DTYPE;
     if (workspace == nullptr) return MMSUM_ERR_WORKSPACE;
-    if (((uintptr_t)x & (dtype == MMSUM_BF16 ? 1 : 3)) || (((uintptr_t)qw | (uintptr_t)workspace) & 15) || ((uintptr_t)y & (dtype_out == MMSUM_BF16 ? 1 : 3)))
+    if (any_null(x, qw, sw, y) || ((uintptr_t)x & (dtype == MMSUM_BF16 ? 1 : 3)) || (((uintptr_t)qw | (uintptr_t)workspace) & 15) || ((uintptr_t)y & (dtype_out == MMSUM_BF16 ? 1 : 3)))
         return MMSUM_ERR_BAD_ALIGN;
     const int Kp = (K + 127) / 128 * 128;
     int8_t* const q = static_cast<int8_t*>(workspace);

@@ -11,6 +11,7 @@
 // Measured (MI355X, 50,265 bf16 logits): scoring 72 x 141 rows 177 us (4.8 TB/s), policy loss 72 x 128 rows 309 us (5.5 TB/s), preference loss
 // of 36 pairs x 128 rows 416 us (4.1 TB/s of what has to move, 5.9 with the second reading).
 // A row is summed in f32, sequences and means in 64 bits, in an order that depends on the sizes alone.
+#include "entry_checks.h"
 #include "mmsum_device.h"
 #include "mmsum_kernels.h"
 
@@ -526,7 +527,7 @@ int launch_counts(const int64_t* labels, int N, int T, int V, int seq_mean, int*
 extern "C" int mmsum_token_logprob(int dtype, const void* logits, long ld, const int64_t* labels, float* logp, float* stats, int R, int V, void* stream) {
     if (bad_rows(R, V, ld)) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
-    if (bad_align(dtype, logits)) return MMSUM_ERR_BAD_ALIGN;
+    if (any_null(logits, labels, logp) || bad_align(dtype, logits)) return MMSUM_ERR_BAD_ALIGN;
     if (dtype == MMSUM_BF16) return launch_rows<bf16_t, false>(row_args<bf16_t>(logits, ld, labels, V, logp, stats), R, (hipStream_t)stream);
     return launch_rows<float, false>(row_args<float>(logits, ld, labels, V, logp, stats), R, (hipStream_t)stream);
 }
@@ -535,13 +536,14 @@ extern "C" int mmsum_token_logprob_bwd(int dtype, const void* logits, long ld, c
                                        const float* alpha, void* dlogits, long ldd, int W, int R, int V, void* stream) {
     if (bad_rows(R, V, ld) || rows_per_coef <= 0 || W < V || W > 0x7fffffff - 16384 || ldd < W) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
-    if (bad_align(dtype, logits) || bad_align(dtype, dlogits)) return MMSUM_ERR_BAD_ALIGN;
+    if (any_null(logits, labels, stats, coef, dlogits) || bad_align(dtype, logits) || bad_align(dtype, dlogits)) return MMSUM_ERR_BAD_ALIGN;
     if (dtype == MMSUM_BF16) return launch_bwd<bf16_t>(logits, ld, labels, stats, coef, rows_per_coef, alpha, dlogits, ldd, W, V, R, (hipStream_t)stream);
     return launch_bwd<float>(logits, ld, labels, stats, coef, rows_per_coef, alpha, dlogits, ldd, W, V, R, (hipStream_t)stream);
 }
 
 extern "C" int mmsum_sequence_logprob(const float* logp, const int64_t* labels, int N, int T, int V, int average, float* out, void* stream) {
     if (N <= 0 || T <= 0 || V <= 0 || (long)N * T > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    if (any_null(logp, labels, out)) return MMSUM_ERR_BAD_ALIGN;
     hipLaunchKernelGGL(sequence_sum_kernel, dim3((N + 3) / 4), dim3(256), 0, (hipStream_t)stream, logp, labels, N, T, V, average, out);
     return ok();
 }
@@ -549,6 +551,7 @@ extern "C" int mmsum_sequence_logprob(const float* logp, const int64_t* labels, 
 extern "C" int mmsum_preference_pairs(const float* logp, const int64_t* labels, const float* ref, int P, int T, int V, float beta, float smoothing, int average,
                                       float* seq, float* margins, float* pair_loss, float* coef, float* loss, void* stream) {
     if (P <= 0 || T <= 0 || V <= 0 || 2L * P * T > 0x7fffffffL || !(smoothing >= 0.f && smoothing <= 1.f)) return MMSUM_ERR_BAD_SHAPE;
+    if (any_null(logp, labels, seq, margins, pair_loss, coef, loss)) return MMSUM_ERR_BAD_ALIGN;
     hipStream_t s = (hipStream_t)stream;
     PairArgs a = {logp, labels, ref, P, T, V, average, beta, smoothing, seq, margins, pair_loss, coef, loss};
     // one workgroup, a wave a pair, with the mean (us, this | two launches: 1 x 33 3.2 | 4.7, 16 x 128 4.5 | 5.4; in turns 36 x 32 6.4 | 5.2, 128 x 256 28 | 6.5)
@@ -569,7 +572,7 @@ extern "C" int mmsum_preference_loss(int dtype, const void* logits, long ld, con
     if (P <= 0 || T <= 0 || bad_rows(2L * P * T, V, ld) || W < V || W > 0x7fffffff - 16384 || ldd < W || !(smoothing >= 0.f && smoothing <= 1.f)) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
     if (workspace == nullptr) return MMSUM_ERR_WORKSPACE;
-    if (bad_align(dtype, logits) || bad_align(dtype, dlogits) || ((uintptr_t)workspace & 15)) return MMSUM_ERR_BAD_ALIGN;
+    if (any_null(logits, labels, loss, margins, seq, dlogits) || bad_align(dtype, logits) || bad_align(dtype, dlogits) || ((uintptr_t)workspace & 15)) return MMSUM_ERR_BAD_ALIGN;
     const int R = 2 * P * T;
     float* const logp = static_cast<float*>(workspace);
     float* const stats = logp + R;
@@ -602,7 +605,7 @@ static int policy_setup(PolicyArgs& p, const int64_t* labels, int V, const float
                         float clip_high, float kl_coef, int seq_mean, void* workspace) {
     if (!(clip_low >= 0.f) || !(clip_high >= 0.f) || kl_coef != kl_coef) return MMSUM_ERR_BAD_SHAPE;
     if (workspace == nullptr) return MMSUM_ERR_WORKSPACE;
-    if ((uintptr_t)workspace & 15) return MMSUM_ERR_BAD_ALIGN;
+    if (any_null(labels, old_logp, adv) || ((uintptr_t)workspace & 15)) return MMSUM_ERR_BAD_ALIGN;
     p.labels = labels; p.V = V;
     p.old_logp = old_logp; p.ref_logp = ref_logp; p.adv = adv;
     p.terms = static_cast<float*>(workspace);
@@ -615,6 +618,7 @@ static int policy_setup(PolicyArgs& p, const int64_t* labels, int V, const float
 extern "C" int mmsum_policy_terms(const float* logp, const int64_t* labels, const float* old_logp, const float* ref_logp, const float* adv, int adv_per_token, int N,
                                   int T, int V, float clip_low, float clip_high, float kl_coef, int seq_mean, float* out, float* coef, void* workspace, void* stream) {
     if (N <= 0 || T <= 0 || V <= 0 || (long)N * T > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    if (any_null(logp, out, coef)) return MMSUM_ERR_BAD_ALIGN;
     PolicyArgs p = {};
     int rc = policy_setup(p, labels, V, old_logp, ref_logp, adv, adv_per_token, N, T, clip_low, clip_high, kl_coef, seq_mean, workspace);
     hipStream_t s = (hipStream_t)stream;
@@ -631,7 +635,7 @@ extern "C" int mmsum_policy_loss(int dtype, const void* logits, long ld, const i
                                  void* dlogits, long ldd, int W, void* workspace, void* stream) {
     if (N <= 0 || T <= 0 || bad_rows((long)N * T, V, ld) || W < V || W > 0x7fffffff - 16384 || ldd < W) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
-    if (bad_align(dtype, logits) || bad_align(dtype, dlogits)) return MMSUM_ERR_BAD_ALIGN;
+    if (any_null(logits, out, logp, dlogits) || bad_align(dtype, logits) || bad_align(dtype, dlogits)) return MMSUM_ERR_BAD_ALIGN;
     PolicyArgs p = {};
     int rc = policy_setup(p, labels, V, old_logp, ref_logp, adv, adv_per_token, N, T, clip_low, clip_high, kl_coef, seq_mean, workspace);
     hipStream_t s = (hipStream_t)stream;

@@ -637,9 +637,11 @@ def _labels_of(labels, N, T):
     return labels.contiguous()
 
 
-def _f32_of(t, shape, what):
-    if t is None:
+def _f32_of(t, shape, what, optional=False):
+    if t is None and optional:
         return None
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s: a float32 tensor expected, got %r" % (what, t))
     if t.dtype != torch.float32:
         raise TypeError("%s: float32 expected, got %s" % (what, t.dtype))
     _need(t.shape == shape, "%s: shape %s expected, got %s", what, shape, t.shape)
@@ -714,7 +716,7 @@ def sequence_logprob(logp, labels, V, average=False):
 def _pairs_of(N, ref, smoothing):
     _need(N % 2 == 0, "preference loss: [chosen; rejected] sequences expected, got an odd number (%d)", N)
     _need(0.0 <= smoothing <= 1.0, "label_smoothing: 0 .. 1 expected, got %r", smoothing)
-    return N // 2, _f32_of(ref, (N,), "ref_logps")
+    return N // 2, _f32_of(ref, (N,), "ref_logps", optional=True)
 
 
 def preference_pairs(logp, labels, ref, V, beta, smoothing, average):
@@ -747,7 +749,8 @@ def _policy_of(N, T, old, adv, ref, clip_low, clip_high, kl_coef, reduction):
     _need(reduction in ("token", "sequence"), "reduction: 'token' or 'sequence' expected, got %r", reduction)
     _need(clip_low >= 0.0 and clip_high >= 0.0, "clip_low, clip_high: not negative")
     _need(kl_coef == kl_coef and (kl_coef == 0.0 or ref is not None), "kl_coef without ref_logps")
-    return _f32_of(old, (N, T), "old_logps"), _f32_of(adv, (N,) if adv.dim() == 1 else (N, T), "advantages"), _f32_of(ref, (N, T), "ref_logps")
+    per_token = isinstance(adv, torch.Tensor) and adv.dim() != 1
+    return _f32_of(old, (N, T), "old_logps"), _f32_of(adv, (N, T) if per_token else (N,), "advantages"), _f32_of(ref, (N, T), "ref_logps", optional=True)
 
 
 def policy_terms(logp, labels, old, adv, ref, V, clip_low, clip_high, kl_coef, reduction):
@@ -852,7 +855,7 @@ def gemm_i8(qx, sx, qw, sw, out, bias=None, gelu=False):
             raise TypeError("%s: int8 expected, got %s" % (what, t.dtype))
     _need(qw.shape[1] == K and K % I8_K_STEP == 0 and 0 < K <= 131072, "gemm_i8: operands as quantize_rows leaves them expected")
     _need(out.shape == (M, N), "out: shape %s expected, got %s", (M, N), out.shape)
-    sx, sw, bias = _f32_of(sx, (M,), "sx"), _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias")
+    sx, sw, bias = _f32_of(sx, (M,), "sx"), _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias", optional=True)
     ldx, ldw, ldy = _pitch2(qx, "qx"), _pitch2(qw, "qw"), _pitch2(out, "out")
     _dt(out)
     dev = _device(qx, sx, qw, sw, out, bias)
@@ -868,7 +871,7 @@ def linear_i8(x, qw, sw, out=None, bias=None, gelu=False, out_dtype=None):
     if qw.dtype != torch.int8:
         raise TypeError("qw: int8 expected, got %s" % qw.dtype)
     _need(0 < K <= 131072 and qw.shape[1] == -(-K // I8_K_STEP) * I8_K_STEP, "linear_i8: weights as quantize_rows leaves them expected")
-    sw, bias = _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias")
+    sw, bias = _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias", optional=True)
     ldx, ldw, dt = _pitch2(x, "x"), _pitch2(qw, "qw"), _dt(x)
     dev = _device(x, qw, sw, out, bias)
     if out is None:

@@ -1,0 +1,58 @@
+"""CPU: calls of the scoring / loss / embedding / 8-bit entry points that have to be refused, and what the host does around a launch."""
+import pytest
+import torch
+
+BF, F32 = 1, 0
+FAKE = 1 << 20                       # a 16-byte aligned address: refused calls never dereference it
+
+
+def refused(exc, fn, *a, **k):
+    with pytest.raises(exc):
+        fn(*a, **k)
+
+
+def calls():
+    """Every C entry with arguments that pass its checks (but for the launch, which needs a device): name, arguments, the positions of pointers that
+    may be missing."""
+    F = FAKE
+    return [
+        ("mmsum_token_logprob", [BF, F, 8, F, F, None, 4, 8, None], {5, 8}),
+        ("mmsum_token_logprob_bwd", [BF, F, 8, F, F, F, 1, None, F, 8, 8, 4, 8, None], {7, 13}),
+        ("mmsum_sequence_logprob", [F, F, 2, 3, 8, 0, F, None], {7}),
+        ("mmsum_preference_pairs", [F, F, None, 2, 3, 8, 0.1, 0.0, 0, F, F, F, F, F, None], {2, 14}),
+        ("mmsum_preference_loss", [BF, F, 8, F, None, 2, 3, 8, 0.1, 0.0, 0, F, F, F, F, 8, 8, F, None], {4, 17, 18}),
+        ("mmsum_policy_terms", [F, F, F, None, F, 0, 2, 3, 8, 0.2, 0.2, 0.0, 0, F, F, F, None], {3, 15, 16}),
+        ("mmsum_policy_loss", [BF, F, 8, F, F, None, F, 0, 2, 3, 8, 0.2, 0.2, 0.0, 0, F, F, F, 8, 8, F, None], {5, 20, 21}),
+        ("mmsum_embed_fwd", [BF, F, F, 8, F, 8, 4, 10, 8, 1.0, None], {10}),
+        ("mmsum_embed_bwd", [BF, F, 8, F, 4, 10, 8, 1.0, -1, 0, F, None, None], {11, 12}),
+        ("mmsum_quantize_i8", [BF, F, 8, 4, 8, F, 128, F, None], {8}),
+        ("mmsum_gemm_i8", [F, 128, F, F, 128, F, None, BF, F, 16, 4, 16, 128, 0, None], {6, 14}),
+        ("mmsum_linear_i8", [BF, F, 128, F, 128, F, None, BF, F, 16, 4, 16, 128, 0, F, None], {6, 14, 15}),
+    ]
+
+
+@pytest.mark.parametrize("call", calls(), ids=lambda c: c[0])
+def test_a_missing_pointer_is_refused(call):
+    from multimodalsum_amd import _lib
+    name, args, may_miss = call
+    tried = 0
+    for i, a in enumerate(args):
+        if a == FAKE and i not in may_miss:
+            assert getattr(_lib.lib, name)(*args[:i], None, *args[i + 1:]) == -3, (name, i)
+            tried += 1
+    assert tried >= 3
+
+
+def test_missing_tensors_are_refused():
+    import multimodalsum_amd as mm
+    from multimodalsum_amd import kernels as kn
+    x, lab, z, adv = torch.zeros(4, 3, 8), torch.zeros(4, 3, dtype=torch.int64), torch.zeros(4, 3), torch.zeros(4)
+    refused(TypeError, mm.policy_loss_and_grad, x, lab, None, adv)
+    refused(TypeError, mm.policy_loss_and_grad, x, lab, z, None)
+    refused(TypeError, mm.policy_loss_and_grad, x, lab, z, 1.0)
+    refused(TypeError, kn.policy_terms, z, lab, None, adv, None, 8, 0.2, 0.2, 0.0, "token")
+    refused(ValueError, mm.policy_loss_and_grad, x, lab, z, torch.zeros(()))
+    q, s, w = torch.zeros(4, 128, dtype=torch.int8), torch.zeros(4), torch.zeros(4, 128)
+    refused(TypeError, kn.gemm_i8, q, None, q, s, torch.zeros(4, 4))
+    refused(TypeError, kn.gemm_i8, q, s, q, None, torch.zeros(4, 4))
+    refused(TypeError, kn.linear_i8, w, q, None)
