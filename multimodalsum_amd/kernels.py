@@ -4,6 +4,7 @@ PyTorch is plumbing here (device memory, streams); every function below enqueues
 kernels from libmmsum_hip.so and nothing else.  There is no fallback path: CPU tensors raise.
 """
 import ctypes
+import operator
 
 import torch
 
@@ -786,6 +787,15 @@ def _ids_of(ids):
     return ids.reshape(-1)
 
 
+def padding_row(index, V):
+    """The table row that gets no gradient: None (no such row) or index as torch.nn.Embedding takes it, negative ones counted from the end."""
+    if index is None:
+        return None
+    index = operator.index(index)
+    _need(-V <= index < V, "padding index %d of a table of %d rows", index, V)
+    return index + V if index < 0 else index
+
+
 def _pitch2(t, what):
     _need(t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1), "%s: [rows, columns] with unit inner stride expected", what)
     ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -807,11 +817,12 @@ def embed_fwd(ids, table, scale=1.0):
 
 
 def embed_bwd(dy, ids, V, scale=1.0, pad_id=None, out=None, accumulate=False):
-    """out f32 [V, D] (+)= scale * sum of dy rows by id (pad_id and ids outside 0 .. V-1: none)."""
+    """out f32 [V, D] (+)= scale * sum of dy rows by id (pad_id, a row as padding_row takes it, and ids outside 0 .. V-1: none)."""
     flat = _ids_of(ids).contiguous()
     D, n = dy.shape[-1], flat.numel()
     _need(dy.shape[:-1] == ids.shape, "dy: shape %s expected, got %s", (*ids.shape, D), dy.shape)
     _need(V > 0 and D > 0 and n < 2 ** 30, "embed_bwd: %d ids into [%d, %d]", n, V, D)
+    pad_id = padding_row(pad_id, V)
     dy = dy.reshape(-1, D)
     if n and ((D > 1 and dy.stride(1) != 1) or (n > 1 and dy.stride(0) < D)):        # a gradient that is one row, repeated, among them
         dy = dy.contiguous()
@@ -826,7 +837,7 @@ def embed_bwd(dy, ids, V, scale=1.0, pad_id=None, out=None, accumulate=False):
         _apart(dy, out)
     nbytes = lib.mmsum_embed_bwd_workspace(n, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _launch("mmsum_embed_bwd", dev, _dt(dy), _p(dy), lddy, _p(flat), n, V, D, float(scale), -1 if pad_id is None else int(pad_id), int(bool(accumulate)), _p(out), _p(ws))
+    _launch("mmsum_embed_bwd", dev, _dt(dy), _p(dy), lddy, _p(flat), n, V, D, float(scale), -1 if pad_id is None else pad_id, int(bool(accumulate)), _p(out), _p(ws))
     return out
 
 

@@ -132,7 +132,8 @@ class _EmbeddingFn(torch.autograd.Function):
 
 def scaled_embedding(ids, table, scale=1.0, padding_idx=None):
     """scale * table[ids] (f32 or bf16 table, int64 ids of any shape; ids outside the table give zero rows), differentiable with respect to the table
-    (padding_idx: no gradient)."""
+    (padding_idx: a row without a gradient, negative ones counted from the end)."""
+    padding_idx = kn.padding_row(padding_idx, table.shape[0])
     if table.requires_grad and torch.is_grad_enabled():
         return _EmbeddingFn.apply(ids, table, float(scale), padding_idx)
     return kn.embed_fwd(ids, table, float(scale))
@@ -143,12 +144,12 @@ class ScaledEmbedding(nn.Module):
 
     def __init__(self, num_embeddings, embedding_dim, scale=1.0, padding_idx=None, device="cuda", dtype=torch.float32):
         super().__init__()
-        self.scale, self.padding_idx = float(scale), padding_idx
+        self.scale, self.padding_idx = float(scale), kn.padding_row(padding_idx, num_embeddings)
         self.weight = nn.Parameter(torch.empty(num_embeddings, embedding_dim, device=device, dtype=dtype))
         nn.init.normal_(self.weight, std=0.02)
         if padding_idx is not None:
             with torch.no_grad():
-                self.weight[padding_idx].zero_()
+                self.weight[self.padding_idx].zero_()
 
     def forward(self, ids):
         return scaled_embedding(ids, self.weight, self.scale, self.padding_idx)

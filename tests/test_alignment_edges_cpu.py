@@ -56,3 +56,44 @@ def test_missing_tensors_are_refused():
     refused(TypeError, kn.gemm_i8, q, None, q, s, torch.zeros(4, 4))
     refused(TypeError, kn.gemm_i8, q, s, q, None, torch.zeros(4, 4))
     refused(TypeError, kn.linear_i8, w, q, None)
+
+
+class Recorder:
+    """In place of a launch: what would have been launched; tensors stay on the CPU."""
+
+    def __init__(self, monkeypatch, fill=None):
+        from multimodalsum_amd import kernels as kn
+        self.calls, self.fill = [], fill or {}
+        monkeypatch.setattr(kn, "_device", lambda *t: torch.device("cpu"))
+        monkeypatch.setattr(kn, "_p", lambda t: t)
+        monkeypatch.setattr(kn, "_launch", self.launch)
+
+    def launch(self, name, device, *args):
+        self.calls.append((name, args))
+        if name in self.fill:
+            self.fill[name](*args)
+
+
+def test_padding_rows_count_from_the_end(monkeypatch):
+    import multimodalsum_amd as mm
+    ids, dy = torch.tensor([[1, 9, 8]]), torch.ones(1, 3, 8)
+
+    def written(*a):
+        a[10].zero_()
+    rec = Recorder(monkeypatch, {"mmsum_embed_bwd": written, "mmsum_embed_fwd": lambda *a: a[4].zero_()})
+    for pad, row in ((None, -1), (0, 0), (1, 1), (9, 9), (-1, 9), (-2, 8), (-10, 0)):
+        mm.scaled_embedding_grad(dy, ids, 10, padding_idx=pad)
+        assert rec.calls[-1][0] == "mmsum_embed_bwd" and rec.calls[-1][1][8] == row
+        t = torch.zeros(10, 8, requires_grad=True)
+        mm.scaled_embedding(ids, t, 2.0, pad).sum().backward()
+        assert rec.calls[-1][0] == "mmsum_embed_bwd" and rec.calls[-1][1][8] == row
+        m = mm.ScaledEmbedding(10, 8, padding_idx=pad, device="cpu")
+        assert (m.weight[row] == 0).all() if pad is not None else (m.weight != 0).any(1).all()
+        m(ids).sum().backward()
+        assert rec.calls[-1][0] == "mmsum_embed_bwd" and rec.calls[-1][1][8] == row
+    for pad in (10, -11, 2 ** 40):
+        refused(ValueError, mm.scaled_embedding_grad, dy, ids, 10, padding_idx=pad)
+        refused(ValueError, mm.scaled_embedding, ids, torch.zeros(10, 8), 1.0, pad)
+        refused(ValueError, mm.scaled_embedding, ids, torch.zeros(10, 8, requires_grad=True), 1.0, pad)
+        refused(ValueError, mm.ScaledEmbedding, 10, 8, padding_idx=pad, device="cpu")
+    refused(TypeError, mm.scaled_embedding_grad, dy, ids, 10, padding_idx=1.5)
