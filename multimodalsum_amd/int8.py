@@ -10,7 +10,8 @@ from . import kernels as kn
 
 class Int8Linear(nn.Module):
     """y = x W^T (+ bias) (then GELU, erf form) with W [N, K] (f32 or bf16) held as int8 [N, Kp] + one f32 scale per row.  x [..., K] f32 or bf16,
-    y [..., N] in out_dtype (default: x's).  A token whose values are not all finite gives NaN.  No gradient: inputs that require one are refused."""
+    y [..., N] in out_dtype (default: x's).  A token whose values are not all finite gives NaN.  No gradient: inputs that require one, or carry a
+    forward-mode tangent, are refused."""
 
     def __init__(self, weight, bias=None, gelu=False, out_dtype=None):
         super().__init__()
@@ -34,6 +35,7 @@ class Int8Linear(nn.Module):
     def forward(self, x):
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("Int8Linear is for inference: no gradient (use torch.no_grad() or detach the input)")
+        kn.no_tangent(x, "Int8Linear")
         K = self.in_features
         if x.dim() < 1 or x.shape[-1] != K:
             raise ValueError("x: [..., %d] expected, got %s" % (K, tuple(x.shape)))

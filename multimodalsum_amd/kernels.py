@@ -787,6 +787,12 @@ def _ids_of(ids):
     return ids.reshape(-1)
 
 
+def no_tangent(t, what):
+    """Refuses a forward-mode dual tensor, whose tangent a launch would drop without a word."""
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError("%s has no forward-mode derivative" % what)
+
+
 def padding_row(index, V):
     """The table row that gets no gradient: None (no such row) or index as torch.nn.Embedding takes it, negative ones counted from the end."""
     if index is None:

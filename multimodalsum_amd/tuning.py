@@ -134,6 +134,7 @@ def scaled_embedding(ids, table, scale=1.0, padding_idx=None):
     """scale * table[ids] (f32 or bf16 table, int64 ids of any shape; ids outside the table give zero rows), differentiable with respect to the table
     (padding_idx: a row without a gradient, negative ones counted from the end)."""
     padding_idx = kn.padding_row(padding_idx, table.shape[0])
+    kn.no_tangent(table, "scaled_embedding")
     if table.requires_grad and torch.is_grad_enabled():
         return _EmbeddingFn.apply(ids, table, float(scale), padding_idx)
     return kn.embed_fwd(ids, table, float(scale))
