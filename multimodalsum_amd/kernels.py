@@ -726,10 +726,13 @@ def preference_pairs(logp, labels, ref, V, beta, smoothing, average):
     labels, logp = _labels_of(labels, N, T), _f32_of(logp, (N, T), "logp")
     P, ref = _pairs_of(N, ref, smoothing)
     dev = _device(logp, labels, ref)
-    seq, margins, pair_loss, coef, loss = torch.empty(6 * P + 1, dtype=torch.float32, device=dev).split([2 * P, P, P, 2 * P, 1])
+    # memory of their own: pieces of one buffer would be views that autograd's outputs may not be, and share a version counter with what a backward
+    # pass saves
+    loss, margins, seq = (torch.empty(shape, dtype=torch.float32, device=dev) for shape in ((), P, 2 * P))
+    pair_loss, coef = torch.empty(3 * P, dtype=torch.float32, device=dev).split([P, 2 * P])
     _launch("mmsum_preference_pairs", dev, _p(logp), _p(labels), _p(ref), P, T, int(V), float(beta), float(smoothing), int(bool(average)), _p(seq), _p(margins),
             _p(pair_loss), _p(coef), _p(loss))
-    return loss.reshape(()), margins, seq, coef
+    return loss, margins, seq, coef
 
 
 def preference_loss(logits, labels, ref, beta, smoothing, average, dlogits=None):

@@ -119,3 +119,27 @@ def test_forward_mode_tangents_are_refused(monkeypatch):
     mm.scaled_embedding(ids, torch.ones(10, 8), 2.0)
     lin(torch.ones(3, 8))
     assert [c[0] for c in rec.calls][-2:] == ["mmsum_embed_fwd", "mmsum_linear_i8"]
+
+
+@pytest.mark.parametrize("kind", ["preference", "policy"])
+def test_losses_may_be_changed_in_place(monkeypatch, kind):
+    """loss /= steps, loss += another loss, and changes of what the module keeps for monitoring leave the backward pass as it was."""
+    import multimodalsum_amd as mm
+
+    def fill(value, *at):
+        def f(*a):
+            for i in at:
+                a[i].fill_(value)
+        return f
+    rec = Recorder(monkeypatch, {"mmsum_preference_pairs": fill(8.0, 9, 10, 11, 12, 13), "mmsum_policy_terms": fill(8.0, 13, 14),
+                                 "mmsum_token_logprob_bwd": lambda *a: a[8].copy_(a[7] * a[5].reshape(-1)[0])})
+    lab, z, adv = torch.zeros(4, 3, dtype=torch.int64), torch.zeros(4, 3), torch.zeros(4)
+    for change in (lambda m, l: l.div_(4), lambda m, l: l.add_(torch.ones(())).div_(4), lambda m, l: (m.logps.zero_(), l.div_(4)),
+                   lambda m, l: ((m.margins if kind == "preference" else m.kl).clamp_(max=1.0), l.div_(4)), lambda m, l: (l.detach().zero_(), l.div_(4))):
+        x = torch.zeros(4, 3, 8, requires_grad=True)
+        m = mm.PreferenceLoss() if kind == "preference" else mm.ClippedPolicyLoss()
+        loss = m(x, lab) if kind == "preference" else m(x, lab, z, adv)
+        assert loss.shape == () and loss == 8.0
+        change(m, loss)
+        loss.backward()
+        assert (x.grad == 2.0).all() and rec.calls[-1][0] == "mmsum_token_logprob_bwd"

@@ -20,3 +20,22 @@ def test_padding_rows_counted_from_the_end(pad, n):
     want[pad] = 0.0
     assert torch.equal(m.weight.grad, want[:, None].expand(50, 16))
     assert torch.equal(mm.scaled_embedding_grad(torch.ones(n, 16, device="cuda"), ids, 50, 2.0, padding_idx=pad), m.weight.grad)
+
+
+def test_losses_may_be_changed_in_place():
+    """Accumulation steps: loss /= 4 and a change of what is kept for monitoring, then the backward pass."""
+    import multimodalsum_amd as mm
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(6, 5, 50, generator=g).cuda()
+    labels, adv = torch.randint(0, 50, (6, 5), generator=g).cuda(), torch.randn(6, generator=g).cuda()
+    _, old = mm.sequence_logprobs(x, labels)
+    pref, pol = mm.PreferenceLoss(beta=0.3), mm.ClippedPolicyLoss(kl_coef=0.1)
+    for call, kept in ((lambda t: pref(t, labels), lambda: (pref.margins, pref.logps)), (lambda t: pol(t, labels, old - 0.1, adv, old + 0.2), lambda: (pol.kl, pol.clipped, pol.logps))):
+        a, b = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+        call(a).backward()
+        loss = call(b)
+        loss /= 4
+        for t in kept():
+            t.zero_()
+        loss.backward()
+        assert torch.equal(b.grad, a.grad / 4) and (a.grad != 0).any()      # a power of two: exact
