@@ -618,6 +618,12 @@ def _launch(name, device, *args):
         check(rc, name)
 
 
+def _wrote(t):
+    """A launch has written into the caller's tensor: a backward pass that saved it has to find out, as after torch's own in-place operations."""
+    if t is not None and not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _rows_of(t, what):
     """[N, T, V] with unit inner stride and one row pitch -> (N, T, V, pitch)."""
     _need(t.dim() == 3, "%s: [N, T, V] expected, got %s", what, t.shape)
@@ -686,6 +692,7 @@ def token_logprob(logits, labels, stats=None):
     dev = _device(logits, labels, stats)
     logp = torch.empty(N, T, dtype=torch.float32, device=dev)
     _launch("mmsum_token_logprob", dev, _dt(logits), _p(logits), ld, _p(labels), _p(logp), _p(stats), N * T, V)
+    _wrote(stats)
     return logp
 
 
@@ -698,9 +705,11 @@ def token_logprob_bwd(logits, labels, stats, coef, alpha=None, dlogits=None):
     if alpha is not None:
         _need(alpha.dtype == torch.float32 and alpha.numel() == 1, "alpha: one float32 expected")
     dev = _device(logits, labels, stats, coef, alpha, dlogits)
+    given = dlogits
     dlogits, ldd, W = _dlogits_of(dlogits, logits, N, T, V, ld)
     _launch("mmsum_token_logprob_bwd", dev, _dt(logits), _p(logits), ld, _p(labels), _p(stats), _p(coef), T if coef.dim() == 1 else 1, _p(alpha),
             _p(dlogits), ldd, W, N * T, V)
+    _wrote(given)
     return dlogits
 
 
@@ -740,12 +749,14 @@ def preference_loss(logits, labels, ref, beta, smoothing, average, dlogits=None)
     N, T, V, ld = _rows_of(logits, "logits")
     labels = _labels_of(labels, N, T)
     P, ref = _pairs_of(N, ref, smoothing)
+    given = dlogits
     dlogits, ldd, W = _dlogits_of(dlogits, logits, N, T, V, ld)
     dev = _device(logits, labels, ref, dlogits)
     seq, margins, loss = torch.empty(3 * P + 1, dtype=torch.float32, device=dev).split([2 * P, P, 1])
     ws = torch.empty(lib.mmsum_preference_workspace(P, T), dtype=torch.uint8, device=dev)
     _launch("mmsum_preference_loss", dev, _dt(logits), _p(logits), ld, _p(labels), _p(ref), P, T, V, float(beta), float(smoothing), int(bool(average)), _p(loss),
             _p(margins), _p(seq), _p(dlogits), ldd, W, _p(ws))
+    _wrote(given)
     return loss.reshape(()), margins, seq, dlogits
 
 
@@ -775,12 +786,14 @@ def policy_loss(logits, labels, old, adv, ref, clip_low, clip_high, kl_coef, red
     N, T, V, ld = _rows_of(logits, "logits")
     labels = _labels_of(labels, N, T)
     old, adv, ref = _policy_of(N, T, old, adv, ref, clip_low, clip_high, kl_coef, reduction)
+    given = dlogits
     dlogits, ldd, W = _dlogits_of(dlogits, logits, N, T, V, ld)
     dev = _device(logits, labels, old, adv, ref, dlogits)
     out, logp = torch.empty(3, dtype=torch.float32, device=dev), torch.empty(N, T, dtype=torch.float32, device=dev)
     ws = torch.empty(lib.mmsum_policy_workspace(N, T), dtype=torch.uint8, device=dev)
     _launch("mmsum_policy_loss", dev, _dt(logits), _p(logits), ld, _p(labels), _p(old), _p(ref), _p(adv), int(adv.dim() == 2), N, T, V, float(clip_low),
             float(clip_high), float(kl_coef), int(reduction == "sequence"), _p(out), _p(logp), _p(dlogits), ldd, W, _p(ws))
+    _wrote(given)
     return out, logp, dlogits
 
 
@@ -840,6 +853,7 @@ def embed_bwd(dy, ids, V, scale=1.0, pad_id=None, out=None, accumulate=False):
     _need(out is None or (out.dtype == torch.float32 and out.shape == (V, D) and out.is_contiguous()), "out: packed float32 [%d, %d] expected", V, D)
     _dt(dy)
     dev = _device(dy, ids, out)
+    given = out
     if out is None:
         out = torch.empty(V, D, dtype=torch.float32, device=dev)
     else:
@@ -847,6 +861,7 @@ def embed_bwd(dy, ids, V, scale=1.0, pad_id=None, out=None, accumulate=False):
     nbytes = lib.mmsum_embed_bwd_workspace(n, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _launch("mmsum_embed_bwd", dev, _dt(dy), _p(dy), lddy, _p(flat), n, V, D, float(scale), -1 if pad_id is None else pad_id, int(bool(accumulate)), _p(out), _p(ws))
+    _wrote(given)
     return out
 
 
@@ -881,6 +896,7 @@ def gemm_i8(qx, sx, qw, sw, out, bias=None, gelu=False):
     dev = _device(qx, sx, qw, sw, out, bias)
     if M and N:
         _launch("mmsum_gemm_i8", dev, _p(qx), ldx, _p(sx), _p(qw), ldw, _p(sw), _p(bias), _dt(out), _p(out), ldy, M, N, K, int(bool(gelu)))
+        _wrote(out)
     return out
 
 
@@ -894,6 +910,7 @@ def linear_i8(x, qw, sw, out=None, bias=None, gelu=False, out_dtype=None):
     sw, bias = _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias", optional=True)
     ldx, ldw, dt = _pitch2(x, "x"), _pitch2(qw, "qw"), _dt(x)
     dev = _device(x, qw, sw, out, bias)
+    given = out
     if out is None:
         out, ldy = torch.empty(M, N, dtype=out_dtype or x.dtype, device=dev), N
     else:
@@ -905,4 +922,5 @@ def linear_i8(x, qw, sw, out=None, bias=None, gelu=False, out_dtype=None):
         ws = torch.empty(M * (qw.shape[1] + 4), dtype=torch.uint8, device=dev)
         _launch("mmsum_linear_i8", dev, dt, x.data_ptr(), ldx, qw.data_ptr(), ldw, sw.data_ptr(), None if bias is None else bias.data_ptr(), dto, out.data_ptr(), ldy, M, N, K,
                 int(bool(gelu)), ws.data_ptr())
+        _wrote(given)
     return out

@@ -4,7 +4,7 @@ term, and the scaled embedding with its reproducible gradient.
 Logits are [N, T, V] (f32 or bf16; a view of a padded buffer will do), labels int64 [N, T]; a label outside 0 .. V-1 (-100, say) marks a
 position that does not count.  Two forms of each loss: a module whose result goes into a larger autograd graph, and a fused call that turns
 logits into loss and gradient at once, as the fused training step does with its label-smoothing loss (`dlogits=logits` writes the gradient
-over the logits).
+over the logits, which are gone then: a backward pass that saved them raises, as after any change in place).
 """
 import torch
 import torch.nn as nn

@@ -143,3 +143,29 @@ def test_losses_may_be_changed_in_place(monkeypatch, kind):
         change(m, loss)
         loss.backward()
         assert (x.grad == 2.0).all() and rec.calls[-1][0] == "mmsum_token_logprob_bwd"
+
+
+def test_results_written_into_a_tensor_count_as_changes_in_place(monkeypatch):
+    """A backward pass that saved a tensor which a later call writes over raises instead of reading the gradient as logits."""
+    import multimodalsum_amd as mm
+    from multimodalsum_amd import kernels as kn
+    Recorder(monkeypatch)
+    lab, z, adv = torch.zeros(4, 3, dtype=torch.int64), torch.zeros(4, 3), torch.zeros(4)
+    for fused in (lambda t: mm.preference_loss_and_grad(t, lab, dlogits=t), lambda t: mm.policy_loss_and_grad(t, lab, z, adv, dlogits=t),
+                  lambda t: kn.token_logprob_bwd(t, lab, torch.zeros(4, 3, 2), z, dlogits=t)):
+        for loss in (lambda t: mm.PreferenceLoss()(t, lab), lambda t: mm.ClippedPolicyLoss()(t, lab, z, adv), lambda t: (t * t).sum()):
+            logits = torch.zeros(4, 3, 8, requires_grad=True) * 1.0
+            value = loss(logits)
+            with torch.no_grad():
+                fused(logits)
+            refused(RuntimeError, value.backward)
+    q, s, out, stats, dy, ids = torch.zeros(4, 128, dtype=torch.int8), torch.zeros(4), torch.zeros(4, 4), torch.zeros(4, 3, 2), torch.zeros(3, 8), torch.tensor([1, 2, 3])
+    for t, call in ((out, lambda t: kn.gemm_i8(q, s, q, s, t)), (out, lambda t: kn.linear_i8(torch.zeros(4, 128), q, s, t)), (stats, lambda t: kn.token_logprob(torch.zeros(4, 3, 8), lab, t)),
+                    (torch.zeros(10, 8), lambda t: kn.embed_bwd(dy, ids, 10, out=t)), (torch.zeros(10, 8), lambda t: kn.embed_bwd(dy, ids, 10, out=t, accumulate=True)),
+                    (torch.zeros(4, 3, 9), lambda t: mm.preference_loss_and_grad(torch.zeros(4, 3, 8), lab, dlogits=t))):
+        before = t._version
+        call(t)
+        assert t._version > before
+    with torch.inference_mode():                                   # tensors without a version
+        t = torch.zeros(4, 3, 8)
+        mm.preference_loss_and_grad(t, lab, dlogits=t)
