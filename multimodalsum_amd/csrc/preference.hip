@@ -59,8 +59,16 @@ template <typename T> __device__ __forceinline__ void store_chunk(T* d, int c, i
             if (c + k < V) d[c + k] = t[k];
     }
 }
-// bf16 results keep 8 bits: the hardware exponential (2^-22) is exact enough; f32 rows take the library's expf
-template <typename T> __device__ __forceinline__ float row_exp(float d) { return sizeof(T) == 2 ? __expf(d) : expf(d); }
+// For the sums, whose log-probabilities are f32 whatever the rows' type.  The hardware's exponential is of base 2, and f32(log2 e) is 1.3e-8 of it too
+// small: alone it makes every term of a row too large, 5.8e-8 of the sum on average at 50,265 logits, an error that does not average out over
+// tokens.  Its rest as a second constant leaves 1e-9, for one more instruction under the loads (72 x 141 rows 177 us with and without).  f32 rows take
+// the library's expf (2e-9).
+template <typename T> __device__ __forceinline__ float row_exp(float d) {
+    if constexpr (sizeof(T) == 4) return expf(d);
+    else return __builtin_amdgcn_exp2f(fmaf(d, 0x1.715476p+0f, d * 0x1.4ae0c0p-26f));
+}
+// for the gradient: bf16 results keep 8 bits, the shorter form (2^-22) is exact enough
+template <typename T> __device__ __forceinline__ float grad_exp(float d) { return sizeof(T) == 2 ? __expf(d) : expf(d); }
 
 template <int NT> __device__ __forceinline__ float block_max(float v, float* sh) {
     v = warp_max(v);
@@ -226,7 +234,7 @@ __global__ __launch_bounds__(NT, NT == 512 && !POLICY ? 6 : 4) void row_kernel(R
                 float f[kPer<T>];
                 unpack<T>(reg[i], f);
 #pragma unroll
-                for (int k = 0; k < kPer<T>; ++k) f[k] = c0 == 0.f ? 0.f : cs * row_exp<T>(f[k] - m);
+                for (int k = 0; k < kPer<T>; ++k) f[k] = c0 == 0.f ? 0.f : cs * grad_exp<T>(f[k] - m);
                 if (y >= c && y < c + kPer<T>) {
 #pragma unroll
                     for (int k = 0; k < kPer<T>; ++k)
@@ -291,7 +299,7 @@ __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs<T> a) {
             float f[kPer<T>];
             unpack<T>(load_chunk(x, (int)c, a.V), f);
 #pragma unroll
-            for (int k = 0; k < kPer<T>; ++k) f[k] = (c0 == 0.f ? 0.f : cs * row_exp<T>(f[k] - m)) + (c + k == y ? c0 : 0.f);
+            for (int k = 0; k < kPer<T>; ++k) f[k] = (c0 == 0.f ? 0.f : cs * grad_exp<T>(f[k] - m)) + (c + k == y ? c0 : 0.f);
             store_chunk(d, (int)c, a.V, f);
         }
         zero_cols<T, NT>(d, a.V, a.W);
@@ -425,7 +433,7 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(const T* logits, long 
                 float f[kPer<T>];
                 unpack<T>(reg[u], f);
 #pragma unroll
-                for (int k = 0; k < kPer<T>; ++k) f[k] = cs * row_exp<T>(f[k] - m);
+                for (int k = 0; k < kPer<T>; ++k) f[k] = cs * grad_exp<T>(f[k] - m);
                 if (y >= c && y < c + kPer<T>) {
 #pragma unroll
                     for (int k = 0; k < kPer<T>; ++k)
