@@ -57,3 +57,31 @@ def test_sums_of_exponentials_are_not_biased(dt):
             off.append(stats[..., 1].double() / s - 1)
         off = torch.stack(off)
         assert off.mean().abs() < H / 3 and off.abs().max() < 160 * H
+
+
+@pytest.mark.parametrize("M", [1, 40, 400, 40000])
+def test_gelu_of_the_8bit_linear_layer(M):
+    """The epilogue's GELU by itself: activations of one give y = w's row, at every size of x; from the tail to values that pass through, zero and infinities.
+
+    Bounds, relative, from the argument z as the same product without GELU has it: the polynomials and their products 10 H, the exponential's argument
+    z^2 / 2 rounded twice (and its factor) 3 z^2 H at most; bf16: the fit's 2.4e-5 and half a step of the result on top.  Results below 1e-37 are zero."""
+    from multimodalsum_amd import kernels as kn
+    w = torch.cat([torch.linspace(-13, 13, 2001), torch.linspace(-1.2, 1.2, 1001), torch.logspace(-30, 30, 301), -torch.logspace(-30, 0, 301), torch.zeros(1)])
+    N = w.numel()
+    qx, sx = kn.quantize_rows(torch.ones(M, 8, device="cuda"))
+    qw, sw = kn.quantize_rows(torch.full((N, 8), 1.0, device="cuda"))
+    qx[:, 1:] = 0                                                     # one product of 127 127
+    bias = w.cuda() - (127.0 * 127.0 * sx[0] * sw)                   # y = one product + bias
+    y = torch.addcmul(bias.double(), torch.full((), 127.0 * 127.0, dtype=torch.float64, device="cuda"), sx[0].double() * sw.double())
+    for out in (torch.float32, torch.bfloat16):
+        got = kn.gemm_i8(qx, sx, qw, sw, torch.empty(M, N, dtype=out, device="cuda"), bias, True)
+        assert (got == got[0]).all()
+        plainly = kn.gemm_i8(qx, sx, qw, sw, torch.empty(M, N, device="cuda"), bias, False)[0].double()      # the argument as the epilogue has it
+        assert ((plainly - y).abs() <= 4 * H * (1 + y.abs())).all()
+        z = plainly
+        want = z * 0.5 * torch.special.erfc(-z / 2 ** 0.5)
+        rel = H * (10 + 3 * z * z) if out == torch.float32 else 2.4e-5 + H * (10 + 4 * z * z) + torch.finfo(out).eps / 2
+        assert ((got[0].double() - want).abs() <= rel * want.abs() + 1e-37).all(), (((got[0].double() - want).abs()) / (rel * want.abs() + 1e-37)).max().item()
+        edge = torch.tensor([float("inf"), float("-inf"), float("nan"), 3e38, -3e38], device="cuda")
+        got = kn.gemm_i8(qx, sx, qw[:5], sw[:5], torch.empty(M, 5, dtype=out, device="cuda"), edge, True)[M - 1]
+        assert got[0] == float("inf") and got[1] == 0 and torch.isnan(got[2]) and got[3] > 2.9e38 and got[4] == 0
