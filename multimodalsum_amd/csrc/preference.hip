@@ -116,6 +116,11 @@ __device__ __forceinline__ float policy_weight(const PolicyArgs& p, int row, int
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
     return 1.f / (fmaxf((float)n, 1.f) * (p.seq_mean ? (float)p.N : 1.f));
 }
+// e^g - 1 - g, g^2 / 2 near 0: by its series there (to g^9 at 1/2, 2e-9), where the difference has no digits left
+__device__ __forceinline__ float exp_rest(float g, float expm1_g) {
+    const float s = fmaf(g, fmaf(g, fmaf(g, fmaf(g, fmaf(g, fmaf(g, fmaf(g, 1.f / 362880, 1.f / 40320), 1.f / 5040), 1.f / 720), 1.f / 120), 1.f / 24), 1.f / 6), 0.5f);
+    return fabsf(g) < 0.5f ? g * g * s : expm1_g - g;
+}
 // loss = max(-A r, -A clip(r, lo, hi)) + kl (e^d - d - 1) with r = exp(log p - old), d = ref - log p; returns dL / d log p.
 // The bounded branch carries no gradient; the KL estimate (non-negative, unbiased under the sampling policy) gives 1 - e^d.
 __device__ __forceinline__ float policy_token(const PolicyArgs& p, int row, float lp, float w, float (&t)[3]) {
@@ -125,10 +130,10 @@ __device__ __forceinline__ float policy_token(const PolicyArgs& p, int row, floa
     float loss = l1 >= l2 ? l1 : l2, d = l1 >= l2 ? l1 : 0.f, kl = 0.f;
     if (l1 != l1 || l2 != l2) loss = d = l1 + l2;                        // NaN in, NaN out: a comparison would lose it
     if (p.ref_logp != nullptr) {
-        const float g = p.ref_logp[row] - lp, e = expf(g);
-        kl = expm1f(g) - g;
+        const float g = p.ref_logp[row] - lp, e1 = expm1f(g);
+        kl = exp_rest(g, e1);
         loss += p.kl_coef * kl;
-        d += p.kl_coef * (1.f - e);
+        d -= p.kl_coef * e1;
     }
     t[0] = w * loss;
     t[1] = w * kl;

@@ -85,3 +85,26 @@ def test_gelu_of_the_8bit_linear_layer(M):
         edge = torch.tensor([float("inf"), float("-inf"), float("nan"), 3e38, -3e38], device="cuda")
         got = kn.gemm_i8(qx, sx, qw[:5], sw[:5], torch.empty(M, 5, dtype=out, device="cuda"), edge, True)[M - 1]
         assert got[0] == float("inf") and got[1] == 0 and torch.isnan(got[2]) and got[3] > 2.9e38 and got[4] == 0
+
+
+def test_kl_estimate_and_its_gradient_near_zero():
+    """d = ref - logp from 1e-7 to 30, both signs: e^d - d - 1 and 1 - e^d keep their digits (an f32 difference of e^d and 1 has none left at 1e-7).
+
+    d is rounded once (H; exact below 2^-24 of its parts), d^2 / 2 doubles that; the series or e^d - 1 and a difference from 1/2 on, where the result is
+    a quarter of its parts: 16 H in all; beyond 1, d e^d / (e^d - 1) H more for d's own rounding."""
+    from multimodalsum_amd import kernels as kn
+    size = torch.logspace(-7, 1.4, 500)
+    d = torch.cat([size, -size, torch.tensor([0.0, 0.5, -0.5])])
+    N = d.numel()
+    labels, adv = torch.zeros(N, 1, dtype=torch.int64, device="cuda"), torch.zeros(N, device="cuda")
+    ref = d.cuda().view(N, 1)
+    logp = torch.zeros(N, 1, device="cuda")                           # d is ref itself
+    out, coef = kn.policy_terms(logp, labels, logp, adv, ref, 5, 0.2, 0.2, 1.0, "sequence")
+    g = ref.double().view(-1)
+    want = -torch.expm1(g) / N
+    assert ((coef.double().view(-1) - want).abs() <= (16 + 2 * g.abs()) * H * want.abs()).all()
+    for i in range(0, N, 10):                                          # the estimates one by one
+        out, _ = kn.policy_terms(logp[:1], labels[:1], logp[:1], adv[:1], ref[i:i + 1], 5, 0.2, 0.2, 0.5, "sequence")
+        z = g[i].item()
+        kl = torch.expm1(g[i]).item() - z if abs(z) > 1e-2 else z * z / 2 + z ** 3 / 6 + z ** 4 / 24 + z ** 5 / 120 + z ** 6 / 720
+        assert abs(out[1].item() - kl) <= (16 + 2 * abs(z)) * H * kl and abs(out[0].item() - 0.5 * kl) <= (18 + 2 * abs(z)) * H * kl, (z, out[1].item(), kl)
