@@ -132,8 +132,10 @@ __device__ __forceinline__ float policy_token(const PolicyArgs& p, int row, floa
     if (p.ref_logp != nullptr) {
         const float g = p.ref_logp[row] - lp, e1 = expm1f(g);
         kl = exp_rest(g, e1);
-        loss += p.kl_coef * kl;
-        d -= p.kl_coef * e1;
+        if (p.kl_coef != 0.f) {                                          // else only reported: an estimate past f32 stays out of the loss
+            loss += p.kl_coef * kl;
+            d -= p.kl_coef * e1;
+        }
     }
     t[0] = w * loss;
     t[1] = w * kl;

@@ -37,8 +37,8 @@ def preference_loss_and_grad(logits, labels, ref_logps=None, *, beta=0.1, label_
 def policy_loss_and_grad(logits, labels, old_logps, advantages, ref_logps=None, *, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="token", dlogits=None):
     """Clipped policy loss of sampled sequences and its gradient, the logits read once:
     token loss = max(-A r, -A clip(r, 1 - clip_low, 1 + clip_high)) + kl_coef (e^d - d - 1), r = exp(logp - old_logps), d = ref_logps - logp;
-    the mean over all counted tokens ("token") or over the sequences' means ("sequence").  old_logps, ref_logps f32 [N, T], advantages f32 [N] or
-    [N, T].  -> (loss, mean KL estimate, share of clipped tokens, logp [N, T], dlogits)."""
+    the mean over all counted tokens ("token") or over the sequences' means ("sequence"); with kl_coef 0 the KL estimate is only reported.
+    old_logps, ref_logps f32 [N, T], advantages f32 [N] or [N, T].  -> (loss, mean KL estimate, share of clipped tokens, logp [N, T], dlogits)."""
     out, logp, dlogits = kn.policy_loss(logits.detach(), labels, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction, dlogits)
     loss, kl, clipped = out.unbind(0)
     return loss, kl, clipped, logp, dlogits

@@ -108,3 +108,21 @@ def test_kl_estimate_and_its_gradient_near_zero():
         z = g[i].item()
         kl = torch.expm1(g[i]).item() - z if abs(z) > 1e-2 else z * z / 2 + z ** 3 / 6 + z ** 4 / 24 + z ** 5 / 120 + z ** 6 / 720
         assert abs(out[1].item() - kl) <= (16 + 2 * abs(z)) * H * kl and abs(out[0].item() - 0.5 * kl) <= (18 + 2 * abs(z)) * H * kl, (z, out[1].item(), kl)
+
+
+def test_kl_without_a_coefficient_is_only_reported():
+    """kl_coef = 0 with a reference that disagrees by more than e^88 on a token: the estimate is infinite, loss and gradient do not know of it."""
+    import multimodalsum_amd as mm
+    x = torch.randn(2, 3, 40, generator=torch.Generator().manual_seed(0)).cuda()
+    labels, adv = torch.zeros(2, 3, dtype=torch.int64, device="cuda"), torch.tensor([1.0, -1.0], device="cuda")
+    x[0, 1, 0] = -300.0
+    old = mm.sequence_logprobs(x, labels)[1] - 0.1
+    ref = old.clone()
+    ref[0, 1], ref[1, 2] = -1.0, float("-inf")
+    plain = mm.policy_loss_and_grad(x, labels, old, adv)
+    got = mm.policy_loss_and_grad(x, labels, old, adv, ref)
+    assert torch.equal(got[0], plain[0]) and torch.equal(got[4], plain[4]) and got[1] == float("inf") and torch.isfinite(got[4]).all()
+    xg = x.clone().requires_grad_(True)
+    loss = mm.ClippedPolicyLoss()(xg, labels, old, adv, ref)
+    loss.backward()
+    assert torch.isfinite(loss) and torch.isfinite(xg.grad).all()
