@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const int64_t* __restric
     constexpr int ROWS = kFwdRows;
     const int tpr = 1 << tpr_log2, rpb = 256 >> tpr_log2;
     const int c0 = ((int)threadIdx.x & (tpr - 1)) * VEC;
-    const long r0 = (long)blockIdx.x * (rpb * ROWS) + (threadIdx.x >> tpr_log2);
+    const long r0 = block_index() * (rpb * ROWS) + (threadIdx.x >> tpr_log2);
     int64_t id[ROWS];
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) id[j] = r0 + j * rpb < n ? ids[r0 + j * rpb] : -1;
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256) void embed_bwd_few_kernel(const T* __restrict_
     __shared__ uint16_t list[kRowsMax][kFew];                          // positions of a row
     __shared__ int at[kRowsMax][R * 4], count[kRowsMax];               // of a round and wave: entries of a row, then those in front of them
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const long v0 = ((long)blockIdx.y * gridDim.x + blockIdx.x) * rows;
+    const long v0 = block_index() * rows;
     if (v0 >= V) return;
     const int here = (int)(V - v0 < rows ? V - v0 : rows);
     int64_t all[R];
@@ -338,8 +338,7 @@ int embed_bwd_few(const void* dy, long lddy, const int64_t* ids, int n, int V, i
     const int rows = D <= 2048 / kRowsMax ? kRowsMax : D <= 1024 ? 2 : 1, steps = vec ? D / 4 : D;
     int lg = 0;
     while ((1 << lg) < steps && lg < 8) ++lg;
-    const long ranges = (V + (long)rows - 1) / rows, wide = ranges < 1 << 20 ? ranges : 1 << 20;
-    const dim3 grid((unsigned)wide, (unsigned)((ranges + wide - 1) / wide));      // (an axis has up to 2^32 threads)
+    const dim3 grid = grid_of((V + (long)rows - 1) / rows);
     if (vec) hipLaunchKernelGGL((embed_bwd_few_kernel<T, 4>), grid, dim3(256), 0, s, (const T*)dy, lddy, ids, n, V, D, scale, pad_id, accumulate, dE, rows, lg);
     else hipLaunchKernelGGL((embed_bwd_few_kernel<T, 1>), grid, dim3(256), 0, s, (const T*)dy, lddy, ids, n, V, D, scale, pad_id, accumulate, dE, rows, lg);
     return ok();
@@ -401,7 +400,7 @@ __global__ __launch_bounds__(256) void stretch_sum_kernel(const T* __restrict__ 
     const int lane = threadIdx.x & 63;
     // the column blocks of a stretch on neighbouring waves: the rows' halves are asked for together
     const int cols = (D + kCols - 1) / kCols;
-    const long idx = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long idx = block_index() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long st = idx / cols, lo = st * sl;
     if (lo >= n) return;
     const int len = (int)(n - lo < sl ? n - lo : sl);
@@ -481,10 +480,13 @@ __device__ __forceinline__ void clear_absent(const uint32_t* __restrict__ keys, 
 template <bool VEC>
 __global__ __launch_bounds__(256) void stretch_join_kernel(const uint32_t* __restrict__ keys, int n, int sl, int V, int D, float scale, int accumulate, const float* __restrict__ part,
                                                            float* __restrict__ dE, int joins) {
-    if ((int)blockIdx.x >= joins) return clear_absent(keys, n, V, D, dE, ((long)((int)blockIdx.x - joins) * 4 + (threadIdx.x >> 6)) * 16);
+    if (block_index() >= joins) {
+        if (!accumulate) clear_absent(keys, n, V, D, dE, ((block_index() - joins) * 4 + (threadIdx.x >> 6)) * 16);
+        return;
+    }
     constexpr int AHEAD = 16;
     const int lane = threadIdx.x & 63;
-    const long st = blockIdx.x, begin = st * sl, end = begin + sl;      // end < n: the grid leaves the last stretch out
+    const long st = block_index(), begin = st * sl, end = begin + sl;      // end < n: the grid leaves the last stretch out
     // five keys at once: the last of the stretch and the first behind it, the first and the one in front, the next stretch's last
     const uint32_t key = keys[end - 1], behind = keys[end], first = keys[begin], front = keys[begin > 0 ? begin - 1 : 0];
     long b = end + sl < n ? end + sl : n;
@@ -543,9 +545,9 @@ int embed_fwd_t(const int64_t* ids, const void* E, long lde, void* y, long ldy, 
     int lg = 0;
     while ((1 << lg) < steps && lg < 8) ++lg;
     const long blocks = (n + kFwdRows * (256 >> lg) - 1) / (kFwdRows * (256 >> lg));
-    if (blocks > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
-    if (vec) hipLaunchKernelGGL((embed_fwd_kernel<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, ids, (const T*)E, lde, (T*)y, ldy, n, V, D, scale, lg);
-    else hipLaunchKernelGGL((embed_fwd_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, s, ids, (const T*)E, lde, (T*)y, ldy, n, V, D, scale, lg);
+    if (blocks > 1L << 36) return MMSUM_ERR_BAD_SHAPE;               // (the second axis holds 2^15 rows of workgroups)
+    if (vec) hipLaunchKernelGGL((embed_fwd_kernel<T, VEC>), grid_of(blocks), dim3(256), 0, s, ids, (const T*)E, lde, (T*)y, ldy, n, V, D, scale, lg);
+    else hipLaunchKernelGGL((embed_fwd_kernel<T, 1>), grid_of(blocks), dim3(256), 0, s, ids, (const T*)E, lde, (T*)y, ldy, n, V, D, scale, lg);
     return ok();
 }
 
@@ -589,12 +591,13 @@ int embed_bwd_t(const void* dy, long lddy, const int64_t* ids, int n, int V, int
     const long stretches = ((long)n + sl - 1) / sl;
     const long waves = stretches * ((D + kCols - 1) / kCols);
     const bool vec = D % 8 == 0 && lddy % (16 / (int)sizeof(T)) == 0 && (((uintptr_t)dy | (uintptr_t)dE) & 15) == 0;
-    const dim3 grid((unsigned)((waves + 3) / 4));
+    const dim3 grid = grid_of((waves + 3) / 4);
     if (vec) hipLaunchKernelGGL((stretch_sum_kernel<T, true>), grid, dim3(256), 0, s, (const T*)dy, lddy, k0, p0, n, sl, V, D, scale, accumulate, part, dE);
     else hipLaunchKernelGGL((stretch_sum_kernel<T, false>), grid, dim3(256), 0, s, (const T*)dy, lddy, k0, p0, n, sl, V, D, scale, accumulate, part, dE);
     const long joins = ((long)n - 1) / sl;                    // stretches with another one behind them
-    const dim3 jg((unsigned)(joins + (accumulate ? 0 : (V + 63L) / 64)));
-    if (jg.x == 0) return ok();
+    const long jn = joins + (accumulate ? 0 : (V + 63L) / 64);
+    if (jn == 0) return ok();
+    const dim3 jg = grid_of(jn);
     if (vec) hipLaunchKernelGGL((stretch_join_kernel<true>), jg, dim3(256), 0, s, k0, n, sl, V, D, scale, accumulate, part, dE, (int)joins);
     else hipLaunchKernelGGL((stretch_join_kernel<false>), jg, dim3(256), 0, s, k0, n, sl, V, D, scale, accumulate, part, dE, (int)joins);
     return ok();

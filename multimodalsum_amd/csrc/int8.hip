@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t wave_top(uint32_t t) {
 template <typename T, int CH>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, long ldx, int M, int K, int8_t* __restrict__ q, long ldq, float* __restrict__ scale) {
     const int lane = threadIdx.x & 63;
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long row = block_index() * 4 + (threadIdx.x >> 6);
     if (row >= M) return;
     float f[CH][8];
     uint32_t top = 0;
@@ -99,9 +99,10 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, 
 }
 // longer rows: a workgroup a row, read twice
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_long_kernel(const T* __restrict__ x, long ldx, int K, int8_t* __restrict__ q, long ldq, float* __restrict__ scale) {
+__global__ __launch_bounds__(256) void quantize_long_kernel(const T* __restrict__ x, long ldx, int M, int K, int8_t* __restrict__ q, long ldq, float* __restrict__ scale) {
     __shared__ uint32_t sh[4];
-    const long row = blockIdx.x;
+    const long row = block_index();
+    if (row >= M) return;
     const int tid = threadIdx.x;
     uint32_t top = 0;
     for (int k = tid * 8; k < K; k += 2048) {
@@ -123,14 +124,14 @@ __global__ __launch_bounds__(256) void quantize_long_kernel(const T* __restrict_
 }
 template <typename T>
 int launch_quantize(const void* x, long ldx, int M, int K, void* q, long ldq, float* scale, hipStream_t s) {
-    const dim3 grid((unsigned)((M + 3L) / 4));
+    const dim3 grid = grid_of((M + 3L) / 4);
     const T* const xt = static_cast<const T*>(x);
     int8_t* const qt = static_cast<int8_t*>(q);
     if (ldq <= 512) hipLaunchKernelGGL((quantize_kernel<T, 1>), grid, dim3(256), 0, s, xt, ldx, M, K, qt, ldq, scale);
     else if (ldq <= 1024) hipLaunchKernelGGL((quantize_kernel<T, 2>), grid, dim3(256), 0, s, xt, ldx, M, K, qt, ldq, scale);
     else if (ldq <= 2048) hipLaunchKernelGGL((quantize_kernel<T, 4>), grid, dim3(256), 0, s, xt, ldx, M, K, qt, ldq, scale);
     else if (ldq <= 4096) hipLaunchKernelGGL((quantize_kernel<T, 8>), grid, dim3(256), 0, s, xt, ldx, M, K, qt, ldq, scale);
-    else hipLaunchKernelGGL((quantize_long_kernel<T>), dim3(M), dim3(256), 0, s, xt, ldx, K, qt, ldq, scale);
+    else hipLaunchKernelGGL((quantize_long_kernel<T>), grid_of(M), dim3(256), 0, s, xt, ldx, M, K, qt, ldq, scale);
     return ok();
 }
 
@@ -623,18 +624,22 @@ int cu_count() {
     return v & ~7;
 }
 
+constexpr long kMaxGroups = 0xffffff;        // workgroups of 256 threads that an axis of a launch holds; products beyond (few rows, 2^29 columns and more) are refused
 template <typename T, bool GELU, int MB, int NB, bool FUSED, typename X>
 int launch_few(const I8Args& p, const X* x, long ldx, int Kx, hipStream_t s) {
+    const long blocks = (p.N + 16L * NB - 1) / (16 * NB);
+    if (blocks > kMaxGroups) return MMSUM_ERR_BAD_SHAPE;
     const size_t lds = 4 * 16 * MB * (16 * NB + 4) * 4 + 64 * MB + (FUSED ? (size_t)p.M * (p.K + 16) : 0);
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_few_kernel<T, GELU, MB, NB, FUSED, X>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
         return MMSUM_ERR_HIP;
-    hipLaunchKernelGGL((gemm_i8_few_kernel<T, GELU, MB, NB, FUSED, X>), dim3((unsigned)((p.N + 16L * NB - 1) / (16 * NB))), dim3(256), lds, s, p, x, ldx, Kx);
+    hipLaunchKernelGGL((gemm_i8_few_kernel<T, GELU, MB, NB, FUSED, X>), dim3((unsigned)blocks), dim3(256), lds, s, p, x, ldx, Kx);
     return ok();
 }
 
 template <typename T, bool GELU, int BM, int BN, int WM, int WN, int NST>
 int launch_ring(const I8Args& p, hipStream_t s) {
     const long tiles = (p.M + (long)BM - 1) / BM * ((p.N + (long)BN - 1) / BN);
+    if (tiles > kMaxGroups) return MMSUM_ERR_BAD_SHAPE;
     const size_t lds = (size_t)NST * (BM + BN) * 128;
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_ring_kernel<T, GELU, BM, BN, WM, WN, NST>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
         return MMSUM_ERR_HIP;

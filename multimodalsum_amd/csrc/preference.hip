@@ -144,7 +144,7 @@ __device__ __forceinline__ float policy_token(const PolicyArgs& p, int row, floa
 }
 
 template <typename T> struct RowArgs {
-    const T* logits; long ld; const int64_t* labels; int V;
+    const T* logits; long ld; const int64_t* labels; int R, V;
     float* logp; float* stats;      // stats [R][2] = {m, s}; may be NULL
     T* dlogits; long ldd; int W;
     int past;                       // rows below it are read past the caches
@@ -166,7 +166,8 @@ template <int MAXC> __device__ __forceinline__ void keep_packed(u32x4_t (&reg)[M
 template <typename T, int NT, int MAXC, bool POLICY>
 __global__ __launch_bounds__(NT, NT == 512 && !POLICY ? 6 : 4) void row_kernel(RowArgs<T> a) {
     __shared__ float sh[2][NT / 64];
-    const int tid = threadIdx.x, row = blockIdx.x;
+    if (block_index() >= a.R) return;
+    const int tid = threadIdx.x, row = (int)block_index();
     const int64_t y = a.labels[row];
     T* const d = POLICY ? a.dlogits + (long)row * a.ldd : nullptr;
     if (y < 0 || y >= a.V) {
@@ -260,7 +261,8 @@ template <typename T, bool POLICY>
 __global__ __launch_bounds__(1024) void long_row_kernel(RowArgs<T> a) {
     constexpr int NT = 1024;
     __shared__ float sh[2][NT / 64];
-    const int tid = threadIdx.x, row = blockIdx.x;
+    if (block_index() >= a.R) return;
+    const int tid = threadIdx.x, row = (int)block_index();
     const int64_t y = a.labels[row];
     T* const d = POLICY ? a.dlogits + (long)row * a.ldd : nullptr;
     const long R = (long)a.pol.N * a.pol.T;
@@ -333,8 +335,9 @@ __device__ __forceinline__ void sequence_sum(const float* __restrict__ logp, con
     for (int o = 32; o > 0; o >>= 1) cnt += __shfl_xor(cnt, o);
 }
 __global__ __launch_bounds__(256) void sequence_sum_kernel(const float* logp, const int64_t* labels, int N, int T, int V, int average, float* out) {
-    const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (n >= N) return;
+    const long nl = block_index() * 4 + (threadIdx.x >> 6);
+    if (nl >= N) return;
+    const int n = (int)nl, lane = threadIdx.x & 63;
     double s;
     int cnt;
     sequence_sum(logp, labels, n, T, V, lane, s, cnt);
@@ -380,7 +383,8 @@ __global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
     __shared__ double sh[16];
     const int lane = threadIdx.x & 63, waves = blockDim.x / 64;
     double mean = 0.0;
-    for (int p = blockIdx.x * waves + (threadIdx.x >> 6); p < a.P; p += gridDim.x * waves) {
+    for (long pl = block_index() * waves + (threadIdx.x >> 6); pl < a.P; pl += (long)gridDim.x * gridDim.y * waves) {
+        const int p = (int)pl;
         const PairTerms t = pair_terms(a, p, lane);
         const float l = pair_loss_of(a, t.h);
         mean += l;
@@ -408,9 +412,10 @@ __global__ __launch_bounds__(1024) void pair_kernel(PairArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void logprob_bwd_kernel(const T* logits, long ld, const int64_t* __restrict__ labels, const float* __restrict__ stats,
                                                           const float* __restrict__ coef, int rows_per_coef, const float* __restrict__ alpha, T* dlogits,
-                                                          long ldd, int W, int V) {
+                                                          long ldd, int W, int V, int R) {
     constexpr int NT = 256, U = 4;
-    const int tid = threadIdx.x, row = gridDim.x - 1 - blockIdx.x;
+    if (block_index() >= R) return;
+    const int tid = threadIdx.x, row = R - 1 - (int)block_index();
     const int64_t y = labels[row];
     T* const d = dlogits + (long)row * ldd;
     const T* x = logits + (long)row * ld;
@@ -468,16 +473,17 @@ __global__ __launch_bounds__(1024) void rows_mean_kernel(const float* __restrict
 }
 
 // counts[i]: counted tokens of sequence i (seq) or of the i-th of kCountParts equal stretches of the batch
-__global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ labels, long R, long per, int V, int* __restrict__ counts) {
+__global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ labels, long R, long per, int V, int* __restrict__ counts, long slots) {
     __shared__ int sh[4];
-    const long lo = (long)blockIdx.x * per, hi = lo + per < R ? lo + per : R;
+    if (block_index() >= slots) return;
+    const long lo = block_index() * per, hi = lo + per < R ? lo + per : R;
     int n = 0;
     for (long i = lo + threadIdx.x; i < hi; i += 256) { const int64_t y = labels[i]; n += y >= 0 && y < V; }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = n;
     __syncthreads();
-    if (threadIdx.x == 0) counts[blockIdx.x] = sh[0] + sh[1] + sh[2] + sh[3];
+    if (threadIdx.x == 0) counts[block_index()] = sh[0] + sh[1] + sh[2] + sh[3];
 }
 
 // The policy loss from log-probabilities that are there already (the two-step form): coef per row and the terms
@@ -502,13 +508,14 @@ __global__ __launch_bounds__(256) void policy_terms_kernel(const float* __restri
 // and a BART row (50,265 bf16 logits: 512 threads x 13 chunks, 52 registers; f32: 1024 x 13) is resident as a whole.  Scoring | policy loss, us, against
 // the next larger workgroup: 8,192 x 2,000 8 | 21 (35 | 53), 4,096 x 16,000 24 | 54 (55 | 175), 4,096 x 50,265 88 | 177 (207 | 289).
 template <typename T, bool POLICY>
-int launch_rows(const RowArgs<T>& a, int blocks, hipStream_t s) {
+int launch_rows(const RowArgs<T>& a, hipStream_t s) {
+    const dim3 g = grid_of(a.R);
     const long chunks = ((long)a.V + kPer<T> - 1) / kPer<T>;
-    if (chunks <= 64 * 4) hipLaunchKernelGGL((row_kernel<T, 64, 4, POLICY>), dim3(blocks), dim3(64), 0, s, a);
-    else if (chunks <= 256 * 8) hipLaunchKernelGGL((row_kernel<T, 256, 8, POLICY>), dim3(blocks), dim3(256), 0, s, a);
-    else if (chunks <= 512 * 13) hipLaunchKernelGGL((row_kernel<T, 512, 13, POLICY>), dim3(blocks), dim3(512), 0, s, a);
-    else if (chunks <= 1024 * 13) hipLaunchKernelGGL((row_kernel<T, 1024, 13, POLICY>), dim3(blocks), dim3(1024), 0, s, a);
-    else hipLaunchKernelGGL((long_row_kernel<T, POLICY>), dim3(blocks), dim3(1024), 0, s, a);
+    if (chunks <= 64 * 4) hipLaunchKernelGGL((row_kernel<T, 64, 4, POLICY>), g, dim3(64), 0, s, a);
+    else if (chunks <= 256 * 8) hipLaunchKernelGGL((row_kernel<T, 256, 8, POLICY>), g, dim3(256), 0, s, a);
+    else if (chunks <= 512 * 13) hipLaunchKernelGGL((row_kernel<T, 512, 13, POLICY>), g, dim3(512), 0, s, a);
+    else if (chunks <= 1024 * 13) hipLaunchKernelGGL((row_kernel<T, 1024, 13, POLICY>), g, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((long_row_kernel<T, POLICY>), g, dim3(1024), 0, s, a);
     return ok();
 }
 
@@ -516,24 +523,24 @@ bool bad_rows(long R, int V, long ld) { return R <= 0 || R > 0x7fffffffL || V <=
 bool bad_align(int dtype, const void* p) { return ((uintptr_t)p & (dtype == MMSUM_BF16 ? 1 : 3)) != 0; }
 
 template <typename T>
-RowArgs<T> row_args(const void* logits, long ld, const int64_t* labels, int V, float* logp, float* stats) {
+RowArgs<T> row_args(const void* logits, long ld, const int64_t* labels, int R, int V, float* logp, float* stats) {
     RowArgs<T> a = {};
-    a.logits = static_cast<const T*>(logits); a.ld = ld; a.labels = labels; a.V = V; a.logp = logp; a.stats = stats;
+    a.logits = static_cast<const T*>(logits); a.ld = ld; a.labels = labels; a.R = R; a.V = V; a.logp = logp; a.stats = stats;
     return a;
 }
 
 template <typename T>
 int launch_bwd(const void* logits, long ld, const int64_t* labels, const float* stats, const float* coef, int rows_per_coef, const float* alpha, void* dlogits,
                long ldd, int W, int V, int R, hipStream_t s) {
-    hipLaunchKernelGGL((logprob_bwd_kernel<T>), dim3(R), dim3(256), 0, s, static_cast<const T*>(logits), ld, labels, stats, coef, rows_per_coef, alpha,
-                       static_cast<T*>(dlogits), ldd, W, V);
+    hipLaunchKernelGGL((logprob_bwd_kernel<T>), grid_of(R), dim3(256), 0, s, static_cast<const T*>(logits), ld, labels, stats, coef, rows_per_coef, alpha,
+                       static_cast<T*>(dlogits), ldd, W, V, R);
     return ok();
 }
 
 long count_slots(int N, int seq_mean) { return seq_mean ? N : kCountParts; }
 int launch_counts(const int64_t* labels, int N, int T, int V, int seq_mean, int* counts, hipStream_t s) {
     const long R = (long)N * T, per = seq_mean ? T : (R + kCountParts - 1) / kCountParts;
-    hipLaunchKernelGGL(count_kernel, dim3((unsigned)count_slots(N, seq_mean)), dim3(256), 0, s, labels, R, per, V, counts);
+    hipLaunchKernelGGL(count_kernel, grid_of(count_slots(N, seq_mean)), dim3(256), 0, s, labels, R, per, V, counts, count_slots(N, seq_mean));
     return ok();
 }
 
@@ -543,8 +550,8 @@ extern "C" int mmsum_token_logprob(int dtype, const void* logits, long ld, const
     if (bad_rows(R, V, ld)) return MMSUM_ERR_BAD_SHAPE;
     if (dtype != MMSUM_BF16 && dtype != MMSUM_F32) return MMSUM_ERR_BAD_DTYPE;
     if (any_null(logits, labels, logp) || bad_align(dtype, logits)) return MMSUM_ERR_BAD_ALIGN;
-    if (dtype == MMSUM_BF16) return launch_rows<bf16_t, false>(row_args<bf16_t>(logits, ld, labels, V, logp, stats), R, (hipStream_t)stream);
-    return launch_rows<float, false>(row_args<float>(logits, ld, labels, V, logp, stats), R, (hipStream_t)stream);
+    if (dtype == MMSUM_BF16) return launch_rows<bf16_t, false>(row_args<bf16_t>(logits, ld, labels, R, V, logp, stats), (hipStream_t)stream);
+    return launch_rows<float, false>(row_args<float>(logits, ld, labels, R, V, logp, stats), (hipStream_t)stream);
 }
 
 extern "C" int mmsum_token_logprob_bwd(int dtype, const void* logits, long ld, const int64_t* labels, const float* stats, const float* coef, int rows_per_coef,
@@ -559,7 +566,7 @@ extern "C" int mmsum_token_logprob_bwd(int dtype, const void* logits, long ld, c
 extern "C" int mmsum_sequence_logprob(const float* logp, const int64_t* labels, int N, int T, int V, int average, float* out, void* stream) {
     if (N <= 0 || T <= 0 || V <= 0 || (long)N * T > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
     if (any_null(logp, labels, out)) return MMSUM_ERR_BAD_ALIGN;
-    hipLaunchKernelGGL(sequence_sum_kernel, dim3((N + 3) / 4), dim3(256), 0, (hipStream_t)stream, logp, labels, N, T, V, average, out);
+    hipLaunchKernelGGL(sequence_sum_kernel, grid_of((N + 3L) / 4), dim3(256), 0, (hipStream_t)stream, logp, labels, N, T, V, average, out);
     return ok();
 }
 
@@ -574,7 +581,7 @@ extern "C" int mmsum_preference_pairs(const float* logp, const int64_t* labels, 
         hipLaunchKernelGGL(pair_kernel, dim3(1), dim3(1024), 0, s, a);
     } else {
         a.loss = nullptr;
-        hipLaunchKernelGGL(pair_kernel, dim3((P + 3) / 4), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(pair_kernel, grid_of((P + 3L) / 4), dim3(256), 0, s, a);
         hipLaunchKernelGGL(rows_mean_kernel, dim3(1), dim3(1024), 0, s, pair_loss, (long)P, (long)P, loss);
     }
     return ok();
@@ -599,10 +606,10 @@ extern "C" int mmsum_preference_loss(int dtype, const void* logits, long ld, con
     // gradient taking its pair's sums itself in place of the pairs' launch: 4 x 128 x 1,009 equal, 36 x 128 x 1,009 30 -> 52 us.)
     const auto run = [&](auto of_type) {
         typedef decltype(of_type) T_;
-        RowArgs<T_> a = row_args<T_>(logits, ld, labels, V, logp, stats);
+        RowArgs<T_> a = row_args<T_>(logits, ld, labels, R, V, logp, stats);
         const long keep = (400L << 20) / (ld * (long)sizeof(T_));
         a.past = keep < R ? R - (int)keep : 0;
-        int rc = launch_rows<T_, false>(a, R, s);
+        int rc = launch_rows<T_, false>(a, s);
         if (rc == MMSUM_OK) rc = mmsum_preference_pairs(logp, labels, ref, P, T, V, beta, smoothing, average, seq, margins, pair_loss, coef, loss, stream);
         return rc == MMSUM_OK ? launch_bwd<T_>(logits, ld, labels, stats, coef, T, nullptr, dlogits, ldd, W, V, R, s) : rc;
     };
@@ -659,13 +666,13 @@ extern "C" int mmsum_policy_loss(int dtype, const void* logits, long ld, const i
     else if (rc == MMSUM_OK) rc = launch_counts(labels, N, T, V, seq_mean, const_cast<int*>(p.counts), s);
     if (rc != MMSUM_OK) return rc;
     if (dtype == MMSUM_BF16) {
-        RowArgs<bf16_t> a = row_args<bf16_t>(logits, ld, labels, V, logp, nullptr);
+        RowArgs<bf16_t> a = row_args<bf16_t>(logits, ld, labels, R, V, logp, nullptr);
         a.dlogits = static_cast<bf16_t*>(dlogits); a.ldd = ldd; a.W = W; a.pol = p;
-        rc = launch_rows<bf16_t, true>(a, R, s);
+        rc = launch_rows<bf16_t, true>(a, s);
     } else {
-        RowArgs<float> a = row_args<float>(logits, ld, labels, V, logp, nullptr);
+        RowArgs<float> a = row_args<float>(logits, ld, labels, R, V, logp, nullptr);
         a.dlogits = static_cast<float*>(dlogits); a.ldd = ldd; a.W = W; a.pol = p;
-        rc = launch_rows<float, true>(a, R, s);
+        rc = launch_rows<float, true>(a, s);
     }
     if (rc != MMSUM_OK) return rc;
     hipLaunchKernelGGL(rows_mean_kernel, dim3(3), dim3(1024), 0, s, p.terms, (long)R, 1L, out);

@@ -126,3 +126,72 @@ def test_kl_without_a_coefficient_is_only_reported():
     loss = mm.ClippedPolicyLoss()(xg, labels, old, adv, ref)
     loss.backward()
     assert torch.isfinite(loss) and torch.isfinite(xg.grad).all()
+
+
+def test_more_rows_than_a_grid_axis_holds():
+    """2^26 rows and a few: an axis of a launch holds fewer than 2^32 threads, 2^26 workgroups of one wave, 2^24 of four."""
+    import multimodalsum_amd as mm
+    N, T, V = 2 ** 25 + 6, 2, 2
+    x = torch.zeros(N, T, V, dtype=torch.bfloat16, device="cuda")
+    labels = torch.zeros(N, T, dtype=torch.int64, device="cuda")
+    x[-1, 1, 0], x[-3, 0, 0], x[5, 0, 0] = 2.0, -1.0, 3.0
+    labels[-2] = -100
+    probe = torch.tensor([0, 5, N // 2, N - 3, N - 2, N - 1], device="cuda")
+    lp = torch.log_softmax(x[probe].double(), -1)[..., 0] * (labels[probe] >= 0)
+    seq, tok = mm.sequence_logprobs(x, labels)
+    for got, want in ((tok[probe], lp), (seq[probe], lp.sum(1))):
+        assert ((got.double() - want).abs() <= 8 * H).all()
+    half = torch.tensor(0.5, dtype=torch.float64).log().item()
+    assert (tok[6:N - 3] - half).abs().max() <= 8 * H and (seq[6:N - 3] - 2 * half).abs().max() <= 16 * H
+    P = N // 2
+    loss, margins, d = mm.preference_loss_and_grad(x, labels, beta=0.5)
+    c = (torch.sigmoid(-margins.double()) * 0.5 / P)[torch.arange(N, device="cuda") % P]      # -d loss / d log p of the chosen one
+    c[P:] *= -1
+    assert (margins[6:P - 3] == 0).all() and (loss.double() - torch.nn.functional.softplus(-margins.double()).mean()).abs() <= 8 * H
+    p1 = torch.softmax(x.double(), -1)[..., 1] * (labels >= 0)
+    want = torch.stack([-c[:, None] * p1, c[:, None] * p1], -1)
+    assert ((d.double() - want).abs() <= want.abs() * 2.0 ** -8 * 1.01).all()
+    old, adv = tok, torch.ones(N, device="cuda")
+    for reduction in ("token", "sequence"):
+        l, _, _, tok2, d2 = mm.policy_loss_and_grad(x, labels, old, adv, reduction=reduction)
+        assert torch.equal(tok2, tok)
+        w = torch.full((N, 1), 1.0 / (2 * N - 2) if reduction == "token" else 0.5 / N, dtype=torch.float64, device="cuda")
+        want = torch.stack([-w * p1, w * p1], -1)                   # d loss / d log p = -A w, and the label is 0
+        assert ((d2.double() - want).abs() <= want.abs() * 2.0 ** -8 * 1.01).all()
+        mean = (2 * N - 2) / (2 * N - 2) if reduction == "token" else (N - 1) / N
+        assert abs(l.item() + mean) <= 4 * H
+
+
+def test_more_ids_than_a_grid_axis_holds():
+    import multimodalsum_amd as mm
+    n, V, D = 2 ** 27 + 3, 1000, 129                                 # a workgroup takes eight of these rows
+    table = (torch.arange(V, device="cuda")[:, None] * 0.25 + torch.arange(D, device="cuda") * 0.5).bfloat16()
+    y = mm.scaled_embedding(torch.arange(n, device="cuda") % V, table, 2.0)
+    assert torch.equal(y[:V], table * 2) and torch.equal(y[-V:], (table * 2).roll(-((n - V) % V), 0))
+    for lo in range(0, n, 2 ** 24):
+        k = min(n, lo + 2 ** 24) - lo
+        assert torch.equal(y[lo:lo + k, 77], (table[:, 77] * 2)[(torch.arange(k, device="cuda") + lo) % V])
+    del y
+    torch.cuda.empty_cache()
+    n, V = 2 ** 29 + 5, 4099                                         # 2^24 stretches of 32 sorted positions
+    ids = torch.arange(n, device="cuda") % V
+    got = mm.scaled_embedding_grad(torch.ones(n, 1, dtype=torch.bfloat16, device="cuda"), ids, V, 0.5, padding_idx=7)
+    want = torch.bincount(ids, minlength=V).float() * 0.5            # below 2^24: exact in any order
+    want[7] = 0.0
+    assert torch.equal(got[:, 0], want)
+    del ids
+    torch.cuda.empty_cache()
+
+
+def test_more_tokens_to_quantise_than_a_grid_axis_holds():
+    from multimodalsum_amd import kernels as kn
+    M = 2 ** 26 + 5
+    x = torch.ones(M, 2, device="cuda")
+    x[:, 1] = torch.arange(M, device="cuda") % 101 * 0.01
+    q, s = kn.quantize_rows(x)
+    assert (q[:, 0] == 127).all() and torch.equal(s, torch.full_like(s, 1.0) / 127.0)
+    for lo in range(0, M, 2 ** 24):
+        assert torch.equal(q[lo:lo + 2 ** 24, 1].float(), torch.round(x[lo:lo + 2 ** 24, 1].double() * 127).float())
+    assert not q[-1000:, 2:].any() and not q[:1000, 2:].any()
+    del q, x
+    torch.cuda.empty_cache()
