@@ -593,6 +593,14 @@ def _need(ok, message, *args):
         raise ValueError(message % args)
 
 
+INT_SIZE = 2 ** 31 - 16384         # sizes that the C entries take as int, and round up
+
+
+def _sizes(what, *sizes):
+    for n in sizes:
+        _need(n < INT_SIZE, "%s: a size of %d", what, n)
+
+
 def _device(*tensors):
     index = -1
     for t in tensors:
@@ -633,7 +641,7 @@ def _rows_of(t, what):
     _need(V == 1 or t.stride(2) == 1, "%s: unit inner stride expected", what)
     ld = t.stride(1) if T > 1 else (t.stride(0) if N > 1 else V)
     _need(ld >= V and (N == 1 or t.stride(0) == T * ld), "%s: rows of one pitch expected (strides %s)", what, t.stride())
-    _need(N * T < 2 ** 31, "%s: too many rows", what)
+    _sizes(what, N * T, V)
     return N, T, V, ld
 
 
@@ -716,6 +724,7 @@ def token_logprob_bwd(logits, labels, stats, coef, alpha=None, dlogits=None):
 def sequence_logprob(logp, labels, V, average=False):
     """out f32 [N]: the sum (mean) of every sequence's counted log-probabilities."""
     N, T = logp.shape
+    _sizes("sequence_logprob", N * T, V)
     labels, logp = _labels_of(labels, N, T), _f32_of(logp, (N, T), "logp")
     dev = _device(logp, labels)
     out = torch.empty(N, dtype=torch.float32, device=dev)
@@ -732,6 +741,7 @@ def _pairs_of(N, ref, smoothing):
 def preference_pairs(logp, labels, ref, V, beta, smoothing, average):
     """From log-probabilities -> (loss [], margins [P], sequence log-probabilities [2P], coef [2P])."""
     N, T = logp.shape
+    _sizes("preference_pairs", N * T, V)
     labels, logp = _labels_of(labels, N, T), _f32_of(logp, (N, T), "logp")
     P, ref = _pairs_of(N, ref, smoothing)
     dev = _device(logp, labels, ref)
@@ -771,6 +781,7 @@ def _policy_of(N, T, old, adv, ref, clip_low, clip_high, kl_coef, reduction):
 def policy_terms(logp, labels, old, adv, ref, V, clip_low, clip_high, kl_coef, reduction):
     """From log-probabilities -> (out f32 [3] = loss, KL, clipped share; coef [N, T])."""
     N, T = logp.shape
+    _sizes("policy_terms", N * T, V)
     labels, logp = _labels_of(labels, N, T), _f32_of(logp, (N, T), "logp")
     old, adv, ref = _policy_of(N, T, old, adv, ref, clip_low, clip_high, kl_coef, reduction)
     dev = _device(logp, labels, old, adv, ref)
@@ -830,6 +841,7 @@ def embed_fwd(ids, table, scale=1.0):
     flat, lde = _ids_of(ids).contiguous(), _pitch2(table, "table")
     (V, D), n = table.shape, flat.numel()
     _need(V > 0 and D > 0, "table: empty")
+    _sizes("table", V, D)
     _dt(table)
     dev = _device(ids, table)
     y = torch.empty(*ids.shape, D, dtype=table.dtype, device=dev)
@@ -844,6 +856,7 @@ def embed_bwd(dy, ids, V, scale=1.0, pad_id=None, out=None, accumulate=False):
     D, n = dy.shape[-1], flat.numel()
     _need(dy.shape[:-1] == ids.shape, "dy: shape %s expected, got %s", (*ids.shape, D), dy.shape)
     _need(V > 0 and D > 0 and n < 2 ** 30, "embed_bwd: %d ids into [%d, %d]", n, V, D)
+    _sizes("embed_bwd", V, D)
     pad_id = padding_row(pad_id, V)
     dy = dy.reshape(-1, D)
     if n and ((D > 1 and dy.stride(1) != 1) or (n > 1 and dy.stride(0) < D)):        # a gradient that is one row, repeated, among them
@@ -873,6 +886,7 @@ def quantize_rows(x):
     ldx = _pitch2(x, "x")
     M, K = x.shape
     _need(0 < K <= 131072, "quantize_rows: K = %d, 1 .. 131072 expected", K)
+    _sizes("quantize_rows", M)
     _dt(x)
     dev = _device(x)
     Kp = -(-K // I8_K_STEP) * I8_K_STEP
@@ -889,6 +903,7 @@ def gemm_i8(qx, sx, qw, sw, out, bias=None, gelu=False):
         if t.dtype != torch.int8:
             raise TypeError("%s: int8 expected, got %s" % (what, t.dtype))
     _need(qw.shape[1] == K and K % I8_K_STEP == 0 and 0 < K <= 131072, "gemm_i8: operands as quantize_rows leaves them expected")
+    _sizes("gemm_i8", M, N)
     _need(out.shape == (M, N), "out: shape %s expected, got %s", (M, N), out.shape)
     sx, sw, bias = _f32_of(sx, (M,), "sx"), _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias", optional=True)
     ldx, ldw, ldy = _pitch2(qx, "qx"), _pitch2(qw, "qw"), _pitch2(out, "out")
@@ -907,6 +922,7 @@ def linear_i8(x, qw, sw, out=None, bias=None, gelu=False, out_dtype=None):
     if qw.dtype != torch.int8:
         raise TypeError("qw: int8 expected, got %s" % qw.dtype)
     _need(0 < K <= 131072 and qw.shape[1] == -(-K // I8_K_STEP) * I8_K_STEP, "linear_i8: weights as quantize_rows leaves them expected")
+    _sizes("linear_i8", M, N)
     sw, bias = _f32_of(sw, (N,), "sw"), _f32_of(bias, (N,), "bias", optional=True)
     ldx, ldw, dt = _pitch2(x, "x"), _pitch2(qw, "qw"), _dt(x)
     dev = _device(x, qw, sw, out, bias)

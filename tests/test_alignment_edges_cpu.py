@@ -169,3 +169,32 @@ def test_results_written_into_a_tensor_count_as_changes_in_place(monkeypatch):
     with torch.inference_mode():                                   # tensors without a version
         t = torch.zeros(4, 3, 8)
         mm.preference_loss_and_grad(t, lab, dlogits=t)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Sizes that the C entries take as 32-bit numbers: ctypes would pass their lower halves."""
+    import multimodalsum_amd as mm
+    from multimodalsum_amd import kernels as kn
+
+    def meta(*shape, dtype=torch.float32):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+    big = 2 ** 32 + 5
+    lab1 = meta(2, 1, dtype=torch.int64)
+    refused(ValueError, mm.sequence_logprobs, meta(2, 1, big), lab1)
+    refused(ValueError, mm.sequence_logprobs, meta(big, 1, 5), meta(big, 1, dtype=torch.int64))
+    refused(ValueError, mm.preference_loss_and_grad, meta(2, 1, 5), lab1, dlogits=meta(2, 1, big))
+    refused(ValueError, kn.sequence_logprob, meta(2, 1), lab1, big)
+    refused(ValueError, kn.sequence_logprob, meta(big, 1), meta(big, 1, dtype=torch.int64), 5)
+    refused(ValueError, kn.preference_pairs, meta(2 * big, 1), meta(2 * big, 1, dtype=torch.int64), None, 5, 0.1, 0.0, False)
+    refused(ValueError, kn.policy_terms, meta(big, 1), meta(big, 1, dtype=torch.int64), meta(big, 1), meta(big), None, 5, 0.2, 0.2, 0.0, "token")
+    ids = meta(3, dtype=torch.int64)
+    refused(ValueError, mm.scaled_embedding, ids, meta(big, 2))
+    refused(ValueError, mm.scaled_embedding, ids, meta(2, big))
+    refused(ValueError, mm.scaled_embedding_grad, meta(3, 2), ids, big)
+    refused(ValueError, mm.scaled_embedding_grad, meta(3, big), ids, 2)
+    refused(ValueError, kn.quantize_rows, meta(big, 2))
+    q, s = meta(4, 128, dtype=torch.int8), meta(4)
+    refused(ValueError, kn.gemm_i8, meta(big, 128, dtype=torch.int8), meta(big), q, s, meta(big, 4))
+    refused(ValueError, kn.gemm_i8, q, s, meta(big, 128, dtype=torch.int8), meta(big), meta(4, big))
+    refused(ValueError, kn.linear_i8, meta(big, 128), q, s)
+    refused(ValueError, kn.linear_i8, meta(4, 128), meta(big, 128, dtype=torch.int8), meta(big))
