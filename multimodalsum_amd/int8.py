@@ -10,8 +10,9 @@ from . import kernels as kn
 
 class Int8Linear(nn.Module):
     """y = x W^T (+ bias) (then GELU, erf form) with W [N, K] (f32 or bf16) held as int8 [N, Kp] + one f32 scale per row.  x [..., K] f32 or bf16,
-    y [..., N] in out_dtype (default: x's).  A token whose values are not all finite gives NaN.  No gradient: inputs that require one, or carry a
-    forward-mode tangent, are refused."""
+    y [..., N] in out_dtype (default: x's).  A token whose values are not all finite gives NaN.
+    Casts of a module around it (.bfloat16(), .to(dtype)) leave its scales and bias f32.  A state dict is loaded by a layer of the same sizes (made from
+    zeros, say).  No gradient: inputs that require one, or carry a forward-mode tangent, are refused."""
 
     def __init__(self, weight, bias=None, gelu=False, out_dtype=None):
         super().__init__()
@@ -27,6 +28,16 @@ class Int8Linear(nn.Module):
         self.register_buffer("qweight", q)
         self.register_buffer("scale", scale)
         self.register_buffer("bias", None if bias is None else bias.detach().to(torch.float32).clone())
+
+    def _apply(self, fn, recurse=True):
+        """Scales and bias are f32 whatever type the model around them is cast to: only the device follows."""
+        kept = {n: getattr(self, n) for n in ("scale", "bias") if getattr(self, n) is not None}
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            moved = getattr(self, name)
+            if moved.dtype != torch.float32:
+                setattr(self, name, t.to(moved.device))
+        return self
 
     @classmethod
     def from_linear(cls, linear, **kw):

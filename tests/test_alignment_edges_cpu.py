@@ -198,3 +198,44 @@ def test_sizes_past_32_bits_are_refused():
     refused(ValueError, kn.gemm_i8, q, s, meta(big, 128, dtype=torch.int8), meta(big), meta(4, big))
     refused(ValueError, kn.linear_i8, meta(big, 128), q, s)
     refused(ValueError, kn.linear_i8, meta(4, 128), meta(big, 128, dtype=torch.int8), meta(big))
+
+
+def quantised(*a):
+    """mmsum_quantize_i8 on the CPU."""
+    x, M, K, q, scale = a[1].detach().double(), a[3], a[4], a[5], a[7]
+    top = x.abs().amax(1)
+    q.zero_()
+    q[:, :K] = torch.nan_to_num(torch.round(x * 127 / top[:, None])).to(torch.int8)
+    scale.copy_((top / 127).float())
+
+
+def test_int8_layer_keeps_its_scales_under_casts(monkeypatch):
+    """model.bfloat16(), .half(), .to(dtype), .double(): scales and bias stay f32, bit for bit; devices still move; the rest of the model is cast."""
+    import multimodalsum_amd as mm
+    rec = Recorder(monkeypatch, {"mmsum_quantize_i8": quantised})
+    w, b = torch.randn(6, 8), torch.randn(6)
+    for cast in (lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(), lambda m: m.to("cpu", torch.bfloat16), lambda m: m.float()):
+        m = torch.nn.Sequential(torch.nn.Linear(3, 8), mm.Int8Linear(w, b))
+        q, s = m[1].qweight.clone(), m[1].scale.clone()
+        kind = cast(torch.nn.Linear(2, 2)).weight.dtype
+        assert cast(m)[0].weight.dtype == kind
+        assert m[1].scale.dtype == m[1].bias.dtype == torch.float32 and torch.equal(m[1].scale, s) and torch.equal(m[1].bias, b) and torch.equal(m[1].qweight, q)
+        x = torch.zeros(2, 8, dtype=torch.bfloat16)
+        assert m[1](x).dtype == torch.bfloat16 and rec.calls[-1][0] == "mmsum_linear_i8"
+    m = mm.Int8Linear(w).bfloat16()
+    assert m.bias is None and m.scale.dtype == torch.float32
+    moved = mm.Int8Linear(w, b).to("meta")
+    assert moved.scale.device.type == moved.bias.device.type == moved.qweight.device.type == "meta" and moved.scale.dtype == torch.float32
+    back = moved.to_empty(device="cpu")
+    assert back.scale.device.type == back.bias.device.type == "cpu" and back.scale.dtype == torch.float32
+
+
+def test_int8_layer_from_its_state_dict(monkeypatch):
+    """A saved layer without its float weights: a layer of the same sizes, made from zeros, loads it."""
+    import multimodalsum_amd as mm
+    Recorder(monkeypatch, {"mmsum_quantize_i8": quantised})
+    for bias in (None, torch.randn(6)):
+        saved = mm.Int8Linear(torch.randn(6, 8), bias).state_dict()
+        again = mm.Int8Linear(torch.zeros(6, 8), None if bias is None else torch.zeros(6)).bfloat16()
+        again.load_state_dict(saved)
+        assert again.state_dict().keys() == saved.keys() and all(torch.equal(v, saved[k]) and v.dtype == saved[k].dtype for k, v in again.state_dict().items())

@@ -195,3 +195,12 @@ def test_more_tokens_to_quantise_than_a_grid_axis_holds():
     assert not q[-1000:, 2:].any() and not q[:1000, 2:].any()
     del q, x
     torch.cuda.empty_cache()
+
+
+def test_int8_layer_in_a_model_that_is_cast():
+    import multimodalsum_amd as mm
+    lin = mm.Int8Linear(torch.randn(40, 24, device="cuda"), torch.randn(40, device="cuda"), out_dtype=torch.float32)
+    x = torch.randn(5, 24, device="cuda").bfloat16()
+    want = lin(x)
+    model = torch.nn.Sequential(torch.nn.Linear(24, 24, device="cuda"), lin).bfloat16()
+    assert model[0].weight.dtype == torch.bfloat16 and torch.equal(model[1](x), want)
