@@ -472,6 +472,14 @@ int mmsum_gemm_i8(const void* qx, long ldx, const float* sx, const void* qw, lon
 long mmsum_linear_i8_workspace(int M, int K);
 int mmsum_linear_i8(int dtype, const void* x, long ldx, const void* qw, long ldw, const float* sw, const float* bias, int dtype_out, void* y, long ldy, int M,
                     int N, int K, int gelu, void* workspace, void* stream);
+/* What mmsum_linear_i8 (quantise != 0) or mmsum_gemm_i8 (0: K a multiple of 128) would launch for the product (pure: no device work): plan[0] = kernel,
+ * plan[1] x plan[2] = tile (few rows: the rows and columns of a workgroup), plan[3] = workgroups (fewer than tiles: they walk the tile list).
+ * Tests use it to assert that a shape reaches the kernel they mean to cover. */
+enum { MMSUM_I8_PLAN_FEW = 0,              /* gemm_i8_few_kernel: up to 64 rows, the weights streamed past the matrix cores */
+       MMSUM_I8_PLAN_FEW_QUANTISING = 1,   /* the same, quantising the rows inside */
+       MMSUM_I8_PLAN_RING = 2,             /* gemm_i8_ring_kernel: a tile a workgroup, 64x64 or 192x128 */
+       MMSUM_I8_PLAN_W4 = 3 };             /* gemm_i8_w4_kernel: 256x256 tiles, four waves, one stream of stages */
+int mmsum_linear_i8_plan(int M, int N, int K, int gelu, int quantise, int* plan);
 
 #pragma GCC visibility pop
 #ifdef __cplusplus

@@ -19,6 +19,7 @@ GEMM_A_T, GEMM_B_T, GEMM_BIAS = 0x1, 0x2, 0x4
 EPI_NONE, EPI_GELU, EPI_GELU_BWD, EPI_RELU, EPI_RELU_BWD = 0, 1, 2, 3, 4
 GEMM_ACCUM, GEMM_OUT_F32, GEMM_SLABS, GEMM_COLSUM, GEMM_COLSUM2, GEMM_A_F32 = 0x40, 0x80, 0x100, 0x200, 0x400, 0x800
 PLAN_GENERIC, PLAN_NT_RING, PLAN_TN_RING, PLAN_SKINNY = 0, 1, 2, 3
+I8_PLAN_FEW, I8_PLAN_FEW_QUANTISING, I8_PLAN_RING, I8_PLAN_W4 = 0, 1, 2, 3
 ABI_VERSION = 10
 
 
@@ -139,6 +140,7 @@ SIGNATURES = {
     "mmsum_gemm_i8": (c_int, [c_void_p, c_long, c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_int, c_void_p, c_long, c_int, c_int, c_int, c_int, c_void_p]),
     "mmsum_linear_i8_workspace": (c_long, [c_int, c_int]),
     "mmsum_linear_i8": (c_int, [c_int, c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_int, c_void_p, c_long] + [c_int] * 4 + [c_void_p, c_void_p]),
+    "mmsum_linear_i8_plan": (c_int, [c_int] * 5 + [ctypes.POINTER(c_int)]),
 }
 
 

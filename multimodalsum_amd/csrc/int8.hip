@@ -647,15 +647,15 @@ int launch_ring(const I8Args& p, hipStream_t s) {
     return ok();
 }
 
-template <typename T, bool GELU>
-int launch_product(const I8Args& p, hipStream_t s) {
-    if (p.M <= 64) {
+// The kernel of a product: family, tile (few rows: rows and columns of a workgroup), workgroups
+struct I8Plan { int kernel, bm, bn; long groups; };
+I8Plan plan_product(int M, int N, int K, bool gelu) {
+    auto up = [](long a, long b) { return (a + b - 1) / b; };
+    if (M <= 64) {
         // Workgroups of 64 columns read the activations less often, of 16 columns fill more CUs (us, 16 | 64 columns, K = 1,024): N = 8,192: 1 row 3.4 | 4.2,
         // 32 rows 4.9 | 5.9; 16,384: 1 row 4.3 | 5.0, 16 rows 5.5 | 5.7, 32 rows 7.8 | 6.1; 50,265: 1 row 10.8 | 10.8, 32 rows 21.5 | 15.9
-        const bool wide = p.N >= (p.M <= 16 ? 32768 : 16384);
-        if (p.M <= 16) return wide ? launch_few<T, GELU, 1, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 1, 1, false, float>(p, nullptr, 0, 0, s);
-        if (p.M <= 32) return wide ? launch_few<T, GELU, 2, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 2, 1, false, float>(p, nullptr, 0, 0, s);
-        return wide ? launch_few<T, GELU, 4, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 4, 1, false, float>(p, nullptr, 0, 0, s);
+        const int bn = N >= (M <= 16 ? 32768 : 16384) ? 64 : 16;
+        return {MMSUM_I8_PLAN_FEW, M <= 16 ? 16 : M <= 32 ? 32 : 64, bn, up(N, bn)};
     }
     // The tile whose rounds of the CUs take the least time, in tenths of a us: so much a stage of 128 k and so much an epilogue, fitted to the
     // three on 24 shapes (worst choice 9 % over the best).  Measured (us, 64x64 | 192x128 | 256x256, bf16 out):
@@ -664,26 +664,39 @@ int launch_product(const I8Args& p, hipStream_t s) {
     //    9,216 x 1,024 x 1,024    23 |  16 |  20                                    2,048 x 2,048 x 2,048    16 |  23 |  19
     //   256 x 50,265 x 1,024      36 |  37 |  27                                      128 x 50,265 x 1,024    21 |  27 |  22
     // The larger tiles are not for fewer than 129 rows: their loads of the missing rows still take their turn.
-    auto up = [](long a, long b) { return (a + b - 1) / b; };
-    const long cus = cu_count(), st = p.K / 128;
-    const long t256 = up(p.M, 256) * up(p.N, 256), t192 = up(p.M, 192) * up(p.N, 128), t64 = up(p.M, 64) * up(p.N, 64);
-    if (t64 > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    const long cus = cu_count(), st = K / 128;
+    const long t256 = up(M, 256) * up(N, 256), t192 = up(M, 192) * up(N, 128), t64 = up(M, 64) * up(N, 64);
     const long half = up(t192, cus);                               // rounds of one workgroup a CU: two at once take 4/3 of one alone
-    const long us256 = up(t256, cus) * (14 * st + 70 + (GELU ? 50 : 0)), us192 = (2 * half + half % 2) * (11 * st + 60 + (GELU ? 20 : 0)) / 4, us64 = up(t64, 2 * cus) * (4 * st + 14);
-    if (p.M <= 128 || (us64 <= us192 && us64 <= us256)) return launch_ring<T, GELU, 64, 64, 2, 2, 4>(p, s);
-    if (us192 <= us256) return launch_ring<T, GELU, 192, 128, 2, 2, 2>(p, s);
+    const long us256 = up(t256, cus) * (14 * st + 70 + (gelu ? 50 : 0)), us192 = (2 * half + half % 2) * (11 * st + 60 + (gelu ? 20 : 0)) / 4, us64 = up(t64, 2 * cus) * (4 * st + 14);
+    if (M <= 128 || (us64 <= us192 && us64 <= us256)) return {MMSUM_I8_PLAN_RING, 64, 64, t64};
+    if (us192 <= us256) return {MMSUM_I8_PLAN_RING, 192, 128, t192};
+    return {MMSUM_I8_PLAN_W4, 256, 256, t256 < cus ? t256 : cus};
+}
+
+template <typename T, bool GELU>
+int launch_product(const I8Args& p, hipStream_t s) {
+    const I8Plan g = plan_product(p.M, p.N, p.K, GELU);
+    if (g.kernel == MMSUM_I8_PLAN_FEW) {
+        if (g.bm == 16) return g.bn == 64 ? launch_few<T, GELU, 1, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 1, 1, false, float>(p, nullptr, 0, 0, s);
+        if (g.bm == 32) return g.bn == 64 ? launch_few<T, GELU, 2, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 2, 1, false, float>(p, nullptr, 0, 0, s);
+        return g.bn == 64 ? launch_few<T, GELU, 4, 4, false, float>(p, nullptr, 0, 0, s) : launch_few<T, GELU, 4, 1, false, float>(p, nullptr, 0, 0, s);
+    }
+    if ((p.M + 63L) / 64 * ((p.N + 63L) / 64) > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    if (g.bm == 64) return launch_ring<T, GELU, 64, 64, 2, 2, 4>(p, s);
+    if (g.bm == 192) return launch_ring<T, GELU, 192, 128, 2, 2, 2>(p, s);
     const size_t lds = 5 * kStageBytes;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_w4_kernel<T, GELU>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return MMSUM_ERR_HIP;
-    hipLaunchKernelGGL((gemm_i8_w4_kernel<T, GELU>), dim3((unsigned)(t256 < cus ? t256 : cus)), dim3(256), lds, s, p);
+    hipLaunchKernelGGL((gemm_i8_w4_kernel<T, GELU>), dim3((unsigned)g.groups), dim3(256), lds, s, p);
     return ok();
 }
 
 // Quantisation and product.  In one launch for up to 8,192 values: there every workgroup's quantising all rows costs no more than the launch (us,
 // two | one, N = 1,024): 1 x 1,024 4.8 | 3.5, 1 x 4,096 9.2 | 7.6, 8 x 1,024 5.2 | 5.0, 16 x 1,024 5.4 | 7.7, 8 x 4,096 10.0 | 12.9; 8 x 1,024 into 16,384
 // columns 7.4 | 7.8, into 50,265 15.9 | 19.4.
+bool quantises_inside(int M, int N, int K) { return M <= 16 && (long)M * K <= 8192 && N <= 16384; }
 template <typename T, bool GELU>
 int launch_linear(int dtype, const void* x, long ldx, I8Args p, int Kx, hipStream_t s) {
-    if (p.M <= 16 && (long)p.M * p.K <= 8192 && p.N <= 16384) {
+    if (quantises_inside(p.M, p.N, p.K)) {
         if (dtype == MMSUM_BF16) return launch_few<T, GELU, 1, 1, true, bf16_t>(p, static_cast<const bf16_t*>(x), ldx, Kx, s);
         return launch_few<T, GELU, 1, 1, true, float>(p, static_cast<const float*>(x), ldx, Kx, s);
     }
@@ -730,4 +743,14 @@ extern "C" int mmsum_linear_i8(int dtype, const void* x, long ldx, const void* q
     hipStream_t s = (hipStream_t)stream;
     if (dtype_out == MMSUM_BF16) return gelu ? launch_linear<bf16_t, true>(dtype, x, ldx, p, K, s) : launch_linear<bf16_t, false>(dtype, x, ldx, p, K, s);
     return gelu ? launch_linear<float, true>(dtype, x, ldx, p, K, s) : launch_linear<float, false>(dtype, x, ldx, p, K, s);
+}
+
+extern "C" int mmsum_linear_i8_plan(int M, int N, int K, int gelu, int quantise, int* plan) {
+    if (M <= 0 || N <= 0 || K <= 0 || K > 131072 || (!quantise && K % 128)) return MMSUM_ERR_BAD_SHAPE;
+    if (plan == nullptr) return MMSUM_ERR_BAD_ALIGN;
+    const int Kp = (K + 127) / 128 * 128;
+    const I8Plan g = quantise && quantises_inside(M, N, Kp) ? I8Plan{MMSUM_I8_PLAN_FEW_QUANTISING, 16, 16, (N + 15L) / 16} : plan_product(M, N, Kp, gelu != 0);
+    if (g.groups > 0x7fffffffL) return MMSUM_ERR_BAD_SHAPE;
+    plan[0] = g.kernel; plan[1] = g.bm; plan[2] = g.bn; plan[3] = (int)g.groups;
+    return MMSUM_OK;
 }

@@ -935,8 +935,15 @@ def linear_i8(x, qw, sw, out=None, bias=None, gelu=False, out_dtype=None):
         _apart(x, out)
     dto = _dt(out)
     if M and N:
-        ws = torch.empty(M * (qw.shape[1] + 4), dtype=torch.uint8, device=dev)
+        ws = torch.empty(lib.mmsum_linear_i8_workspace(M, K), dtype=torch.uint8, device=dev)
         _launch("mmsum_linear_i8", dev, dt, x.data_ptr(), ldx, qw.data_ptr(), ldw, sw.data_ptr(), None if bias is None else bias.data_ptr(), dto, out.data_ptr(), ldy, M, N, K,
                 int(bool(gelu)), ws.data_ptr())
         _wrote(given)
     return out
+
+
+def linear_i8_plan(M, N, K, gelu=False, quantise=True):
+    """(kernel, rows, columns of a tile, workgroups) that linear_i8 (quantise False: gemm_i8) launches for the product, see mmsum_linear_i8_plan."""
+    plan = (ctypes.c_int * 4)()
+    check(lib.mmsum_linear_i8_plan(M, N, K, int(bool(gelu)), int(bool(quantise)), plan), "mmsum_linear_i8_plan")
+    return tuple(plan)

@@ -239,3 +239,31 @@ def test_int8_layer_from_its_state_dict(monkeypatch):
         again = mm.Int8Linear(torch.zeros(6, 8), None if bias is None else torch.zeros(6)).bfloat16()
         again.load_state_dict(saved)
         assert again.state_dict().keys() == saved.keys() and all(torch.equal(v, saved[k]) and v.dtype == saved[k].dtype for k, v in again.state_dict().items())
+
+
+def test_int8_plan():
+    """Every product of the 8-bit linear layer is reached by sizes that the GPU tests run; the rules' borders; the plan needs no device."""
+    from multimodalsum_amd import _lib, kernels as kn
+    from tests import test_alignment_edges_gpu as edges, test_alignment_ops_gpu as ops
+    few, inside, ring, w4 = _lib.I8_PLAN_FEW, _lib.I8_PLAN_FEW_QUANTISING, _lib.I8_PLAN_RING, _lib.I8_PLAN_W4
+
+    def p(M, N, K, **kw):
+        return kn.linear_i8_plan(M, N, K, **kw)[:3]
+    assert kn.linear_i8_plan(8, 1024, 1024) == (inside, 16, 16, 64) and p(9, 1024, 1024) == (few, 16, 16) and p(8, 1024, 1024, quantise=False) == (few, 16, 16)
+    assert p(8, 16385, 1024) == (few, 16, 16) and p(16, 32768, 128) == (few, 16, 64) and p(17, 16383, 128) == (few, 32, 16) and p(17, 16384, 128) == (few, 32, 64)
+    assert p(33, 100, 128) == (few, 64, 16) and p(64, 50265, 1024) == (few, 64, 64) and p(65, 50265, 1024) == (ring, 64, 64) == p(128, 4096, 1024)
+    assert kn.linear_i8_plan(32, 50265, 1024) == (few, 32, 64, 786)
+    assert p(36864, 4096, 1024) == (w4, 256, 256) and p(36864, 4096, 1024, gelu=True) == p(36864, 1024, 4096) == (ring, 192, 128) and kn.linear_i8_plan(8192, 8192, 8192) == (w4, 256, 256, 256)
+    listed = ops.I8 + edges.I8_WIDE
+    edge = [m.args[1] for m in ops.test_int8_product_at_tile_edges.pytestmark if m.name == "parametrize" and m.args[0] == "M,N,K"][0]
+    for gelu in (False, True):
+        reached = {p(M, N, K, gelu=gelu) for M, N, K in listed} | {p(M, N, -(-K // 128) * 128, gelu=gelu, quantise=False) for M, N, K in edge}
+        assert reached == {(inside, 16, 16), (few, 16, 16), (few, 16, 64), (few, 32, 16), (few, 32, 64), (few, 64, 16), (few, 64, 64), (ring, 64, 64), (ring, 192, 128),
+                           (w4, 256, 256)}, reached
+        at_edges = [p(M, N, -(-K // 128) * 128, gelu=gelu, quantise=False) for M, N, K in edge]
+        assert at_edges.count((w4, 256, 256)) >= 2 and at_edges.count((ring, 192, 128)) >= 2, at_edges
+    for bad in ((0, 4, 128), (4, 0, 128), (4, 4, 0), (4, 4, 131073)):
+        refused(RuntimeError, kn.linear_i8_plan, *bad)
+    refused(RuntimeError, kn.linear_i8_plan, 4, 4, 100, quantise=False)
+    for M, K in ((1, 1), (3, 128), (5, 129), (1000, 131072), (2 ** 20, 4096)):      # the entry's own statement of its workspace: rows padded to 128, then their scales
+        assert _lib.lib.mmsum_linear_i8_workspace(M, K) == M * (-(-K // 128) * 128 + 4)

@@ -204,3 +204,31 @@ def test_int8_layer_in_a_model_that_is_cast():
     want = lin(x)
     model = torch.nn.Sequential(torch.nn.Linear(24, 24, device="cuda"), lin).bfloat16()
     assert model[0].weight.dtype == torch.bfloat16 and torch.equal(model[1](x), want)
+
+
+# up to 64 rows into many columns: workgroups of 64 columns, the last one not full, for one, two and four blocks of 16 rows
+I8_WIDE = [(1, 32769, 256), (16, 50265, 1024), (17, 16385, 384), (32, 50265, 1024), (33, 16400, 300), (64, 20011, 512)]
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,N,K", I8_WIDE)
+def test_int8_linear_of_few_rows_into_many_columns(M, N, K, dt):
+    """Exact integer sums in 64 bits; the sum's conversion, two scales and the bias: 8 H of the parts, GELU as for the other sizes 40 H, half a step of the result."""
+    from multimodalsum_amd import Int8Linear, _lib, kernels as kn
+    g = torch.Generator().manual_seed(M + N + K)
+    x = (torch.randn(M, K, generator=g) * (0.2 + torch.rand(M, 1, generator=g))).to(dt).cuda()
+    lin = Int8Linear((torch.randn(N, K, generator=g) * 0.05).cuda(), torch.randn(N, generator=g).cuda())
+    assert kn.linear_i8_plan(M, N, K)[:3] == (_lib.I8_PLAN_FEW, 16 if M <= 16 else 32 if M <= 32 else 64, 64)
+    qx, sx = kn.quantize_rows(x)
+    product = torch.mm(qx.double(), lin.qweight.double().t().contiguous()) * sx.double()[:, None] * lin.scale.double()
+    for bias, gelu in ((None, False), (lin.bias, False), (lin.bias, True)):
+        want = product if bias is None else product + bias.double()
+        mag = product.abs() + (0.0 if bias is None else bias.double().abs())
+        if gelu:
+            want = 0.5 * want * torch.special.erfc(-want / 2 ** 0.5)
+        for out in (torch.float32, torch.bfloat16):
+            wide = torch.full((M + 2, N + 6), float("nan"), dtype=out, device="cuda")
+            kn.linear_i8(x, lin.qweight, lin.scale, wide[1:-1, 3:N + 3], bias, gelu)
+            y = wide[1:-1, 3:N + 3].double()
+            assert ((y - want).abs() <= mag * (40 if gelu else 8) * H + want.abs() * torch.finfo(out).eps / 2 + torch.finfo(out).tiny).all()
+            assert torch.isnan(wide[0]).all() and torch.isnan(wide[-1]).all() and torch.isnan(wide[:, :3]).all() and torch.isnan(wide[:, N + 3:]).all()
