@@ -232,3 +232,47 @@ def test_int8_linear_of_few_rows_into_many_columns(M, N, K, dt):
             y = wide[1:-1, 3:N + 3].double()
             assert ((y - want).abs() <= mag * (40 if gelu else 8) * H + want.abs() * torch.finfo(out).eps / 2 + torch.finfo(out).tiny).all()
             assert torch.isnan(wide[0]).all() and torch.isnan(wide[-1]).all() and torch.isnan(wide[:, :3]).all() and torch.isnan(wide[:, N + 3:]).all()
+
+
+@pytest.mark.parametrize("average", [False, True])
+@pytest.mark.parametrize("eps", [0.0, 0.1])
+@pytest.mark.parametrize("P,T,V", [(1, 1100, 5), (16, 300, 7), (17, 300, 7), (33, 1000, 3), (300, 40, 9)])
+def test_preference_gradient_of_long_sequences(P, T, V, eps, average):
+    """The factor of every sequence and the gradient of the logits, by both forms, against 64 bits from the f32 log-probabilities that the kernel itself
+    sums, so that only these roundings count.  h: the f32 of a 64-bit sum (beta and ref are f32 values): H |h|.  Factor: sigmoid's slope in h is below its
+    value, so |h| H, and the exponential, quotient, difference (smoothing: of values it is a tenth of at least) and four products: 40 H in all.  Gradient:
+    the row's own statistics on top, 400 H of the factor's two products for rows of this kind.  What the tolerance rejects is asserted beside it."""
+    from multimodalsum_amd import kernels as kn
+    g = torch.Generator().manual_seed(P + T)
+    x = torch.randn(2 * P, T, V, generator=g).cuda()
+    labels = torch.randint(0, V, (2 * P, T), generator=g)
+    for i in range(2 * P):                                             # ragged, one sequence empty
+        labels[i, T - (7 * i) % (T // 2):] = -100
+    if P > 1:
+        labels[1] = -100
+    labels = labels.cuda()
+    keep = (labels >= 0) & (labels < V)
+    stats = torch.empty(2 * P, T, 2, device="cuda")
+    logp = kn.token_logprob(x, labels, stats)
+    cnt = keep.sum(1).clamp(min=1).double()
+    seq = (logp.double() * keep).sum(1) / (cnt if average else 1.0)
+    ref = (seq + torch.randn(2 * P, generator=g).cuda() * 2).float()    # margins of a few units
+    beta = torch.tensor(0.3).item()
+    r = seq - ref.double()
+    h = beta * (r[:P] - r[P:])
+    dh = (eps - torch.sigmoid(-h)) * beta / P
+    want = torch.cat([dh, -dh]) / (cnt if average else 1.0)
+    loss, margins, got_seq, coef = kn.preference_pairs(logp, labels, ref, V, 0.3, eps, average)
+    tol = (40 + 2 * h.abs().repeat(2)) * H * torch.cat([beta / P * (eps + torch.sigmoid(-h))] * 2) / (cnt if average else 1.0)
+    assert ((coef.double() - want).abs() <= tol).all() and (tol < 0.01 * want.abs().max()).all()
+    p = torch.softmax(x.double(), -1)
+    lab = torch.where(keep, labels, torch.zeros_like(labels))
+    one = torch.zeros_like(p).scatter_(-1, lab[..., None], 1.0)
+    d_want = torch.where(keep[..., None], want[:, None, None] * (one - p), torch.zeros_like(p))
+    d_tol = (tol[:, None, None] + 400 * H * want.abs()[:, None, None]) * (one + p)
+    fused = kn.preference_loss(x, labels, ref, 0.3, eps, average)
+    assert torch.equal(fused[0], loss) and torch.equal(fused[1], margins) and torch.equal(fused[2], got_seq)
+    for d in (fused[3], kn.token_logprob_bwd(x, labels, stats, coef)):
+        assert ((d.double() - d_want).abs() <= d_tol).all() and (d[~keep] == 0).all()
+    for wrong in (torch.zeros_like(d_want), -d_want, 2 * d_want, d_want.roll(1, 0)) + ((d_want * cnt[:, None, None],) if average else ()):
+        assert not ((wrong - d_want).abs() <= d_tol).all()
