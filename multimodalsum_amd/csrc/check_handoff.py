@@ -15,6 +15,13 @@ This script reads the device assembly the object was built from (hipcc -save-tem
   3. an `s_waitcnt` with vmcnt(0) lies between the last payload store and the ticket;
   4. after the ticket at least one `global_load_dword*` carries sc1 and at most ALLOW[kernel] dword loads do not (dec_gemm: the bias).
 
+Counted waits (int8.hip, gemm_i8_w4_kernel with bf16 results): the first stage of a tile waits with vmcnt(40) for pieces that were requested before
+the last tile's epilogue, leaving 8 younger pieces and that epilogue's 32 stores in flight.  With fewer stores (two of them merged, say) the wait would
+not reach the pieces, and the stage would multiply what LDS held before.  In such a kernel the build also fails unless
+
+  5. it has a wait of that count, and
+  6. its wide stores are that many in one straight run: no branch, load or other store between them (results of whole tiles, in one piece each).
+
 usage: check_handoff.py <device .s file> [...]
 """
 import re
@@ -24,6 +31,9 @@ import sys
 # split of the small NT products, gemm_nt_ring_kernel<..., FS = true>: whatever the ordinary epilogue behind the reduction reads --
 # bias, saved pre-activation, the C of an accumulating store)
 KERNELS = {"dec_gemm_kernel": 1, "decode_cross_attn_kernel": 0, "decode_cross_attn_f32_kernel": 0, r"gemm_nt_ring_kernel\w*Lb1EEEv8GemmArgs": 256}
+# kernel family -> (count of the wait, wide stores that it counts on)
+COUNTED = {r"gemm_i8_w4_kernelIDF16b": (40, 32)}
+VMEM = re.compile(r"(global|buffer|flat|scratch)_|s_c?branch|s_barrier|s_endpgm")
 LABEL = re.compile(r"^(_Z\w+):")
 
 
@@ -70,10 +80,37 @@ def check(name, allow, body):
     return errs
 
 
+def check_counted(wait, stores, body):
+    errs = []
+    if not any(t.startswith("s_waitcnt") and re.search(r"vmcnt\(%d\)" % wait, t) for t in body):
+        errs.append("no s_waitcnt vmcnt(%d)" % wait)
+    runs, last = [], ""
+    for t in body:
+        m = VMEM.match(t)
+        if m:
+            name = t.split()[0]
+            if name == "global_store_dwordx4":
+                if last == name:
+                    runs[-1] += 1
+                else:
+                    runs.append(1)
+            last = name
+    if runs != [stores]:
+        errs.append("runs of wide stores: %s, one of %d expected behind the counted wait" % (runs, stores))
+    return errs
+
+
 def main(paths):
-    seen, bad = {k: 0 for k in KERNELS}, 0
+    seen, bad = {k: 0 for k in list(KERNELS) + list(COUNTED)}, 0
     for path in paths:
         for name, body in functions(path):
+            counted = next((k for k in COUNTED if re.search(k, name)), None)
+            if counted is not None and any(t.startswith("s_endpgm") for t in body):
+                seen[counted] += 1
+                for e in check_counted(*COUNTED[counted], body):
+                    bad += 1
+                    print("check_handoff: %s: %s" % (name, e), file=sys.stderr)
+                continue
             fam = next((k for k in sorted(KERNELS, key=len, reverse=True) if re.search(k, name)), None)
             if fam is None or not any(t.startswith("s_endpgm") for t in body):
                 continue
@@ -83,7 +120,7 @@ def main(paths):
                 print("check_handoff: %s: %s" % (name, e), file=sys.stderr)
     present = [k for k, n in seen.items() if n]
     if not present:
-        print("check_handoff: none of %s found in %s" % (sorted(KERNELS), paths), file=sys.stderr)
+        print("check_handoff: none of %s found in %s" % (sorted(seen), paths), file=sys.stderr)
         return 1
     if bad:
         return 1

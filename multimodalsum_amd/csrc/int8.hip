@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(I8Args p) {
             if constexpr (LEFT >= 2) { if (!(g & 1)) I8_A(g >> 1) }
         }
         // vmcnt counts down in order: behind stage s + 1's pieces come, in a tile's first stage, the last tile's 32 stores of a whole bf16
-        // epilogue (its loads are back before its first store), which may stay in flight
+        // epilogue (its loads are back before its first store), which may stay in flight (check_handoff.py: the build fails unless they are 32)
         if constexpr (LEFT >= 2 && FIRST && sizeof(T) == 2) {
             if (whole) asm volatile("s_waitcnt vmcnt(40)" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");

@@ -267,3 +267,24 @@ def test_int8_plan():
     refused(RuntimeError, kn.linear_i8_plan, 4, 4, 100, quantise=False)
     for M, K in ((1, 1), (3, 128), (5, 129), (1000, 131072), (2 ** 20, 4096)):      # the entry's own statement of its workspace: rows padded to 128, then their scales
         assert _lib.lib.mmsum_linear_i8_workspace(M, K) == M * (-(-K // 128) * 128 + 4)
+
+
+def test_the_build_checks_the_counted_wait(tmp_path):
+    """The four-wave 8-bit kernel's vmcnt(40) counts on 32 wide stores in a row: the build's check accepts those and nothing else."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "multimodalsum_amd", "csrc", "check_handoff.py")
+    spec = importlib.util.spec_from_file_location("check_handoff", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    store, wait = "\tglobal_store_dwordx4 v[0:1], v[2:5], off", "\ts_waitcnt vmcnt(40)"
+
+    def rc(*lines):
+        f = tmp_path / "k.s"
+        f.write_text("\n".join(["_Z17gemm_i8_w4_kernelIDF16bLb1EEvX:", *lines, "\ts_endpgm", ".Lfunc_end0:"]) + "\n")
+        return mod.main([str(f)])
+    tail = ["\ts_cbranch_scc0 .LBB0_1", "\tglobal_store_short v0, v1, off"]
+    assert rc(wait, *[store] * 32, *tail) == 0 and rc(*["\tv_add_f32 v0, v0, v1", store] * 32, wait, *tail) == 0
+    assert rc(wait, *[store] * 31, *tail) == 1 and rc(wait, *[store] * 33, *tail) == 1 and rc(*[store] * 32, *tail) == 1
+    assert rc(wait, *[store] * 16, "\ts_branch .LBB0_2", *[store] * 16) == 1 and rc(wait, *[store] * 16, "\tglobal_load_dword v0, v1, off", *[store] * 16) == 1
+    assert rc("\ts_waitcnt vmcnt(41)", *[store] * 32) == 1
