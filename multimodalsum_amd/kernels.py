@@ -686,7 +686,7 @@ def _dlogits_of(dlogits, logits, N, T, V, ld):
     n, t, W, ldd = _rows_of(dlogits, "dlogits")
     _need((n, t) == (N, T) and W >= V, "dlogits: [%d, %d, >= %d] expected, got %s", N, T, V, dlogits.shape)
     a, b = _span(logits), _span(dlogits)
-    _need(a[0] >= b[1] or b[0] >= a[1] or (a[0] == b[0] and ld == ldd), "dlogits overlaps the logits without being them")
+    _need(a[0] >= b[1] or b[0] >= a[1] or (a[0] == b[0] and (ld == ldd or N * T == 1)), "dlogits overlaps the logits without being them")
     return dlogits, ldd, W
 
 

@@ -288,3 +288,19 @@ def test_the_build_checks_the_counted_wait(tmp_path):
     assert rc(wait, *[store] * 31, *tail) == 1 and rc(wait, *[store] * 33, *tail) == 1 and rc(*[store] * 32, *tail) == 1
     assert rc(wait, *[store] * 16, "\ts_branch .LBB0_2", *[store] * 16) == 1 and rc(wait, *[store] * 16, "\tglobal_load_dword v0, v1, off", *[store] * 16) == 1
     assert rc("\ts_waitcnt vmcnt(41)", *[store] * 32) == 1
+
+
+def test_gradient_over_the_padded_buffer_of_the_logits(monkeypatch):
+    """dlogits = the buffer that the logits are a view of: for any number of rows, one among them; buffers of another pitch or start stay refused."""
+    import multimodalsum_amd as mm
+    rec = Recorder(monkeypatch)
+    for N, T in ((4, 3), (2, 1), (1, 3), (1, 1)):
+        lab, z, adv = torch.zeros(N, T, dtype=torch.int64), torch.zeros(N, T), torch.zeros(N)
+        for W in (8, 9, 12):
+            buf = torch.zeros(N, T, 12)
+            assert mm.policy_loss_and_grad(buf[:, :, :8], lab, z, adv, dlogits=buf[:, :, :W])[4].data_ptr() == buf.data_ptr()
+            assert rec.calls[-1][1][18:20] == (12 if N * T > 1 else W, W)
+        for other in (buf[:, :, 1:9], buf[:, :, 4:]):
+            refused(ValueError, mm.policy_loss_and_grad, buf[:, :, :8], lab, z, adv, dlogits=other)
+    refused(ValueError, mm.policy_loss_and_grad, buf.view(-1)[:8].view(1, 1, 8).expand(1, 1, 8), torch.zeros(1, 1, dtype=torch.int64), torch.zeros(1, 1), torch.zeros(1),
+            dlogits=buf.view(-1)[2:10].view(1, 1, 8))

@@ -276,3 +276,14 @@ def test_preference_gradient_of_long_sequences(P, T, V, eps, average):
         assert ((d.double() - d_want).abs() <= d_tol).all() and (d[~keep] == 0).all()
     for wrong in (torch.zeros_like(d_want), -d_want, 2 * d_want, d_want.roll(1, 0)) + ((d_want * cnt[:, None, None],) if average else ()):
         assert not ((wrong - d_want).abs() <= d_tol).all()
+
+
+def test_gradient_over_the_padded_buffer_of_one_row():
+    import multimodalsum_amd as mm
+    for dt in (torch.float32, torch.bfloat16):
+        for V in (50, 50265, 110003):
+            buf = torch.randn(1, 1, V + 7, generator=torch.Generator().manual_seed(V)).to(dt).cuda()
+            args = (torch.full((1, 1), 3, device="cuda"), torch.full((1, 1), -2.0, device="cuda"), torch.ones(1, device="cuda"))
+            want = mm.policy_loss_and_grad(buf[:, :, :V].clone(), *args)
+            got = mm.policy_loss_and_grad(buf[:, :, :V], *args, dlogits=buf)
+            assert torch.equal(got[0], want[0]) and torch.equal(buf[:, :, :V], want[4]) and (buf[:, :, V:] == 0).all()
