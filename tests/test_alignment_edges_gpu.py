@@ -287,3 +287,25 @@ def test_gradient_over_the_padded_buffer_of_one_row():
             want = mm.policy_loss_and_grad(buf[:, :, :V].clone(), *args)
             got = mm.policy_loss_and_grad(buf[:, :, :V], *args, dlogits=buf)
             assert torch.equal(got[0], want[0]) and torch.equal(buf[:, :, :V], want[4]) and (buf[:, :, V:] == 0).all()
+
+
+@pytest.mark.parametrize("dt,P,T", [(torch.bfloat16, 10, 160), (torch.float32, 5, 160), (torch.bfloat16, 10, 141)])
+def test_preference_loss_of_more_logits_than_the_cache_holds(dt, P, T):
+    """Rows on both sides of the 256 MB that the second reading finds in the cache: the fused call's numbers are the two-step form's, bit for bit, also over the
+    logits themselves."""
+    from multimodalsum_amd import kernels as kn
+    V = 50265
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.randn(2 * P, T, V, generator=g, device="cuda").to(dt)
+    assert x.numel() * x.element_size() > 268 * 2 ** 20
+    labels = torch.randint(0, V, (2 * P, T), generator=g, device="cuda")
+    labels[3, 5:] = -100
+    stats = torch.empty(2 * P, T, 2, device="cuda")
+    logp = kn.token_logprob(x, labels, stats)
+    loss, margins, seq, coef = kn.preference_pairs(logp, labels, None, V, 0.1, 0.0, False)
+    want = kn.token_logprob_bwd(x, labels, stats, coef)
+    for over in (None, x):
+        got = kn.preference_loss(x, labels, None, 0.1, 0.0, False, over)
+        for a, b in zip(got, (loss, margins, seq, want)):
+            assert torch.equal(a, b)
+    assert (want != 0).any() and not (want[3, 5:] != 0).any()
