@@ -7,6 +7,7 @@ import ctypes
 import operator
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib, check, AttnDesc, F32, BF16
@@ -597,8 +598,8 @@ INT_SIZE = 2 ** 31 - 16384         # sizes that the C entries take as int, and r
 
 
 def _sizes(what, *sizes):
-    for n in sizes:
-        _need(n < INT_SIZE, "%s: a size of %d", what, n)
+    if max(sizes) >= INT_SIZE:
+        raise ValueError("%s: a size of %d" % (what, max(sizes)))
 
 
 def _device(*tensors):
@@ -816,7 +817,7 @@ def _ids_of(ids):
 
 def no_tangent(t, what):
     """Refuses a forward-mode dual tensor, whose tangent a launch would drop without a word."""
-    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:      # (the level first: a fifth of the look)
         raise RuntimeError("%s has no forward-mode derivative" % what)
 
 
@@ -886,7 +887,7 @@ def quantize_rows(x):
     ldx = _pitch2(x, "x")
     M, K = x.shape
     _need(0 < K <= 131072, "quantize_rows: K = %d, 1 .. 131072 expected", K)
-    _sizes("quantize_rows", M)
+    _sizes("quantize_rows", M, K)
     _dt(x)
     dev = _device(x)
     Kp = -(-K // I8_K_STEP) * I8_K_STEP
@@ -935,7 +936,7 @@ def linear_i8(x, qw, sw, out=None, bias=None, gelu=False, out_dtype=None):
         _apart(x, out)
     dto = _dt(out)
     if M and N:
-        ws = torch.empty(lib.mmsum_linear_i8_workspace(M, K), dtype=torch.uint8, device=dev)
+        ws = torch.empty(M * (qw.shape[1] + 4), dtype=torch.uint8, device=dev)      # mmsum_linear_i8_workspace, a call less
         _launch("mmsum_linear_i8", dev, dt, x.data_ptr(), ldx, qw.data_ptr(), ldw, sw.data_ptr(), None if bias is None else bias.data_ptr(), dto, out.data_ptr(), ldy, M, N, K,
                 int(bool(gelu)), ws.data_ptr())
         _wrote(given)
