@@ -601,16 +601,18 @@ extern "C" int mmsum_preference_loss(int dtype, const void* logits, long ld, con
     float* const pair_loss = stats + 2L * R;
     float* const coef = pair_loss + P;
     hipStream_t s = (hipStream_t)stream;
-    // Statistics, the pairs, then the gradient from the last row to the first.  All rows but the last 256 MB, what the memory-side cache holds, are read
-    // past the caches, which leaves those to the second reading.  Measured (us; every row past the caches | all but the last 128 MB | 256 | 400 | none past):
-    // bf16, 128 x 50,265 a sequence: 4 pairs 71 | 65 | 64 | 64 | 64, 9: 142 | 130 | 122 | 122 | 122, 18: 261 | 251 | 238 | 240 | 241, 36: 497 | 487 | 476 | 480 |
-    // 488, 72: 975 | 963 | 954 | 965 | 989; f32, 12: 403 | 384 | 378 | 379 | 380, 36: 1,143 | 1,122 | 1,115 | 1,118 | 1,121; the gradient's memory reused or
-    // fresh alike.  (Every row's workgroup of the gradient taking its pair's sums itself in place of the pairs' launch: 4 x 128 x 1,009 equal,
-    // 36 x 128 x 1,009 30 -> 52 us.)
+    // Statistics, the pairs, then the gradient from the last row to the first.  All rows but the last 400 MB are read past the caches, which leaves those
+    // to the second reading.  The memory-side cache holds 256 MB, and rows that do not count are not read: 400 MB are 256 where 64 % count, between a full
+    // batch, for which less were better, and a ragged one, for which more were.  Measured (us; every row past the caches | all but the last 256 MB | 400 | 512 |
+    // none past; bf16, 128 x 50,265 a sequence), 36 pairs: all counted 497 | 477 | 481 | 484 | 488, 84 % 456 | 429 | 427 | 427 | 435, 51 % 362 | 338 | 324 | 317 |
+    // 316; 18 pairs: 261 | 240 | 241 | 242 | 242, 84 % 240 | 215 | 211 | 211 | 211, 51 % 193 | 168 | 155 | 152 | 152; 72 pairs: 975 | 953 | 965 | 969 | 992, 84 % 879 |
+    // 855 | 854 | 855 | 876, 51 % 693 | 669 | 656 | 650 | 653; f32, 18 pairs: 588 | 565 | 566 | 567 | 569, 84 % 543 | 515 | 510 | 510 | 514, 51 % 423 | 407 | 387 |
+    // 377 | 373; the gradient's memory reused or fresh alike.  (Every row's workgroup of the gradient taking its pair's sums itself in place of the pairs'
+    // launch: 4 x 128 x 1,009 equal, 36 x 128 x 1,009 30 -> 52 us.)
     const auto run = [&](auto of_type) {
         typedef decltype(of_type) T_;
         RowArgs<T_> a = row_args<T_>(logits, ld, labels, R, V, logp, stats);
-        const long keep = (256L << 20) / (ld * (long)sizeof(T_));
+        const long keep = (400L << 20) / (ld * (long)sizeof(T_));
         a.past = keep < R ? R - (int)keep : 0;
         int rc = launch_rows<T_, false>(a, s);
         if (rc == MMSUM_OK) rc = mmsum_preference_pairs(logp, labels, ref, P, T, V, beta, smoothing, average, seq, margins, pair_loss, coef, loss, stream);
