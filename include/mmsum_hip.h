@@ -419,7 +419,8 @@ int mmsum_decode_self_attn(int dtype, const void* q, long ldq, void* k_cache, vo
  * Losses on the log-probability of given tokens.  Rows are positions (r = n T + t of N sequences of T), ld / ldd row pitches in elements;
  * rows may start at any element (packed [N, T, V] logits with an odd V).  A label outside 0 .. V-1 marks a position that does not count:
  * its logits are not read, its log-probability is 0 and its gradient a row of zeros.  dlogits [R, W >= V] (pitch ldd) is written whole,
- * columns V .. W-1 as zeros; it may be the logits themselves (same pitch).  Sums are f32 in a fixed order: results are reproducible.
+ * columns V .. W-1 as zeros; it may be the logits themselves (same pitch).  A row is summed in f32,
+ * sequences and means in 64 bits, in a fixed order: results are reproducible.  A required pointer that is NULL: MMSUM_ERR_BAD_ALIGN.
  *
  * logp[r] = log_softmax(logits[r, :V])[labels[r]]; stats (may be NULL): {max, sum of exponentials} of every row, for the backward pass. */
 int mmsum_token_logprob(int dtype, const void* logits, long ld, const int64_t* labels, float* logp, float* stats, int R, int V, void* stream);
@@ -440,7 +441,7 @@ int mmsum_preference_loss(int dtype, const void* logits, long ld, const int64_t*
                           int average, float* loss, float* margins, float* seq, void* dlogits, long ldd, int W, void* workspace, void* stream);
 /* Clipped policy loss with a KL term: ratio = exp(logp - old_logp), A = adv[row] (adv_per_token) or adv[sequence],
  * token loss = max(-A ratio, -A min(max(ratio, 1 - clip_low), 1 + clip_high)) + kl_coef kl, kl = e^d - d - 1 with d = ref_logp - logp (ref_logp NULL:
- * none); mean over the counted tokens, or (seq_mean) over the sequences of the mean over a sequence's counted tokens (an empty one counts 0).
+ * none; kl_coef 0: reported, not part of the loss); mean over the counted tokens, or (seq_mean) over the sequences of the mean over a sequence's counted tokens (an empty one counts 0).
  * out [3] = {loss, the same mean of kl, the same mean of [the bounded branch is the larger]}.  old_logp, ref_logp [N T].
  * _terms: from log-probabilities, coef [N T] for mmsum_token_logprob_bwd with rows_per_coef = 1.  _loss: logits to gradient with the logits read
  * once; logp [N T].  workspace: mmsum_policy_workspace bytes. */

@@ -414,7 +414,9 @@ __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(I8Args p) {
 // One tile of BM x BN a workgroup of WM x WN waves, the stages in a ring that runs NST - 1 of them ahead of the products, at most 80 KB of
 // LDS: two workgroups a CU, and the main loop of one runs under the waits and the epilogue of the other.  Operand rows, swizzle and the order
 // of the weight rows as above.  192x128 (two stages) for large products of a short sum, where the epilogue weighs; 64x64 (four) for small ones.
-// Measured (MI355X, 192x128): 36,864 x 4,096 x 1,024 178 us, with GELU 207; 36,864 x 1,024 x 4,096 127 us = 2,435 TOP/s.
+// Measured (MI355X, 192x128): 36,864 x 4,096 x 1,024 178 us, with GELU 193 - 207 launch after launch (228 in a kernel trace, every launch on an idle
+// card); 36,864 x 1,024 x 4,096 127 us = 2,435 TOP/s.  38,400 x 3,584 x 1,024, plain | GELU: matrix cores busy 39 | 36 % of the cycles, vector units 29 | 61 %:
+// with GELU the two take turns.
 template <typename T, bool GELU, int BM, int BN, int WM, int WN, int NST>
 __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_i8_ring_kernel(I8Args p) {
     constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * 128, PA = BM / 8 / NW, PB = BN / 8 / NW, PPW = PA + PB;

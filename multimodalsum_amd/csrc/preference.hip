@@ -8,8 +8,9 @@
 // Bound: HBM.  The policy loss knows c as soon as the row's own log p is known, so its kernel reads the logits once and writes the
 // gradient once, the row waiting in registers in between.  The preference loss needs the sums over both summaries of a pair first:
 // statistics (read), the pairs' sums and factors, gradient (read, write).
-// Measured (MI355X, 50,265 bf16 logits): scoring 72 x 141 rows 177 us (4.8 TB/s), policy loss 72 x 128 rows 309 us (5.5 TB/s), preference loss
-// of 36 pairs x 128 rows 416 us (4.1 TB/s of what has to move, 5.9 with the second reading).
+// Measured (MI355X, 50,265 bf16 logits, whole calls one after the other): scoring 72 x 141 rows 177 us (4.7 TB/s), policy loss 72 x 128 rows 317 us (5.3
+// TB/s), preference loss of 36 pairs x 128 rows 425 us (4.0 TB/s of what has to move, 5.8 with the second reading); the results' memory new or reused
+// alike.  In a kernel trace, where every launch finds the card idle, the policy kernel takes 313 - 388 us, 358 in the middle.
 // A row is summed in f32, sequences and means in 64 bits, in an order that depends on the sizes alone.
 #include "entry_checks.h"
 #include "mmsum_device.h"
