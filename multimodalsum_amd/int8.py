@@ -30,13 +30,13 @@ class Int8Linear(nn.Module):
         self.register_buffer("bias", None if bias is None else bias.detach().to(torch.float32).clone())
 
     def _apply(self, fn, recurse=True):
-        """Scales and bias are f32 whatever type the model around them is cast to: only the device follows."""
-        kept = {n: getattr(self, n) for n in ("scale", "bias") if getattr(self, n) is not None}
+        """The weights are 8-bit, scales and bias f32, whatever type the model around them is cast to: only the device follows."""
+        kept = {n: t for n, t in self._buffers.items() if t is not None}
         super()._apply(fn, recurse)
         for name, t in kept.items():
-            moved = getattr(self, name)
-            if moved.dtype != torch.float32:
-                setattr(self, name, t.to(moved.device))
+            moved = self._buffers[name]
+            if moved.dtype != t.dtype:
+                self._buffers[name] = t.to(moved.device)
         return self
 
     @classmethod

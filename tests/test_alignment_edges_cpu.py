@@ -304,3 +304,14 @@ def test_gradient_over_the_padded_buffer_of_the_logits(monkeypatch):
             refused(ValueError, mm.policy_loss_and_grad, buf[:, :, :8], lab, z, adv, dlogits=other)
     refused(ValueError, mm.policy_loss_and_grad, buf.view(-1)[:8].view(1, 1, 8).expand(1, 1, 8), torch.zeros(1, 1, dtype=torch.int64), torch.zeros(1, 1), torch.zeros(1),
             dlogits=buf.view(-1)[2:10].view(1, 1, 8))
+
+
+def test_int8_layer_under_type(monkeypatch):
+    """Module.type casts every buffer, the 8-bit weights among them: the layer keeps its own types."""
+    import multimodalsum_amd as mm
+    Recorder(monkeypatch, {"mmsum_quantize_i8": quantised})
+    lin = mm.Int8Linear(torch.randn(6, 8), torch.randn(6))
+    want = {k: v.clone() for k, v in lin.state_dict().items()}
+    for dtype in (torch.bfloat16, torch.float64):
+        got = lin.type(dtype).state_dict()
+        assert all(torch.equal(got[k], v) and got[k].dtype == v.dtype for k, v in want.items())
